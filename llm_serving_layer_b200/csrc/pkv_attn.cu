@@ -45,6 +45,7 @@ constexpr int DK_PREFETCH = 8;             // pages a CTA prefetches into L2 bef
 #ifndef DK_PRODUCER_SLEEP_NS
 #define DK_PRODUCER_SLEEP_NS 64            // producer back-off while the ring is full
 #endif
+constexpr int DK_SMEM_MAX = 232448;        // shared memory a CTA may have
 constexpr int DK_MAXNREG = 168;            // 10 warps: <= 3 per SM sub-partition x 32 x 168 <= 16K registers
 
 // ---------------------------------------------------------------- workspace
@@ -1104,7 +1105,7 @@ int decode_nst() {
 // the deepest ring (<= the requested depth) whose shared memory fits a CTA
 int decode_nst_for(int n_kv_heads, int groups) {
   int n = decode_nst();
-  while (n > 3 && decode_smem(n_kv_heads, groups, n) > size_t(232448)) --n;
+  while (n > 3 && decode_smem(n_kv_heads, groups, n) > size_t(DK_SMEM_MAX)) --n;
   return n;
 }
 int decode_prefetch() {
@@ -1138,7 +1139,9 @@ int decode_grid_limit(int n_kv_heads) {
   if (!o) {
     auto fn = decode_kernel<T, GROUPS, NST, FUSE>;
     const size_t sm = decode_smem(n_kv_heads, GROUPS, NST);
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sm));
+    // the limit is the function's, not this geometry's: a pool of fewer KV heads
+    // must not lower it under a launch for more
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, DK_SMEM_MAX);
     int v = 0;
     if (e == cudaSuccess)
       e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, fn, 32 * (n_kv_heads + 2), sm);
