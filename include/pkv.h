@@ -193,6 +193,97 @@ PKV_API int pkv_append_attend_rope_planned(const pkv_pool* pool, int32_t layer, 
                                    size_t workspace_bytes, const int64_t* positions, const float* rope_cos,
                                    const float* rope_sin, int64_t rope_max_pos, void* stream);
 
+/* ---- rotating append and the page index -------------------------------------
+ * No counterpart in the reference (its engine rotates q and k with tensor
+ * operations before append_kv, docs/ARCHITECTURE.md:167-172).
+ *
+ * A page index holds, per layer, block and KV head, int8 bounds of the page's
+ * keys: with lo / hi the elementwise minimum / maximum over the page's
+ * block_size keys and scale = max(|lo|, |hi|) * (1/127) (fp32 product),
+ *   codes[layer][block][kv head][0][d] = floor(lo / scale)
+ *   codes[layer][block][kv head][1][d] = ceil(hi / scale)
+ * clamped to [-127, 127] (0 where scale is 0). Only entries of completed pages
+ * are meaningful. */
+typedef struct pkv_page_index {
+  int8_t* codes;  /* device [num_layers][num_blocks][n_kv_heads][2][head_dim], 16-byte aligned */
+  float* scales;  /* device [num_layers][num_blocks][n_kv_heads] */
+} pkv_page_index;
+
+/* Rotates q and k at the tokens' positions and appends, in one launch:
+ * q_out = rotated q, pool slot slot_mapping[t] of layer `layer` = rotated k[t]
+ * and v[t]. q [n_tokens][n_heads][head_dim], k and v [n_tokens][n_kv_heads]
+ * [head_dim] in the pool dtype (PKV_F16, PKV_BF16 or PKV_F32), each token's
+ * row contiguous and token t's row at t * stride elements (so slices of a fused
+ * projection are taken as they are); q_out contiguous. n_heads may be 0 (k and v
+ * only). The first rotary_dim dims of each head are rotated, the rest copied:
+ * pair (i, i + rotary_dim / 2), or (2i, 2i + 1) when `interleaved`, by the
+ * angle whose cosine / sine are rope_cos / rope_sin[positions[t]][i] (fp32
+ * [rope_max_pos][rotary_dim / 2]); rounding as pkv_rope, so the bits are those
+ * of pkv_rope followed by pkv_append_kv. With `index` non-NULL the pages whose
+ * last slot the step fills are indexed (a second launch). A position outside
+ * the tables leaves its token unrotated (PKV_DEV_META_BAD), a slot outside the
+ * pool is skipped (PKV_DEV_SLOT_OOB). */
+PKV_API int pkv_rope_append(const pkv_pool* pool, int32_t layer, const void* q, int64_t q_stride, void* q_out,
+                            int32_t n_heads, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                            const int32_t* slot_mapping, const int64_t* positions, int64_t n_tokens,
+                            const float* rope_cos, const float* rope_sin, int64_t rope_max_pos, int32_t rotary_dim,
+                            int32_t interleaved, const pkv_page_index* index, int32_t* dev_status, void* stream);
+
+/* Index entries, for layer `layer`, of the pages whose last slot is among
+ * slot_mapping[0..n_tokens) (device): after an append that did not index. */
+PKV_API int pkv_page_index_update(const pkv_pool* pool, const pkv_page_index* index, int32_t layer,
+                                  const int32_t* slot_mapping, int64_t n_tokens, int32_t* dev_status, void* stream);
+/* Index entries of blocks block_ids[0..nb) (device) in every layer: after a
+ * copy_block, a swap-in, or for a pool filled before the index existed. */
+PKV_API int pkv_page_index_rebuild(const pkv_pool* pool, const pkv_page_index* index, const int32_t* block_ids,
+                                   int64_t nb, int32_t* dev_status, void* stream);
+
+/* ---- page-sparse attention ----------------------------------------------------
+ * No counterpart in the reference (its attention reads every page). Each query
+ * token and KV head attends over at most `budget` pages of its sequence. With
+ * PKV_SPARSE_SELECT the pages are chosen and written to pages[n_tokens]
+ * [n_kv_heads][budget] (page numbers within the sequence, ascending, -1 past
+ * the end): the first `sink` pages, the last `recent` (the query's own page and
+ * those before it), then the pages of highest score, ties to the lower page:
+ *   qs_g = max_d |q_gd| * (1/127), q8_g = round-half-even(q_g / qs_g)
+ *   I_g = sum_d max(q8_gd * codes[0][d], q8_gd * codes[1][d])
+ *   score = (max over the KV head's query heads g of fl(I_g * qs_g)) * scale
+ * With PKV_SPARSE_ATTEND out = softmax(scale q.K) V over the tokens of the
+ * listed pages up to the query's position (pages read as given when not
+ * selected; entries outside the sequence's pages up to the query's own are
+ * skipped, a page listed twice counts twice, nothing listed gives zeros).
+ * fp16, bf16 or fp32 pools, head_dim up to 256; batch_indices [n_tokens] is
+ * BatchMeta's; max_pages bounds the pages of any sequence of the batch
+ * (PKV_DEV_META_BAD and zeros for a longer one; PKV_ERR_UNSUPPORTED when a
+ * list does not fit in shared memory, about 50000 pages). One launch. */
+#define PKV_SPARSE_SELECT 1
+#define PKV_SPARSE_ATTEND 2
+PKV_API int pkv_attend_sparse(const pkv_pool* pool, const pkv_page_index* index, int32_t layer, int32_t n_heads,
+                              const void* q, void* out, int32_t* pages, float scale, int32_t budget, int32_t sink,
+                              int32_t recent, const pkv_batch* batch, const int32_t* batch_indices,
+                              int32_t max_pages, int32_t mode, void* stream);
+
+/* ---- shared-prefix attention --------------------------------------------------
+ * pkv_attend for a batch whose sequences come in n_groups consecutive groups
+ * (group g: sequences group_indptr[g] .. group_indptr[g+1] - 1), the first
+ * prefix_pages[g] pages of a group's sequences being the same physical pages
+ * (what RadixCache sharing gives): same result, the shared pages read once per
+ * group. prefix_pages[g] * block_size must not exceed any member's
+ * kv_len - query_len; page lists that disagree are computed without sharing and
+ * set PKV_DEV_META_BAD. The plan is made once per step and reused by every
+ * layer with the same batch and workspace (device, 256-byte aligned, of
+ * pkv_shared_workspace_size bytes). decode_hint as pkv_attend: 1 every query
+ * length is 1, 2 none is, 0 unknown. Geometry of the decode kernel only
+ * (PKV_ERR_UNSUPPORTED otherwise: use pkv_attend). */
+PKV_API size_t pkv_shared_workspace_size(const pkv_pool* pool, int32_t n_heads, int32_t n_seqs, int32_t n_tokens,
+                                         int64_t total_pages);
+PKV_API int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* batch, int32_t n_groups,
+                            const int32_t* group_indptr, const int32_t* prefix_pages, void* workspace,
+                            size_t workspace_bytes, void* stream);
+PKV_API int pkv_attend_shared_planned(const pkv_pool* pool, int32_t layer, int32_t n_heads, const void* q, void* out,
+                                      float scale, const pkv_batch* batch, int32_t decode_hint, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
 /* Which kernel pkv_attend_planned runs for a batch of this shape and hint
  * (host only, nothing touches the device): PKV_KERNEL_GENERIC,
  * PKV_KERNEL_DECODE or PKV_KERNEL_PREFILL; -PKV_ERR_ARG for a bad pool. No

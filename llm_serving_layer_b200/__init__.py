@@ -13,6 +13,13 @@ Drop-ins behind the reference's own interfaces:
   and a vectorised host assembler;
 * ``DeviceBlockTables`` — block tables kept on the device and each step's
   ``BatchMeta`` assembled there, replacing the engine's ``build_batch_meta``;
+* ``SharedPrefix`` / ``B200PagedBackend.attend_shared`` — attention of a batch
+  whose sequences share leading pages (what the radix cache's block tables
+  give), the shared pages read once;
+* ``PageIndex`` / ``B200PagedBackend.attend_sparse`` — attention of each query
+  over the pages a score of the page index selects;
+* ``B200PagedBackend.rope_append`` — rotary embedding and KV-append of any step
+  in one launch, from the slices of the fused projection;
 * ``BlockAllocator`` / ``RadixCache`` / ``attach_prefix`` (``radix``) — the
   block manager and prefix cache the scheduler drives, with eviction in
   O(log nodes) and an O(1) invariant check, replacing
@@ -26,9 +33,11 @@ All compute runs in ``_lib/libpkv.so`` (hand-written CUDA, C ABI in
 """
 
 from .backend import B200PagedBackend
+from .index import PageIndex
 from .meta import AttentionBackend, BatchMeta, build_meta
 from .radix import BlockAllocator, RadixCache, attach_prefix
 from .sampling import TokenReadback, sample_greedy
+from .shared import SharedPrefix
 from .swap import B200SwapSpace, SwapHandle, SwapSpaceFull
 from .tables import DeviceBlockTables
 
@@ -44,6 +53,8 @@ __all__ = [
     "BlockAllocator",
     "RadixCache",
     "attach_prefix",
+    "SharedPrefix",
+    "PageIndex",
     "sample_greedy",
     "TokenReadback",
 ]

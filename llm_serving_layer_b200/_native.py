@@ -19,6 +19,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libpkv.so"
 PKV_OK, PKV_ERR_ARG, PKV_ERR_UNSUPPORTED, PKV_ERR_CUDA, PKV_ERR_DEVICE = 0, 1, 2, 3, 4
 PKV_KERNEL_GENERIC, PKV_KERNEL_DECODE, PKV_KERNEL_PREFILL = 0, 1, 2
 KERNEL_NAMES = {PKV_KERNEL_GENERIC: "generic", PKV_KERNEL_DECODE: "decode", PKV_KERNEL_PREFILL: "prefill"}
+SPARSE_SELECT, SPARSE_ATTEND = 1, 2
 DEV_SLOT_OOB, DEV_META_BAD, DEV_QLEN_BAD, DEV_WAIT_TIMEOUT, DEV_WORKSPACE = 0x1, 0x2, 0x4, 0x8, 0x10
 
 DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2, torch.float64: 3}
@@ -51,10 +52,15 @@ class MetaOutDesc(ctypes.Structure):
                 ("seqs_cap", c_i32), ("reserved", c_i32), ("tokens_cap", c_i64), ("pages_cap", c_i64)]
 
 
+class PageIndexDesc(ctypes.Structure):
+    _fields_ = [("codes", c_vp), ("scales", c_vp)]
+
+
 P_POOL = ctypes.POINTER(PoolDesc)
 P_BATCH = ctypes.POINTER(BatchDesc)
 P_TABLES = ctypes.POINTER(BlockTablesDesc)
 P_META_OUT = ctypes.POINTER(MetaOutDesc)
+P_INDEX = ctypes.POINTER(PageIndexDesc)
 
 # name -> (restype, argtypes); every symbol include/pkv.h declares
 SIGNATURES = {
@@ -72,6 +78,16 @@ SIGNATURES = {
                          c_vp]),
     "pkv_append_attend_rope_planned": (c_i32, [P_POOL, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_float, P_BATCH,
                                                c_i32, c_vp, c_size, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "pkv_rope_append": (c_i32, [P_POOL, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64,
+                                c_vp, c_vp, c_i64, c_i32, c_i32, P_INDEX, c_vp, c_vp]),
+    "pkv_page_index_update": (c_i32, [P_POOL, P_INDEX, c_i32, c_vp, c_i64, c_vp, c_vp]),
+    "pkv_page_index_rebuild": (c_i32, [P_POOL, P_INDEX, c_vp, c_i64, c_vp, c_vp]),
+    "pkv_attend_sparse": (c_i32, [P_POOL, P_INDEX, c_i32, c_i32, c_vp, c_vp, c_vp, c_float, c_i32, c_i32, c_i32,
+                                  P_BATCH, c_vp, c_i32, c_i32, c_vp]),
+    "pkv_shared_workspace_size": (c_size, [P_POOL, c_i32, c_i32, c_i32, c_i64]),
+    "pkv_plan_shared": (c_i32, [P_POOL, c_i32, P_BATCH, c_i32, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "pkv_attend_shared_planned": (c_i32, [P_POOL, c_i32, c_i32, c_vp, c_vp, c_float, P_BATCH, c_i32, c_vp, c_size,
+                                          c_vp]),
     "pkv_attend_decode_noalloc": (c_i32, [P_POOL, c_i32, c_i32, c_vp, c_vp, c_float, P_BATCH, c_vp]),
     "pkv_wait_probe": (c_i32, [c_vp, c_vp, c_vp, c_vp]),
     "pkv_sample_greedy": (c_i32, [c_i32, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),

@@ -26,7 +26,23 @@ import torch
 
 from . import _native as N
 
-__all__ = ["B200PagedBackend"]
+__all__ = ["B200PagedBackend", "SharedPlan", "SparsePlan"]
+
+
+class SharedPlan:
+    """One step of ``attend_shared``: made by ``B200PagedBackend.plan_shared``,
+    used by every layer of the step. Holds the step's tables and a workspace of
+    its own (``workspace`` may be passed on to the next step's plan)."""
+
+    __slots__ = ("meta", "n_tokens", "hint", "batch", "batch_ref", "tensors", "workspace", "ws_ptr", "ws_bytes")
+
+
+class SparsePlan:
+    """One step of ``attend_sparse``: made by ``B200PagedBackend.plan_sparse``,
+    used by every layer of the step."""
+
+    __slots__ = ("index", "budget", "sink", "recent", "max_pages", "n_tokens", "batch", "batch_ref", "tensors",
+                 "batch_indices_ptr")
 
 
 class B200PagedBackend:
@@ -286,6 +302,88 @@ class B200PagedBackend:
             N.raw_stream(self._dev_index)), "rope")
         return qo, ko
 
+    def rope_append(self, layer_idx: int, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, meta: Any,
+                    rope: tuple[torch.Tensor, torch.Tensor], *, interleaved: bool = False, index: Any = None,
+                    q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Rotates q ``(T, n_heads, head_dim)`` and k ``(T, n_kv_heads, head_dim)``
+        at ``meta.positions`` and appends the rotated k and v at
+        ``meta.slot_mapping``, in one launch for any step; returns the rotated q
+        (``q_out`` or a new tensor; None when q is None). q, k and v may be
+        slices of the fused projection: any stride between tokens, each token's
+        heads contiguous (other layouts are copied first).
+
+        ``rope = (cos, sin)``: fp32 ``[max_pos, rotary_dim // 2]`` on this
+        device, ``rotary_dim <= head_dim``; the dims after rotary_dim pass
+        through. Pair (i, i + rotary_dim // 2) is turned, or (2i, 2i + 1) when
+        ``interleaved``. Same bits as ``rope`` followed by ``append_kv``.
+        ``index`` (a ``PageIndex`` of this backend): the entries of the pages
+        this step completes are written too. fp16, bf16 or fp32 pools."""
+        cos, sin = self._rope_tables(rope, None)
+        rotary = 2 * cos.shape[1]
+        if rotary > self.head_dim:
+            raise ValueError(f"the rope tables turn {rotary} dims of heads of {self.head_dim}")
+        self._check_layer(layer_idx)
+        if getattr(meta, "slot_mapping", None) is None or getattr(meta, "positions", None) is None:
+            raise ValueError("rope_append requires meta.slot_mapping and meta.positions")
+        tokens = k.shape[0]
+        if k.shape != (tokens, self.n_kv_heads, self.head_dim):
+            raise ValueError(f"k has shape {tuple(k.shape)}, expected ({tokens}, {self.n_kv_heads}, {self.head_dim})")
+        if v.shape != k.shape:
+            raise ValueError(f"v shape {tuple(v.shape)} != k shape {tuple(k.shape)}")
+        if q is not None and q.shape != (tokens, self.n_heads, self.head_dim):
+            raise ValueError(f"q has shape {tuple(q.shape)}, expected ({tokens}, {self.n_heads}, {self.head_dim})")
+        for name in ("slot_mapping", "positions"):
+            if getattr(meta, name).shape != (tokens,):
+                raise ValueError(f"{name} has {getattr(meta, name).shape[0]} entries but {tokens} tokens were supplied")
+        if index is not None and index.backend is not self:
+            raise ValueError("index belongs to another backend")
+        k, v = self._rows(k), self._rows(v)
+        if q is not None:
+            q = self._rows(q)
+            if q_out is None:
+                q_out = torch.empty((tokens, self.n_heads, self.head_dim), dtype=self.dtype, device=self.device)
+            elif (q_out.shape != q.shape or q_out.dtype != self.dtype or not q_out.is_cuda
+                  or q_out.get_device() != self._dev_index or not q_out.is_contiguous()):
+                raise ValueError(f"q_out must be a contiguous {tuple(q.shape)} {self.dtype} tensor on {self.device}")
+            elif _overlap(q_out, q) and not (q_out.data_ptr() == q.data_ptr() and q.is_contiguous()):
+                raise ValueError("q_out overlaps q without being q")
+        elif q_out is not None:
+            raise ValueError("q_out given without q")
+        if tokens == 0:
+            return q_out
+        slots, pos = self._i32(meta.slot_mapping), self._own(meta.positions, torch.int64)
+        N.check(self._lib.pkv_rope_append(
+            self._pdesc, layer_idx, N.ptr(q), 0 if q is None else q.stride(0), N.ptr(q_out),
+            0 if q is None else self.n_heads, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slots.data_ptr(),
+            pos.data_ptr(), tokens, cos.data_ptr(), sin.data_ptr(), cos.shape[0], rotary, int(interleaved),
+            None if index is None else index._pdesc, self._status_ptr, N.raw_stream(self._dev_index)), "rope_append")
+        return q_out
+
+    def _rope_tables(self, rope, half):
+        try:
+            cos, sin = rope
+        except (TypeError, ValueError):
+            raise ValueError("rope must be a (cos, sin) pair of tensors") from None
+        for t, name in ((cos, "cos"), (sin, "sin")):
+            if (not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] < 1 or t.shape[1] < 1
+                    or (half is not None and t.shape[1] != half) or t.dtype != torch.float32 or not t.is_cuda
+                    or t.get_device() != self._dev_index or not t.is_contiguous()):
+                raise ValueError(f"rope {name} must be a contiguous float32 [max_pos, dims] tensor on {self.device}")
+        if cos.shape != sin.shape:
+            raise ValueError(f"rope cos {tuple(cos.shape)} and sin {tuple(sin.shape)} differ in shape")
+        return cos, sin
+
+    def _rows(self, t: torch.Tensor) -> torch.Tensor:
+        """t on this device in the pool dtype with each token's row contiguous
+        (no op for slices of a fused projection)."""
+        if (t.is_cuda and t.dtype == self.dtype and t.get_device() == self._dev_index and t.stride(2) == 1
+                and (t.stride(1) == t.shape[2] or t.shape[1] == 1)
+                and (t.stride(0) >= t.shape[1] * t.shape[2] or t.shape[0] <= 1)):
+            if t.shape[0] <= 1 and t.stride(0) < t.shape[1] * t.shape[2]:
+                return t.contiguous()
+            return t
+        return t.to(device=self.device, dtype=self.dtype).contiguous()
+
     def _rope_args(self, rope, meta):
         try:
             cos, sin = rope
@@ -368,6 +466,188 @@ class B200PagedBackend:
             st["batch_ref"], st["hint"], st["ws_ptr"], st["ws_bytes"],
             N.raw_stream(self._dev_index)), "attend")
         return out
+
+    # -- attention of a batch that shares leading pages ---------------------------
+    def plan_shared(self, meta: Any, shared: Any, *, workspace: torch.Tensor | None = None) -> SharedPlan:
+        """Prepare a step whose sequences come in families that share leading
+        pages (``shared``: a ``SharedPrefix``). The returned plan serves every
+        layer's ``attend_shared``; its tables are copies, so ``meta`` may be
+        reused. ``workspace``: a finished plan's, taken over when large enough.
+        A family whose page lists disagree, or whose shared pages reach past the
+        tokens before the step, raises ``ValueError`` with ``validate="host"``;
+        with ``"device"`` it is computed without sharing and recorded for
+        ``check_status``."""
+        n = int(meta.query_lens.shape[0])
+        if shared.n_seqs != n:
+            raise ValueError(f"the groups hold {shared.n_seqs} sequences but the batch has {n}")
+        plan = SharedPlan()
+        self._plan_batch(plan, meta)
+        mql, mnql = getattr(meta, "max_query_len", None), getattr(meta, "min_query_len", None)
+        plan.hint = 1 if plan.n_tokens == n and mql == 1 else (2 if mnql is not None and int(mnql) > 1 else 0)
+        plan.meta = None
+        if self.validate == "host":
+            decode, hint = self._host_validate(meta, n, int(meta.kv_indices.shape[0]))
+            plan.hint = hint
+            self._validate_shared(meta, shared)
+        bounds = [0]
+        for size in shared.group_sizes:
+            bounds.append(bounds[-1] + size)
+        groups = torch.tensor(bounds + shared.prefix_pages, dtype=torch.int32).to(self.device)
+        plan.tensors["groups"] = groups
+        b = plan.batch
+        need = int(self._lib.pkv_shared_workspace_size(self._pdesc, self.n_heads, n, plan.n_tokens, b.total_pages))
+        if workspace is None or workspace.numel() < need or workspace.device != self.device:
+            workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        plan.workspace, plan.ws_ptr, plan.ws_bytes = workspace, workspace.data_ptr(), workspace.numel()
+        rc = self._lib.pkv_plan_shared(
+            self._pdesc, self.n_heads, plan.batch_ref, len(shared.group_sizes), groups.data_ptr(),
+            groups.data_ptr() + 4 * len(bounds), plan.ws_ptr, plan.ws_bytes, N.stream_ptr(self.device))
+        if rc == N.PKV_ERR_UNSUPPORTED:  # other geometries: every sequence by itself, in attend
+            plan.meta, plan.workspace, plan.ws_ptr, plan.ws_bytes = meta, None, None, 0
+            return plan
+        N.check(rc, "plan_shared")
+        return plan
+
+    def attend_shared(self, q: torch.Tensor, layer_idx: int, scale: float, plan: SharedPlan, *,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+        """``attend`` for a step planned by ``plan_shared``: same result (to
+        rounding), the pages a family shares read once for all its sequences.
+        Geometries outside the tensor-core kernels' (fp16 / bf16, head_dim 64,
+        16-token pages, up to 8 KV heads, 1/2/4/8 query heads per KV head) run
+        ``attend`` itself."""
+        if plan.meta is not None:
+            return self.attend(q, layer_idx, scale, plan.meta, out=out)
+        self._check_layer(layer_idx)
+        self._check_q(q, plan.n_tokens)
+        q = self._own(q, self.dtype)
+        out = self._out(q, out)
+        if plan.n_tokens == 0:
+            return out
+        N.check(self._lib.pkv_attend_shared_planned(
+            self._pdesc, layer_idx, self.n_heads, q.data_ptr(), out.data_ptr(), float(scale), plan.batch_ref,
+            plan.hint, plan.ws_ptr, plan.ws_bytes, N.raw_stream(self._dev_index)), "attend_shared")
+        self.n_runs += 1
+        self.last_kernel = "shared"
+        return out
+
+    def _validate_shared(self, meta: Any, shared: Any) -> None:
+        ip, ix = meta.kv_indptr.tolist(), meta.kv_indices.tolist()
+        ql, lp = meta.query_lens.tolist(), meta.kv_last_page_len.tolist()
+        s = 0
+        for g, (size, pages) in enumerate(zip(shared.group_sizes, shared.prefix_pages)):
+            lead = ix[ip[s]:ip[s] + pages]
+            for i in range(s, s + size) if pages else ():
+                kv = (ip[i + 1] - ip[i] - 1) * self.block_size + lp[i]
+                if pages * self.block_size > kv - ql[i]:
+                    raise ValueError(f"group {g}: {pages} shared pages reach past the {kv - ql[i]} tokens sequence "
+                                     f"{i} held before this step")
+                if ix[ip[i]:ip[i] + pages] != lead:
+                    raise ValueError(f"group {g}: sequence {i} does not start with the group's {pages} shared pages")
+            s += size
+
+    # -- page-sparse attention ------------------------------------------------------
+    def plan_sparse(self, meta: Any, index: Any, budget: int, *, sink: int = 1, recent: int = 1,
+                    max_pages: int | None = None) -> SparsePlan:
+        """Prepare a step of page-sparse attention: each query and KV head
+        attends over at most ``budget`` pages — the first ``sink``, the last
+        ``recent`` (its own page included) and the highest scoring others.
+        ``max_pages``: a bound on the pages of any sequence of the batch; without
+        it the longest is read back from the device once. The plan serves every
+        layer of the step; its tables are copies, so ``meta`` may be reused."""
+        if index.backend is not self:
+            raise ValueError("index belongs to another backend")
+        budget, sink, recent = int(budget), int(sink), int(recent)
+        if budget <= 0 or sink < 0 or recent < 1 or sink + recent > budget:
+            raise ValueError(f"budget={budget}, sink={sink}, recent={recent}: sink >= 0, recent >= 1 and "
+                             "sink + recent <= budget are needed")
+        plan = SparsePlan()
+        self._plan_batch(plan, meta)
+        if self.validate == "host":
+            self._host_validate(meta, int(meta.query_lens.shape[0]), int(meta.kv_indices.shape[0]))
+        if getattr(meta, "batch_indices", None) is None or meta.batch_indices.shape != (plan.n_tokens,):
+            raise ValueError(f"plan_sparse needs meta.batch_indices with {plan.n_tokens} entries")
+        plan.tensors["bi"] = self._copy_i32(meta.batch_indices)
+        plan.batch_indices_ptr = plan.tensors["bi"].data_ptr()
+        if max_pages is None:
+            ip = plan.tensors["ip"]
+            max_pages = int((ip[1:] - ip[:-1]).max())
+        if max_pages <= 0:
+            raise ValueError(f"max_pages must be positive, got {max_pages}")
+        plan.index, plan.budget, plan.sink, plan.recent = index, budget, sink, recent
+        plan.max_pages = int(max_pages)
+        return plan
+
+    def attend_sparse(self, q: torch.Tensor, layer_idx: int, scale: float, plan: SparsePlan, *,
+                      out: torch.Tensor | None = None,
+                      pages: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Selects each query's pages with the plan's index and attends over
+        them, in one launch. Returns ``(out, pages)``: out as ``attend``'s,
+        pages int32 ``(tokens, n_kv_heads, budget)`` — page numbers within the
+        sequence, ascending, -1 past the end (``pages``: a tensor to write)."""
+        return self._sparse(q, layer_idx, scale, plan, out, pages, N.SPARSE_SELECT | N.SPARSE_ATTEND)
+
+    def select_pages(self, q: torch.Tensor, layer_idx: int, plan: SparsePlan, *,
+                     pages: torch.Tensor | None = None) -> torch.Tensor:
+        """The pages ``attend_sparse`` would read, without the attention."""
+        return self._sparse(q, layer_idx, 1.0, plan, None, pages, N.SPARSE_SELECT)[1]
+
+    def attend_pages(self, q: torch.Tensor, layer_idx: int, scale: float, plan: SparsePlan, pages: torch.Tensor, *,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention over given pages: ``pages`` int32 ``(tokens, n_kv_heads,
+        budget)`` as ``select_pages`` returns (another layer's or the caller's
+        own). Entries that are negative or past the query's own page are skipped,
+        a page listed twice counts twice, a row listing nothing gives zeros."""
+        return self._sparse(q, layer_idx, scale, plan, out, pages, N.SPARSE_ATTEND)[0]
+
+    def _sparse(self, q, layer_idx, scale, plan, out, pages, mode):
+        self._check_layer(layer_idx)
+        self._check_q(q, plan.n_tokens)
+        q = self._own(q, self.dtype)
+        shape = (plan.n_tokens, self.n_kv_heads, plan.budget)
+        if pages is None and mode & N.SPARSE_SELECT:
+            pages = torch.empty(shape, dtype=torch.int32, device=self.device)
+        elif (pages is None or pages.shape != shape or pages.dtype != torch.int32 or not pages.is_cuda
+              or pages.get_device() != self._dev_index or not pages.is_contiguous()):
+            raise ValueError(f"pages must be a contiguous int32 {shape} tensor on {self.device}")
+        if mode & N.SPARSE_ATTEND:
+            out = self._out(q, out)
+        if plan.n_tokens == 0:
+            return out, pages
+        N.check(self._lib.pkv_attend_sparse(
+            self._pdesc, plan.index._pdesc, layer_idx, self.n_heads, q.data_ptr(), N.ptr(out), pages.data_ptr(),
+            float(scale), plan.budget, plan.sink, plan.recent, plan.batch_ref, plan.batch_indices_ptr, plan.max_pages,
+            mode, N.raw_stream(self._dev_index)), "attend_sparse")
+        if mode & N.SPARSE_ATTEND:
+            self.n_runs += 1
+            self.last_kernel = "sparse"
+        return out, pages
+
+    def _plan_batch(self, plan: Any, meta: Any) -> None:
+        """The step's device tables and batch descriptor of a plan object."""
+        n = int(meta.query_lens.shape[0])
+        if n <= 0:
+            raise ValueError("BatchMeta has no sequences")
+        plan.n_tokens = int(meta.positions.shape[0]) if getattr(meta, "positions", None) is not None \
+            else int(meta.batch_indices.shape[0])
+        t = plan.tensors = {
+            "cu": self._copy_i32(meta.cu_query_lens),
+            "kl": self._copy_i32(meta.kv_lens) if getattr(meta, "kv_lens", None) is not None else None,
+            "ip": self._copy_i32(meta.kv_indptr),
+            "ix": self._copy_i32(meta.kv_indices),
+            "lp": self._copy_i32(meta.kv_last_page_len),
+        }
+        total_pages = int(meta.kv_indices.shape[0])
+        plan.batch = N.BatchDesc(
+            n, plan.n_tokens, total_pages, t["cu"].data_ptr(), N.ptr(t["kl"]), t["ip"].data_ptr(),
+            t["ix"].data_ptr() if total_pages else None, t["lp"].data_ptr(), self._status_ptr)
+        plan.batch_ref = ctypes.byref(plan.batch)
+
+    def _check_q(self, q: torch.Tensor, tokens: int) -> None:
+        if q.shape != (tokens, self.n_heads, self.head_dim):
+            raise ValueError(f"q has shape {tuple(q.shape)}, expected ({tokens}, {self.n_heads}, {self.head_dim})")
+
+    def _copy_i32(self, t: torch.Tensor) -> torch.Tensor:
+        return t.to(device=self.device, dtype=torch.int32, copy=True).contiguous()
 
     # -- per-step plan -----------------------------------------------------------
 
@@ -547,3 +827,13 @@ class B200PagedBackend:
             f"block_size={self.block_size}, kv_heads={self.n_kv_heads}, heads={self.n_heads}, "
             f"head_dim={self.head_dim}, dtype={self.dtype}, device={self.device}, pool={mib:.1f} MiB)"
         )
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        n = 1 + sum((d - 1) * st for d, st in zip(t.shape, t.stride())) if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1

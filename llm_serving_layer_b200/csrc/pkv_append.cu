@@ -1,0 +1,410 @@
+// pkv_append.cu — the way into the paged cache: rotary embedding and KV-append
+// of any step in one launch, and the page index (int8 key bounds per page and
+// KV head) that page-sparse attention scores pages with.
+//
+//   rope_append_kernel   q' = R(pos) q -> q_out, k' = R(pos) k and v -> their
+//                        slots. R turns pair i of each head by the angle whose
+//                        cosine / sine are the tables' row `pos`, entry i; the
+//                        pair is (i, i + rot/2), or (2i, 2i + 1) interleaved;
+//                        dims rot.. of a head pass through. Products are
+//                        rounded to fp32 before the difference / sum
+//                        (rope_pair), then once to the pool dtype: the bits of
+//                        pkv_rope followed by pkv_append_kv.
+//   page_index_kernel    bounds of whole pages: lo / hi = elementwise min / max
+//                        of the page's keys, scale = max(|lo|, |hi|) / 127,
+//                        codes floor(lo / scale), ceil(hi / scale).
+//
+// Both move each byte once and do a few operations on it: HBM bound.
+#include <algorithm>
+#include <type_traits>
+
+#include "pkv_common.cuh"
+
+namespace pkv {
+namespace {
+
+struct RopeAppendArgs {
+  const char* q;
+  const char* k;
+  const char* v;
+  char* q_out;
+  char* k_slab;
+  char* v_slab;
+  const int32_t* slots;
+  const int64_t* positions;
+  const float* cs;
+  const float* sn;
+  int32_t* st;
+  int64_t q_stride, k_stride, v_stride, qo_stride;  // bytes between tokens
+  int64_t n_tokens, n_slots, max_pos;
+  int hq, hkv, d, half;  // half = rotated pairs per head
+  int wpt;               // warps per token
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack_vec(const uint4& u, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  } else {
+    const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y), c = unpack2<T>(u.z), d = unpack2<T>(u.w);
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_vec(const float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  else
+    return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+}
+
+// VE elements per unit (16 bytes, or 1 where alignment or sizes do not allow
+// vectors). A token's units: for each rotated head VE pairs at a time, the
+// pass-through dims, then v; wpt warps share a token's units.
+template <typename T, bool VECTOR, bool INTER>
+__global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a) {
+  constexpr int VE = VECTOR ? 16 / int(sizeof(T)) : 1;
+  pdl_trigger();
+  pdl_wait();  // q, k, v, positions and slots may come from the kernels just before
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int64_t t = warp / a.wpt;
+  if (t >= a.n_tokens) return;
+  const int u0 = int(warp % a.wpt) * 32 + lane, du = a.wpt * 32;
+  const int64_t pos = a.positions[t], slot = a.slots[t];
+  const bool turn = pos >= 0 && pos < a.max_pos;
+  const bool store = slot >= 0 && slot < a.n_slots;
+  if (u0 == 0) {
+    if (!turn) flag(a.st, PKV_DEV_META_BAD);
+    if (!store) flag(a.st, PKV_DEV_SLOT_OOB);
+  }
+  const int d = a.d, half = a.half;
+  const int64_t row = int64_t(a.hkv) * d * sizeof(T);
+  const T* q = reinterpret_cast<const T*>(a.q + t * a.q_stride);
+  const T* k = reinterpret_cast<const T*>(a.k + t * a.k_stride);
+  const T* v = reinterpret_cast<const T*>(a.v + t * a.v_stride);
+  T* qo = reinterpret_cast<T*>(a.q_out + t * a.qo_stride);
+  T* ko = reinterpret_cast<T*>(a.k_slab + slot * row);
+  T* vo = reinterpret_cast<T*>(a.v_slab + slot * row);
+  const float* cs = a.cs + (turn ? pos : 0) * half;
+  const float* sn = a.sn + (turn ? pos : 0) * half;
+  // the head's source and destination (NULL: a key whose slot is outside the pool)
+  auto head = [&](int hh, const T*& x, T*& y) {
+    const bool isq = hh < a.hq;
+    x = isq ? q + hh * d : k + (hh - a.hq) * d;
+    y = isq ? qo + hh * d : (store ? ko + (hh - a.hq) * d : nullptr);
+  };
+
+  const int cols = half / VE;  // units of VE pairs per head (host: half % VE == 0)
+  const int n_rot = (a.hq + a.hkv) * cols;
+#pragma unroll 2
+  for (int u = u0; u < n_rot; u += du) {
+    const int hh = u / cols, i = (u - hh * cols) * VE;
+    const T* x;
+    T* y;
+    head(hh, x, y);
+    if constexpr (VECTOR) {
+      // half-split: elements i.. and half + i..; interleaved: the 2 VE elements from 2 i
+      const int e0 = INTER ? 2 * i : i, e1 = INTER ? 2 * i + VE : half + i;
+      const uint4 xa = *reinterpret_cast<const uint4*>(x + e0), xb = *reinterpret_cast<const uint4*>(x + e1);
+      float c[VE], s[VE], p[VE], r[VE];
+#pragma unroll
+      for (int e = 0; e < VE; e += 4) {
+        const float4 cv = __ldg(reinterpret_cast<const float4*>(cs + i + e));
+        const float4 sv = __ldg(reinterpret_cast<const float4*>(sn + i + e));
+        c[e] = cv.x; c[e + 1] = cv.y; c[e + 2] = cv.z; c[e + 3] = cv.w;
+        s[e] = sv.x; s[e + 1] = sv.y; s[e + 2] = sv.z; s[e + 3] = sv.w;
+      }
+      unpack_vec<T>(xa, p);
+      unpack_vec<T>(xb, r);
+      if (turn) {
+        if constexpr (INTER) {
+#pragma unroll
+          for (int e = 0; e < VE; e += 2) rope_pair(p[e], p[e + 1], c[e / 2], s[e / 2]);
+#pragma unroll
+          for (int e = 0; e < VE; e += 2) rope_pair(r[e], r[e + 1], c[VE / 2 + e / 2], s[VE / 2 + e / 2]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) rope_pair(p[e], r[e], c[e], s[e]);
+        }
+      }
+      if (y) {
+        *reinterpret_cast<uint4*>(y + e0) = pack_vec<T>(p);
+        *reinterpret_cast<uint4*>(y + e1) = pack_vec<T>(r);
+      }
+    } else {
+      const int e0 = INTER ? 2 * i : i, e1 = INTER ? 2 * i + 1 : half + i;
+      float p = to_f<T>(x[e0]), r = to_f<T>(x[e1]);
+      if (turn) rope_pair(p, r, cs[i], sn[i]);
+      if (y) {
+        y[e0] = from_f<T>(p);
+        y[e1] = from_f<T>(r);
+      }
+    }
+  }
+  using V = typename std::conditional<VECTOR, uint4, T>::type;
+  const int pass = (d - 2 * half) / VE;  // pass-through vectors per head
+  for (int u = u0; u < (a.hq + a.hkv) * pass; u += du) {
+    const int hh = u / pass, e = 2 * half + (u - hh * pass) * VE;
+    const T* x;
+    T* y;
+    head(hh, x, y);
+    const V w = *reinterpret_cast<const V*>(x + e);
+    if (y) *reinterpret_cast<V*>(y + e) = w;
+  }
+  if (store) {
+    const V* src = reinterpret_cast<const V*>(v);
+    V* dst = reinterpret_cast<V*>(vo);
+    const int n = a.hkv * d / VE;
+#pragma unroll 2
+    for (int u = u0; u < n; u += du) dst[u] = src[u];
+  }
+}
+
+// ---------------------------------------------------------------- page index
+struct IndexArgs {
+  const char* k_base;   // layer 0's K slab
+  int8_t* codes;        // [layers][num_blocks][n_kv][2][d]
+  float* scales;        // [layers][num_blocks][n_kv]
+  const int32_t* ids;   // slots of the step's tokens (layer >= 0) or block ids (layer < 0: every layer)
+  int32_t* st;
+  int64_t n, num_blocks, slab_bytes;
+  int layer, num_layers, hkv, d, page;
+};
+
+constexpr int IX_MAX_EPL = 8;  // head_dim <= 256
+
+// One warp: index entry of KV head h of block `blk`, layer `layer`.
+template <typename T>
+__device__ __forceinline__ void index_entry(const IndexArgs& a, int layer, int64_t blk, int h, int lane) {
+  const int d = a.d;
+  const T* k = reinterpret_cast<const T*>(a.k_base + int64_t(2) * layer * a.slab_bytes) +
+               (blk * a.page * a.hkv + h) * d;
+  const int64_t row = int64_t(a.hkv) * d;
+  float lo[IX_MAX_EPL], hi[IX_MAX_EPL];
+#pragma unroll
+  for (int i = 0; i < IX_MAX_EPL; ++i) {
+    lo[i] = INFINITY;
+    hi[i] = -INFINITY;
+  }
+#pragma unroll 4
+  for (int r = 0; r < a.page; ++r) {
+#pragma unroll
+    for (int i = 0; i < IX_MAX_EPL; ++i) {
+      const int e = lane + 32 * i;
+      if (e < d) {
+        const float x = to_f<T>(k[r * row + e]);
+        lo[i] = fminf(lo[i], x);
+        hi[i] = fmaxf(hi[i], x);
+      }
+    }
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < IX_MAX_EPL; ++i)
+    if (lane + 32 * i < d) top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+#pragma unroll
+  for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const float scale = __fmul_rn(top, 1.0f / 127.0f);
+  const int64_t entry = (int64_t(layer) * a.num_blocks + blk) * a.hkv + h;
+  int8_t* c = a.codes + entry * 2 * d;
+#pragma unroll
+  for (int i = 0; i < IX_MAX_EPL; ++i) {
+    const int e = lane + 32 * i;
+    if (e < d) {
+      // scale 0 (or not a number): the codes are 0
+      const float x = scale > 0.f ? floorf(__fdiv_rn(lo[i], scale)) : 0.f;
+      const float y = scale > 0.f ? ceilf(__fdiv_rn(hi[i], scale)) : 0.f;
+      c[e] = int8_t(fminf(fmaxf(x, -127.f), 127.f));
+      c[d + e] = int8_t(fminf(fmaxf(y, -127.f), 127.f));
+    }
+  }
+  if (lane == 0) a.scales[entry] = scale;
+}
+
+// layer >= 0: one CTA per 32 tokens; the pages whose last slot one of them
+// fills are indexed, its warps taking the KV heads. layer < 0: one CTA per
+// (block, layer).
+template <typename T>
+__global__ void __launch_bounds__(256) page_index_kernel(const IndexArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  pdl_trigger();
+  pdl_wait();  // the keys were written by the append just before
+  if (a.layer < 0) {
+    const int64_t i = blockIdx.x / a.num_layers;
+    const int layer = int(blockIdx.x % a.num_layers);
+    const int64_t blk = a.ids[i];
+    if (blk < 0 || blk >= a.num_blocks) {
+      if (threadIdx.x == 0 && layer == 0) flag(a.st, PKV_DEV_SLOT_OOB);
+      return;
+    }
+    for (int h = warp; h < a.hkv; h += nw) index_entry<T>(a, layer, blk, h, lane);
+    return;
+  }
+  const int64_t t = int64_t(blockIdx.x) * 32 + lane;
+  const int64_t slot = t < a.n ? a.ids[t] : -1;
+  // a slot outside the pool was flagged by the append
+  const bool done = slot >= 0 && slot < a.num_blocks * a.page && slot % a.page == a.page - 1;
+  uint32_t todo = __ballot_sync(0xffffffffu, done);
+  while (todo) {
+    const int l = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const int64_t blk = __shfl_sync(0xffffffffu, slot, l) / a.page;
+    for (int h = warp; h < a.hkv; h += nw) index_entry<T>(a, a.layer, blk, h, lane);
+  }
+}
+
+template <typename T>
+int launch_index(const IndexArgs& a, int64_t grid, cudaStream_t s) {
+  PKV_CUDA_RET(launch_kernel(page_index_kernel<T>, dim3(unsigned(grid)), dim3(unsigned(32 * std::min(a.hkv, 8))), 0, s,
+                             true, a));
+  return PKV_OK;
+}
+
+int run_index(const pkv_pool& p, const pkv_page_index* ix, int layer, const int32_t* ids, int64_t n, int32_t* st,
+              cudaStream_t s) {
+  IndexArgs a;
+  a.k_base = static_cast<const char*>(p.base);
+  a.codes = ix->codes;
+  a.scales = ix->scales;
+  a.ids = ids;
+  a.st = st;
+  a.n = n;
+  a.num_blocks = p.num_blocks;
+  a.slab_bytes = slab_bytes(p);
+  a.layer = layer;
+  a.num_layers = p.num_layers;
+  a.hkv = p.n_kv_heads;
+  a.d = p.head_dim;
+  a.page = p.block_size;
+  const int64_t grid = layer >= 0 ? (n + 31) / 32 : n * p.num_layers;
+  if (grid >= (int64_t(1) << 31)) return fail(PKV_ERR_ARG, "too many blocks for one call");
+  switch (p.dtype) {
+    case PKV_F16: return launch_index<__half>(a, grid, s);
+    case PKV_BF16: return launch_index<__nv_bfloat16>(a, grid, s);
+    default: return launch_index<float>(a, grid, s);
+  }
+}
+
+template <typename T>
+int launch_rope_append(const RopeAppendArgs& a, bool vec, bool inter, cudaStream_t s) {
+  const int64_t warps = a.n_tokens * a.wpt;
+  const int64_t grid = (warps * 32 + 255) / 256;
+  if (grid >= (int64_t(1) << 31)) return fail(PKV_ERR_ARG, "too many tokens for one call");
+  auto kern = vec ? (inter ? rope_append_kernel<T, true, true> : rope_append_kernel<T, true, false>)
+                  : (inter ? rope_append_kernel<T, false, true> : rope_append_kernel<T, false, false>);
+  PKV_CUDA_RET(launch_kernel(kern, dim3(unsigned(grid)), dim3(256), 0, s, true, a));
+  return PKV_OK;
+}
+
+}  // namespace
+
+int check_index(const pkv_pool& p, const pkv_page_index* ix) {
+  if (!ix || !ix->codes || !ix->scales) return fail(PKV_ERR_ARG, "page index codes and scales must be non-NULL");
+  if (reinterpret_cast<uintptr_t>(ix->codes) & 15) return fail(PKV_ERR_ARG, "page index codes must be 16-byte aligned");
+  if (p.dtype != PKV_F16 && p.dtype != PKV_BF16 && p.dtype != PKV_F32)
+    return fail(PKV_ERR_UNSUPPORTED, "the page index takes fp16, bf16 or fp32 pools");
+  if (p.head_dim > 256) return fail(PKV_ERR_UNSUPPORTED, "the page index takes head_dim up to 256");
+  return PKV_OK;
+}
+
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" int pkv_page_index_update(const pkv_pool* pool, const pkv_page_index* index, int32_t layer,
+                                     const int32_t* slot_mapping, int64_t n_tokens, int32_t* dev_status,
+                                     void* stream) {
+  if (int rc = check_pool(pool)) return rc;
+  if (int rc = check_index(*pool, index)) return rc;
+  if (layer < 0 || layer >= pool->num_layers)
+    return fail(PKV_ERR_ARG, "layer_idx " + std::to_string(layer) + " out of range [0, " +
+                                 std::to_string(pool->num_layers) + ")");
+  if (n_tokens < 0) return fail(PKV_ERR_ARG, "n_tokens must be >= 0");
+  if (n_tokens == 0) return PKV_OK;
+  if (!slot_mapping) return fail(PKV_ERR_ARG, "slot_mapping must be non-NULL");
+  return run_index(*pool, index, layer, slot_mapping, n_tokens, dev_status, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int pkv_page_index_rebuild(const pkv_pool* pool, const pkv_page_index* index, const int32_t* block_ids,
+                                      int64_t nb, int32_t* dev_status, void* stream) {
+  if (int rc = check_pool(pool)) return rc;
+  if (int rc = check_index(*pool, index)) return rc;
+  if (nb < 0) return fail(PKV_ERR_ARG, "nb must be >= 0");
+  if (nb == 0) return PKV_OK;
+  if (!block_ids) return fail(PKV_ERR_ARG, "block_ids must be non-NULL");
+  return run_index(*pool, index, -1, block_ids, nb, dev_status, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int pkv_rope_append(const pkv_pool* pool, int32_t layer, const void* q, int64_t q_stride, void* q_out,
+                               int32_t n_heads, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                               const int32_t* slot_mapping, const int64_t* positions, int64_t n_tokens,
+                               const float* rope_cos, const float* rope_sin, int64_t rope_max_pos,
+                               int32_t rotary_dim, int32_t interleaved, const pkv_page_index* index,
+                               int32_t* dev_status, void* stream) {
+  if (int rc = check_pool(pool)) return rc;
+  const pkv_pool& p = *pool;
+  if (layer < 0 || layer >= p.num_layers)
+    return fail(PKV_ERR_ARG, "layer_idx " + std::to_string(layer) + " out of range [0, " +
+                                 std::to_string(p.num_layers) + ")");
+  if (p.dtype != PKV_F16 && p.dtype != PKV_BF16 && p.dtype != PKV_F32)
+    return fail(PKV_ERR_UNSUPPORTED, "pkv_rope_append takes fp16, bf16 or fp32 pools");
+  if (index)
+    if (int rc = check_index(p, index)) return rc;
+  if (n_tokens < 0 || n_heads < 0) return fail(PKV_ERR_ARG, "n_tokens and n_heads must be >= 0");
+  if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > p.head_dim)
+    return fail(PKV_ERR_ARG, "rotary_dim must be even and in [2, head_dim]");
+  if (n_tokens == 0) return PKV_OK;
+  if ((n_heads > 0 && (!q || !q_out)) || !k || !v || !slot_mapping || !positions || !rope_cos || !rope_sin)
+    return fail(PKV_ERR_ARG, "q, q_out, k, v, slot_mapping, positions and the rope tables must be non-NULL");
+  if (rope_max_pos <= 0) return fail(PKV_ERR_ARG, "rope_max_pos must be positive");
+  const int es = elem_size(p.dtype);
+  const int64_t qrow = int64_t(n_heads) * p.head_dim, krow = int64_t(p.n_kv_heads) * p.head_dim;
+  if ((n_heads > 0 && q_stride < qrow) || k_stride < krow || v_stride < krow)
+    return fail(PKV_ERR_ARG, "a token stride is smaller than the token's row");
+  if (qrow + krow >= (int64_t(1) << 30)) return fail(PKV_ERR_ARG, "heads * head_dim too large");
+  RopeAppendArgs a;
+  a.q = static_cast<const char*>(q);
+  a.k = static_cast<const char*>(k);
+  a.v = static_cast<const char*>(v);
+  a.q_out = static_cast<char*>(q_out);
+  a.k_slab = static_cast<char*>(p.base) + int64_t(2) * layer * slab_bytes(p);
+  a.v_slab = a.k_slab + slab_bytes(p);
+  a.slots = slot_mapping;
+  a.positions = positions;
+  a.cs = rope_cos;
+  a.sn = rope_sin;
+  a.st = dev_status;
+  a.q_stride = q_stride * es;
+  a.k_stride = k_stride * es;
+  a.v_stride = v_stride * es;
+  a.qo_stride = qrow * es;
+  a.n_tokens = n_tokens;
+  a.n_slots = p.num_blocks * p.block_size;
+  a.max_pos = rope_max_pos;
+  a.hq = n_heads;
+  a.hkv = p.n_kv_heads;
+  a.d = p.head_dim;
+  a.half = rotary_dim / 2;
+  // 16-byte vectors where every row, head and column a unit touches is 16-byte aligned
+  const int ve = 16 / es;
+  uintptr_t al = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | uintptr_t(a.k_stride) |
+                 uintptr_t(a.v_stride) | uintptr_t(int64_t(p.head_dim) * es) | reinterpret_cast<uintptr_t>(rope_cos) |
+                 reinterpret_cast<uintptr_t>(rope_sin) | uintptr_t(slab_bytes(p));
+  if (n_heads > 0)
+    al |= reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | uintptr_t(a.q_stride);
+  const bool vec = (al & 15) == 0 && a.half % ve == 0;
+  // one warp per token once that fills the SMs' warp slots, else up to 8
+  const int64_t want = int64_t(num_sms()) * 32;
+  a.wpt = n_tokens >= want ? 1 : (2 * n_tokens >= want ? 2 : (4 * n_tokens >= want ? 4 : 8));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool inter = interleaved != 0;
+  int rc;
+  switch (p.dtype) {
+    case PKV_F16: rc = launch_rope_append<__half>(a, vec, inter, s); break;
+    case PKV_BF16: rc = launch_rope_append<__nv_bfloat16>(a, vec, inter, s); break;
+    default: rc = launch_rope_append<float>(a, vec, inter, s); break;
+  }
+  if (rc || !index) return rc;
+  return run_index(p, index, layer, slot_mapping, n_tokens, dev_status, s);
+}

@@ -47,6 +47,9 @@ inline int64_t row_bytes(const pkv_pool& p) {
 inline int64_t block_bytes(const pkv_pool& p) { return row_bytes(p) * p.block_size; }
 inline int64_t slab_bytes(const pkv_pool& p) { return block_bytes(p) * p.num_blocks; }
 
+// Validates a page index against its pool (pkv_append.cu).
+int check_index(const pkv_pool& p, const pkv_page_index* ix);
+
 int num_sms();  // SM count of the current device (cached per device)
 
 // Programmatic dependent launch (PDL): the per-layer kernels of a step
@@ -100,6 +103,19 @@ int prefill_tc_tile_tokens(int n_heads, int n_kv_heads);
 int prefill_tc_attend(const pkv_pool& p, int layer, int n_heads, const void* q, void* out, float scale,
                       const pkv_batch& b, const int2* tiles, const int32_t* n_tiles, int64_t tiles_cap,
                       cudaStream_t s);
+
+// The decode kernel over listed q_len == 1 rows whose sequences start from
+// pieces computed before (pkv_attn.cu, for shared-prefix attention). The list
+// (descriptors, zeroed split-K counters) lies in `ws` as decode_list_layout says;
+// rows / p_dec as in PrefillMixedPlan, fold / fold_o / fold_ml as DecodeArgs'.
+struct DecodeListLayout {
+  size_t page_desc, counters, total;
+};
+bool decode_fold_supported(const pkv_pool& p, int n_heads);
+DecodeListLayout decode_list_layout(int n_heads, int n_seqs, int64_t total_pages);
+int decode_fold(const pkv_pool& p, int layer, int n_heads, const void* q, void* out, float scale, const pkv_batch& b,
+                char* ws, const int32_t* rows, const int64_t* p_dec, const int4* fold, const float* fold_o,
+                const float2* fold_ml, cudaStream_t s);
 
 // ---------------------------------------------------------------- device side
 // PDL: let the next kernel in the stream be scheduled now; wait until the

@@ -1,0 +1,1050 @@
+// pkv_shared.cu — attention of a batch whose sequences share leading pages
+// (families of the radix prefix cache: their block tables start with the same
+// physical pages).
+//
+// The sequences of a batch come in groups; group g's sequences share their
+// first n_g pages. For a row of group g with keys split into the shared prefix A
+// and its own rest B,
+//   out = (w_A O_A + w_B O_B) / (w_A + w_B),   w_X = l_X 2^(m_X - m),
+// with O_X the normalised attention over X, m_X its score maximum (log2 units) and
+// l_X its sum of 2^(s - m_X). All rows of a group see all of A, so A is one dense
+// product of (rows of the group) x (keys of A) per KV head, read once:
+//
+//   shared_check_kernel  once per step: verifies that a group's page lists agree
+//   shared_plan_kernel   once per step: the work items, the pieces each row
+//                        merges, and the decode kernel's page list of the rest
+//   shared_tc_kernel     tcgen05 tiles of 128 rows (128 / G tokens of the group
+//                        x the G query heads of a KV head) over a range of A's
+//                        64-key blocks -> pieces (O, m, l) in fp32. Also the rest
+//                        B of sequences with several new tokens (causal).
+//   decode kernel        the rest B of sequences with one new token; starts from
+//                        the row's pieces (decode_fold, pkv_attn.cu)
+//   shared_merge_kernel  the pieces of rows of several-token sequences -> out
+//
+// A's keys are read once per 128 rows instead of once per sequence; its
+// arithmetic is 4 D flops per (row, key) on the tensor cores. The range length
+// of an item is chosen on the device so that the items fill the SMs.
+#include <algorithm>
+#include <mutex>
+#include <string>
+#include <type_traits>
+#include <vector>
+
+#include "pkv_tc.cuh"
+
+namespace pkv {
+namespace {
+
+constexpr int SH_MINB = 3;          // CTAs per SM of the tile kernel
+constexpr int SH_NST = 2;           // slots of the K ring and of the V ring
+constexpr int SH_TMEM_COLS = 128;   // S in columns 0-63, O in 64-127
+constexpr int SH_PIECES = 16384;    // token pieces the workspace holds at most (x n_heads x 264 bytes)
+constexpr int SH_OVERHEAD = 4;      // cost of an item besides its blocks, in blocks (set-up, piece written and read)
+
+// Rows (consecutive tokens) against a page range of one list.
+struct ShEnt {
+  int t0, nt;      // first token, tokens
+  int pa;          // first entry of the page list
+  int pg0, pg1;    // pages of the list
+  int lim0;        // last key token t0 sees
+  int causal;      // 1: token t0 + i sees i more keys
+  int lpl;         // tokens in page pg1 - 1
+  int base;        // first piece row (-1: the result goes straight to out)
+  int splits;      // ranges the pages are cut into
+  int tiles;
+  int item0;       // first item
+};
+
+struct ShCtl {
+  int n_items;
+  int claim[2];    // next item, CTAs finished
+  int chunk;       // blocks per range
+  int64_t p_dec;   // pages listed for the decode kernel
+  int n_ents;
+  int n_shared;    // groups whose prefix is shared
+};
+
+struct ShLayout {
+  DecodeListLayout dec;
+  size_t ctl, rows, seq_np, group_bad, ents, items, fold, rest, part_o, part_ml, total;
+  int64_t pieces, items_cap;
+};
+
+inline size_t al256(size_t x) { return (x + 255) & ~size_t(255); }
+
+int split_cap(int n_tokens) { return std::max(1, std::min(64, 4096 / std::max(n_tokens, 1))); }
+
+ShLayout sh_layout(int n_heads, int groups, int n_seqs, int n_tokens, int64_t total_pages) {
+  ShLayout w;
+  w.dec = decode_list_layout(n_heads, n_seqs, total_pages);
+  size_t off = al256(w.dec.total);
+  const int cap = split_cap(n_tokens);
+  const int tpt = TC_ROWS / groups;
+  w.pieces = std::min<int64_t>(int64_t(2) * n_tokens * cap, SH_PIECES);
+  // every entity's last tile may be partial; an entity is a group or a sequence
+  w.items_cap = (int64_t(2) * ((n_tokens + tpt - 1) / tpt) + 2 * int64_t(n_seqs)) * cap;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off = al256(off + bytes);
+    return at;
+  };
+  w.ctl = take(sizeof(ShCtl));
+  w.rows = take(sizeof(int32_t) * n_seqs);
+  w.seq_np = take(sizeof(int32_t) * n_seqs);
+  w.group_bad = take(sizeof(int32_t) * n_seqs);
+  w.ents = take(sizeof(ShEnt) * 2 * n_seqs);
+  w.items = take(sizeof(int4) * w.items_cap);
+  w.fold = take(sizeof(int4) * std::max(n_tokens, 1));
+  w.rest = take(sizeof(int4) * std::max(n_tokens, 1));
+  w.part_o = take(sizeof(float) * size_t(w.pieces) * n_heads * TC_D);
+  w.part_ml = take(sizeof(float2) * size_t(w.pieces) * n_heads);
+  w.total = off;
+  return w;
+}
+
+// ---------------------------------------------------------------- plan
+struct PlanArgs {
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* last_page_len;
+  const int32_t* group_indptr;  // [n_groups + 1] over the sequences
+  const int32_t* prefix_pages;  // [n_groups]
+  int32_t* st;
+  int64_t num_blocks, total_pages;
+  int n_seqs, n_tokens, n_groups, n_kv, tpt, slots, splits_cap;
+  int64_t pieces_cap, items_cap;
+  ShCtl* ctl;
+  int32_t* rows;
+  int32_t* seq_np;
+  int32_t* group_bad;
+  ShEnt* ents;
+  int4* items;
+  int4* fold;
+  int4* rest;
+  int4* desc;
+  int32_t* counters;
+};
+
+struct SeqInfo {
+  bool ok;
+  int q0, ql, pa, pages, lpl;
+  int64_t kv;
+};
+__device__ __forceinline__ SeqInfo seq_info(const PlanArgs& a, int s) {
+  SeqInfo r;
+  r.q0 = a.cu_q[s];
+  r.ql = a.cu_q[s + 1] - r.q0;
+  const int64_t pa = a.kv_indptr[s], pb = a.kv_indptr[s + 1];
+  r.lpl = a.last_page_len[s];
+  r.pa = int(pa);
+  r.pages = int(pb - pa);
+  r.kv = (pb - pa - 1) * TC_P + r.lpl;
+  r.ok = r.q0 >= 0 && r.ql >= 1 && int64_t(r.q0) + r.ql <= a.n_tokens && pa >= 0 && pb > pa && pb <= a.total_pages &&
+         r.lpl >= 1 && r.lpl <= TC_P && r.kv >= r.ql && r.kv < 0x7fffffff && (!a.kv_lens || a.kv_lens[s] == r.kv);
+  return r;
+}
+// group of sequence s: the last g with group_indptr[g] <= s
+__device__ __forceinline__ int group_of(const PlanArgs& a, int s) {
+  int lo = 0, hi = a.n_groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.group_indptr[mid] <= s) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// One CTA per sequence: do its leading pages agree with its group's first
+// sequence's, and do its new tokens lie after them? If not the group is marked
+// (and flagged) and computed without sharing.
+__global__ void __launch_bounds__(128) shared_check_kernel(const PlanArgs a) {
+  const int s = blockIdx.x;
+  const int g = group_of(a, s);
+  const int f = a.group_indptr[g], e = a.group_indptr[g + 1];
+  const int np = a.prefix_pages[g];
+  bool bad = f < 0 || s < f || s >= e || e > a.n_seqs || np < 0;
+  if (!bad && np > 0) {
+    const SeqInfo x = seq_info(a, s), y = seq_info(a, f);
+    bad = !x.ok || !y.ok || int64_t(np) * TC_P > x.kv - x.ql || np > y.pages;
+    if (!bad)
+      for (int i = threadIdx.x; i < np; i += blockDim.x) {
+        const int id = a.kv_indices[x.pa + i];
+        bad |= id != a.kv_indices[y.pa + i] || id < 0 || id >= a.num_blocks;
+      }
+  }
+  if (bad) {
+    flag(a.st, PKV_DEV_META_BAD);
+    if (g >= 0 && g < a.n_groups) a.group_bad[g] = 1;
+  }
+}
+
+__global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
+  __shared__ int warp_sum[32];
+  __shared__ int s_bad, s_maxblk, s_tot;
+  __shared__ unsigned long long s_best;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    s_bad = (a.cu_q[0] != 0 || a.cu_q[a.n_seqs] != a.n_tokens || a.group_indptr[0] != 0 ||
+             a.group_indptr[a.n_groups] != a.n_seqs) ? 1 : 0;
+    a.ctl->n_items = 0;
+    a.ctl->claim[0] = a.ctl->claim[1] = 0;
+    a.ctl->p_dec = 0;
+  }
+  for (int t = tid; t < a.n_tokens; t += blockDim.x) a.fold[t] = a.rest[t] = make_int4(0, 0, 0, 0);
+  __syncthreads();
+  if (s_bad) {
+    if (tid == 0) flag(a.st, PKV_DEV_META_BAD);
+    for (int d = tid; d < a.n_seqs; d += blockDim.x) a.rows[d] = -1;
+    __threadfence();
+    return;
+  }
+  // share = 1: as the groups say. Should even one piece per row and range not
+  // fit the workspace, a second round (share = 0) computes every sequence by itself.
+  int n_ents = 0, n_shared = 0, chunk = 1;
+  for (int share = 1; share >= 0; --share) {
+    for (int s = tid; s < a.n_seqs; s += blockDim.x) {
+      const int g = group_of(a, s);
+      const int f = a.group_indptr[g], e = a.group_indptr[g + 1];
+      // a group of one sequence shares nothing
+      a.seq_np[s] = share && e - f >= 2 && !a.group_bad[g] ? a.prefix_pages[g] : 0;
+    }
+    if (tid == 0) s_maxblk = 1;
+    __syncthreads();
+    // ---- entities: the shared groups, then the several-token sequences
+    n_ents = 0;
+    for (int c0 = 0; c0 < a.n_groups; c0 += blockDim.x) {
+      const int g = c0 + tid;
+      ShEnt x{};
+      int is = 0;
+      if (g < a.n_groups) {
+        const int f = a.group_indptr[g], e = a.group_indptr[g + 1];
+        const int np = f < e && f >= 0 && e <= a.n_seqs ? a.seq_np[f] : 0;
+        if (np > 0) {
+          is = 1;
+          x.t0 = a.cu_q[f];
+          x.nt = a.cu_q[e] - x.t0;
+          x.pa = a.kv_indptr[f];
+          x.pg0 = 0;
+          x.pg1 = np;
+          x.lim0 = np * TC_P - 1;
+          x.lpl = TC_P;
+          x.tiles = (x.nt + a.tpt - 1) / a.tpt;
+          atomicMax(&s_maxblk, (np + TC_PPB - 1) / TC_PPB);
+        }
+      }
+      int tot;
+      const int i = n_ents + block_excl_scan(is, warp_sum, &tot);
+      if (is) a.ents[i] = x;
+      n_ents += tot;
+    }
+    n_shared = n_ents;
+    for (int c0 = 0; c0 < a.n_seqs; c0 += blockDim.x) {
+      const int s = c0 + tid;
+      ShEnt x{};
+      int is = 0;
+      if (s < a.n_seqs) {
+        const SeqInfo q = seq_info(a, s);
+        if (!q.ok) {
+          flag(a.st, PKV_DEV_META_BAD);
+        } else if (q.ql > 1) {
+          is = 1;
+          x.t0 = q.q0;
+          x.nt = q.ql;
+          x.pa = q.pa;
+          x.pg0 = a.seq_np[s];
+          x.pg1 = q.pages;
+          x.lim0 = int(q.kv) - q.ql;
+          x.causal = 1;
+          x.lpl = q.lpl;
+          x.tiles = (x.nt + a.tpt - 1) / a.tpt;
+          x.base = x.pg0 > 0 ? 0 : -1;
+          if (x.pg0 > 0) atomicMax(&s_maxblk, (x.pg1 - x.pg0 + TC_PPB - 1) / TC_PPB);
+        }
+      }
+      int tot;
+      const int i = n_ents + block_excl_scan(is, warp_sum, &tot);
+      if (is) a.ents[i] = x;
+      n_ents += tot;
+    }
+    __threadfence_block();
+    __syncthreads();
+    // ---- blocks per range: each thread weighs one length. A launch of items
+    // claimed by `slots` resident CTAs takes about the average load plus one
+    // item; ranges too short pay the items' overhead, too long the last item.
+    const int maxblk = s_maxblk;
+    const int step = (maxblk + int(blockDim.x) - 1) / int(blockDim.x);
+    const int cand = min(maxblk, (tid + 1) * step);
+    float work = 0.f, n_it = 0.f;
+    int64_t pieces = 0;
+    bool fits = true;
+    for (int i = 0; i < n_ents; ++i) {
+      const ShEnt x = a.ents[i];
+      const int nb = (x.pg1 - x.pg0 + TC_PPB - 1) / TC_PPB;
+      const int sp = x.base < 0 ? 1 : (nb + cand - 1) / cand;
+      fits &= sp <= a.splits_cap;
+      work += float(x.tiles) * nb;
+      n_it += float(x.tiles) * sp;
+      if (x.base >= 0) pieces += int64_t(x.nt) * sp;
+    }
+    fits &= pieces <= a.pieces_cap;
+    const float est = (work + n_it * SH_OVERHEAD) * a.n_kv / a.slots + cand + SH_OVERHEAD;
+    if (tid == 0) s_best = ~0ull;
+    __syncthreads();
+    if (fits && (tid == 0 || (tid + 1) * step < maxblk + step))
+      atomicMin(&s_best, (static_cast<unsigned long long>(__float_as_uint(est)) << 32) | unsigned(cand));
+    __syncthreads();
+    const unsigned long long best = s_best;
+    __syncthreads();
+    chunk = int(best & 0xffffffffu);
+    if (best != ~0ull) break;  // always in the second round: nothing is shared, no pieces
+  }
+  // ---- piece rows and items of each entity
+  int base0 = 0, item0 = 0;
+  for (int c0 = 0; c0 < n_ents; c0 += blockDim.x) {
+    const int i = c0 + tid;
+    ShEnt x{};
+    int np = 0, ni = 0;
+    if (i < n_ents) {
+      x = a.ents[i];
+      const int nb = (x.pg1 - x.pg0 + TC_PPB - 1) / TC_PPB;
+      x.splits = x.base < 0 ? 1 : (nb + chunk - 1) / chunk;
+      np = x.base < 0 ? 0 : x.nt * x.splits;
+      ni = x.tiles * x.splits;
+    }
+    int tp, ti;
+    const int b = base0 + block_excl_scan(np, warp_sum, &tp);
+    const int it = item0 + block_excl_scan(ni, warp_sum, &ti);
+    if (i < n_ents) {
+      if (x.base >= 0) x.base = b;
+      x.item0 = it;
+      a.ents[i] = x;
+    }
+    base0 += tp;
+    item0 += ti;
+  }
+  __threadfence_block();
+  __syncthreads();
+  if (tid == 0) s_tot = item0 <= a.items_cap ? 1 : 0;
+  __syncthreads();
+  const bool room = s_tot != 0;  // the capacity covers every case: kept as a check
+  for (int i = warp; room && i < n_ents; i += 32) {
+    const ShEnt x = a.ents[i];
+    for (int k = lane; k < x.tiles * x.splits; k += 32)
+      a.items[x.item0 + k] = make_int4(i, k / x.splits, k % x.splits, 0);
+    if (x.base >= 0) {
+      int4* to = x.causal ? a.rest : a.fold;
+      for (int k = lane; k < x.nt; k += 32) to[x.t0 + k] = make_int4(x.base + k, x.splits, x.nt, 0);
+    }
+  }
+  if (tid == 0) {
+    if (!room) flag(a.st, PKV_DEV_WORKSPACE);
+    a.ctl->n_items = room ? item0 : 0;
+    a.ctl->chunk = chunk;
+    a.ctl->n_ents = n_ents;
+    a.ctl->n_shared = n_shared;
+  }
+  // ---- the decode kernel's list: one-token sequences, their pages after the shared ones
+  int base_seq = 0, base_pg = 0;
+  for (int c0 = 0; c0 < a.n_seqs; c0 += blockDim.x) {
+    const int s = c0 + tid;
+    int is = 0, np = 0;
+    SeqInfo q{};
+    if (s < a.n_seqs) {
+      q = seq_info(a, s);
+      if (q.ok && q.ql == 1) {
+        is = 1;
+        np = q.pages - a.seq_np[s];
+      }
+    }
+    int tot_seq, tot_pg;
+    const int d = base_seq + block_excl_scan(is, warp_sum, &tot_seq);
+    const int off = base_pg + block_excl_scan(np, warp_sum, &tot_pg);
+    if (is) {
+      a.rows[d] = q.q0;
+      a.counters[d] = 0;
+    }
+    // the warp writes its sequences' descriptors one sequence at a time
+    for (int l = 0; l < 32; ++l) {
+      if (!__shfl_sync(0xffffffffu, is, l)) continue;
+      const int dn = __shfl_sync(0xffffffffu, d, l), on = __shfl_sync(0xffffffffu, off, l);
+      const int nn = __shfl_sync(0xffffffffu, np, l), lp = __shfl_sync(0xffffffffu, q.lpl, l);
+      const int from = __shfl_sync(0xffffffffu, q.pa + q.pages - np, l);
+      for (int p = lane; p < nn && int64_t(on) + nn <= a.total_pages; p += 32) {
+        const int id = a.kv_indices[from + p];
+        if (id < 0 || id >= a.num_blocks) flag(a.st, PKV_DEV_SLOT_OOB);
+        const int first = p == 0, last = p == nn - 1;
+        a.desc[on + p] = make_int4(id, (dn << 7) | (first << 6) | (last << 5) | (last ? lp : TC_P), on, on + nn);
+      }
+    }
+    base_seq += tot_seq;
+    base_pg += tot_pg;
+  }
+  for (int d = base_seq + tid; d < a.n_seqs; d += blockDim.x) a.rows[d] = -1;
+  if (tid == 0) {
+    // overlapping page lists (some indptr entry runs backwards) list more pages
+    // than there are: nothing is decoded
+    if (base_pg > a.total_pages) flag(a.st, PKV_DEV_META_BAD);
+    a.ctl->p_dec = base_pg > a.total_pages ? 0 : base_pg;
+  }
+  // read by later kernels before their griddepcontrol.wait (this kernel never
+  // triggers its dependents early): visible at GPU scope before the block exits
+  __threadfence();
+}
+
+// ---------------------------------------------------------------- tile kernel
+struct ShArgs {
+  void* out;
+  const ShCtl* ctl;
+  int32_t* claim;
+  const ShEnt* ents;
+  const int4* items;
+  const int32_t* kv_indices;
+  float* part_o;
+  float2* part_ml;
+  int32_t* st;
+  int64_t num_blocks;
+  int n_heads, n_kv, layer;
+  float scale_log2;
+};
+
+// A work item as the producer publishes it (nblk = 0: no more items).
+struct ShItem {
+  int h, t0, nt;     // KV head, first token, tokens of the tile
+  int n_pg, nblk;    // pages and 64-key blocks of the range
+  int lim0, causal;  // last key (counted from the range's first) the first token sees
+  int tail_pg, lpl;  // page of the range with only lpl written tokens (-1: none)
+  int piece;         // piece row of the first token (-1: straight to out)
+  int zero;          // a page id outside the pool: the item's rows are zeros
+};
+
+// The tile pipeline of prefill_tc_lean_kernel (pkv_prefill_tc.cu) over the
+// plan's items: three persistent CTAs per SM; warp 0 claims items and loads the
+// query tile and the K / V blocks by TMA, warp 1 issues S = Q K^T and O += P V
+// (tcgen05, accumulators in TMEM), warps 2-5 hold one row a thread: running
+// maximum and sum, P to shared memory, lazy rescale of O. The epilogue writes
+// the row as a piece: O / l in fp32 and (m, l).
+template <typename T, int G>
+__global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_tc_kernel(
+    const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap qmap, const ShArgs a) {
+  constexpr int TPT = TC_ROWS / G;  // tokens per tile
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* qbuf = smem;                             // [128 rows][128 B], 128B swizzle
+  unsigned char* kst = smem + TC_QTILE;                   // SH_NST x K [64 keys][128 B]
+  unsigned char* vst = kst + size_t(SH_NST) * TC_KTILE;   // SH_NST x V [64 keys][128 B]
+  unsigned char* pbuf = vst + size_t(SH_NST) * TC_KTILE;  // P [128 rows][128 B], 128B swizzle
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(pbuf + TC_QTILE);
+  uint64_t* kempty = kfull + SH_NST;
+  uint64_t* vfull = kempty + SH_NST;
+  uint64_t* vempty = vfull + SH_NST;
+  uint64_t* s_full = vempty + SH_NST;
+  uint64_t* s_free = s_full + 1;
+  uint64_t* p_full = s_free + 1;
+  uint64_t* pv_done = p_full + 1;
+  uint64_t* q_full = pv_done + 1;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* o_free = q_empty + 1;
+  uint64_t* item_full = o_free + 1;
+  uint64_t* item_empty = item_full + 2;
+  uint64_t* drain = item_empty + 2;
+  __shared__ uint32_t s_tmem;
+  __shared__ ShItem s_item[2];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  // the plan completed before this kernel could start and fenced its stores
+  const int n_items = __ldcg(&a.ctl->n_items) * a.n_kv;
+  if (int(blockIdx.x) >= n_items) {  // no item for this CTA (uniform over the CTA)
+    pdl_wait();                      // the counters belong to the previous launch until it completed
+    if (threadIdx.x == 0) tl_count_exit(a.claim);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmap);
+    prefetch_tmap(&qmap);
+    for (int i = 0; i < SH_NST; ++i) {
+      mbar_init(&kfull[i], 1);
+      mbar_init(&kempty[i], 1);
+      mbar_init(&vfull[i], 1);
+      mbar_init(&vempty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_free, 128);
+    mbar_init(p_full, 128);
+    mbar_init(pv_done, 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(o_free, 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 129);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+  }
+  // ---- tensor memory: 128 columns S | O, freed on every path below
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                 "r"(SH_TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = s_tmem;
+  const uint32_t tO = tbase + TC_KB;
+  pdl_wait();  // q and this layer's appended K/V rows are written by earlier kernels
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const int kvc = 2 * a.layer;
+    const int chunk_pg = a.ctl->chunk * TC_PPB;
+    uint32_t kiss = 0, viss = 0;  // K / V slots filled so far
+    int it = 0;                   // items published
+    bool dead = false;
+    while (!dead) {
+      int w = 0;
+      if (lane == 0) w = atomicAdd(a.claim, 1);
+      w = __shfl_sync(0xffffffffu, w, 0);
+      const bool end = w >= n_items;
+      ShItem I{};
+      int pg_at = 0;  // first entry of the range in kv_indices
+      if (!end) {
+        const int4 d = a.items[w / a.n_kv];
+        const ShEnt e = a.ents[d.x];
+        I.h = w % a.n_kv;
+        const int i0 = d.y * TPT;  // first token of the tile within the entity
+        I.t0 = e.t0 + i0;
+        I.nt = min(TPT, e.nt - i0);
+        const int first = e.pg0 + (e.base < 0 ? 0 : d.z * chunk_pg);
+        const int last = e.base < 0 ? e.pg1 : min(e.pg1, first + chunk_pg);
+        I.lim0 = e.lim0 + e.causal * i0 - first * TC_P;
+        I.causal = e.causal;
+        const int seen = I.lim0 + e.causal * (I.nt - 1);  // last key any of its rows sees
+        I.n_pg = seen < 0 ? 0 : min(last - first, seen / TC_P + 1);
+        I.nblk = max(1, (I.n_pg + TC_PPB - 1) / TC_PPB);  // a range no row sees: one block, all masked
+        I.tail_pg = e.lpl < TC_P && e.pg1 - 1 - first < I.n_pg ? e.pg1 - 1 - first : -1;
+        I.lpl = e.lpl;
+        I.piece = e.base < 0 ? -1 : e.base + d.z * e.nt + i0;
+        pg_at = e.pa + first;
+      }
+      bool pg_bad = false;
+      for (int pg = lane; pg < I.n_pg; pg += 32) {
+        const int id = a.kv_indices[pg_at + pg];
+        pg_bad |= id < 0 || id >= a.num_blocks;
+      }
+      pg_bad = __any_sync(0xffffffffu, pg_bad);
+      const int sl = it & 1;
+      if (it >= 2 && !mbar_wait_bounded_sleepy(&item_empty[sl], ((it - 2) >> 1) & 1, a.st, 32)) dead = true;
+      dead = __any_sync(0xffffffffu, dead);
+      if (dead) break;
+      if (lane == 0) {
+        I.zero = pg_bad ? 1 : 0;
+        if (end) I.nblk = 0;
+        s_item[sl] = I;
+        if (pg_bad) flag(a.st, PKV_DEV_SLOT_OOB);
+        mbar_arrive(&item_full[sl]);
+      }
+      __syncwarp();
+      if (end) break;
+      if (lane == 0) {
+        if (it >= 1 && !mbar_wait_bounded_sleepy(q_empty, (it - 1) & 1, a.st, 64)) dead = true;
+        if (!dead) {
+          mbar_arrive_expect_tx(q_full, TC_QTILE);
+          tma_load_3d(qbuf, &qmap, q_full, 0, I.h * G, I.t0);
+        }
+        for (int j = 0; j < I.nblk && !dead; ++j) {
+          int rows[TC_PPB];
+#pragma unroll
+          for (int u = 0; u < TC_PPB; ++u) {
+            const int pg = j * TC_PPB + u;
+            // a page past the range reads the zero fill of a negative coordinate
+            rows[u] = pg < I.n_pg && !pg_bad ? a.kv_indices[pg_at + pg] * TC_P : -TC_P;
+          }
+          const int st = int(kiss % SH_NST);
+          if (kiss >= SH_NST && !mbar_wait_bounded_sleepy(&kempty[st], ((kiss / SH_NST) - 1) & 1, a.st, 32)) {
+            dead = true;
+            break;
+          }
+          mbar_arrive_expect_tx(&kfull[st], TC_KTILE);
+#pragma unroll
+          for (int u = 0; u < TC_PPB; ++u)
+            tma_load_4d(kst + size_t(st) * TC_KTILE + u * TC_PAGE, &tmap, &kfull[st], 0, rows[u], I.h, kvc);
+          ++kiss;
+          if (viss >= SH_NST && !mbar_wait_bounded_sleepy(&vempty[st], ((viss / SH_NST) - 1) & 1, a.st, 32)) {
+            dead = true;
+            break;
+          }
+          mbar_arrive_expect_tx(&vfull[st], TC_KTILE);
+#pragma unroll
+          for (int u = 0; u < TC_PPB; ++u)
+            tma_load_4d(vst + size_t(st) * TC_KTILE + u * TC_PAGE, &tmap, &vfull[st], 0, rows[u], I.h, kvc + 1);
+          ++viss;
+        }
+      }
+      dead = __shfl_sync(0xffffffffu, dead, 0);
+      ++it;
+    }
+    if (dead && lane == 0) {
+      // let this CTA's own copies land before its shared memory can be released
+      for (uint32_t i = kiss > SH_NST ? kiss - SH_NST : 0; i < kiss; ++i)
+        mbar_wait_bounded(&kfull[i % SH_NST], (i / SH_NST) & 1, nullptr);
+      for (uint32_t i = viss > SH_NST ? viss - SH_NST : 0; i < viss; ++i)
+        mbar_wait_bounded(&vfull[i % SH_NST], (i / SH_NST) & 1, nullptr);
+      if (it >= 1) mbar_wait_bounded(q_full, (it - 1) & 1, nullptr);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    constexpr uint32_t idS = idesc_f16(fmt, 0, TC_KB);
+    constexpr uint32_t idPV = idesc_f16(fmt, 1, TC_D);
+    const uint32_t q_addr = smem_u32(qbuf), p_addr = smem_u32(pbuf);
+    uint32_t g = 0;
+    int it = 0;
+    bool dead = false;
+    auto pv = [&](uint32_t gp, int jp, const ShItem& I) -> bool {
+      const int stp = int(gp % SH_NST);
+      bool bad = !mbar_wait_bounded(p_full, gp & 1, a.st);
+      if (!bad && jp == 0 && it >= 1 && !mbar_wait_bounded(o_free, (it - 1) & 1, a.st)) bad = true;
+      if (!bad && !mbar_wait_bounded(&vfull[stp], (gp / SH_NST) & 1, a.st)) bad = true;
+      bad = __any_sync(0xffffffffu, bad);
+      if (bad) return false;
+      if (I.tail_pg >= 0 && jp == I.tail_pg / TC_PPB) {
+        // rows lpl..15 of the last page's V slice were never written: zero them
+        uint4* vt = reinterpret_cast<uint4*>(vst + size_t(stp) * TC_KTILE + (I.tail_pg - jp * TC_PPB) * TC_PAGE);
+        for (int rr = I.lpl * 8 + lane; rr < TC_P * 8; rr += 32) vt[rr] = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) {
+        tc_fence_after();
+        const uint32_t vaddr = smem_u32(vst + size_t(stp) * TC_KTILE);
+#pragma unroll
+        for (int kk = 0; kk < TC_KB / 16; ++kk)
+          umma_ss(tO, sw128_desc(p_addr + 32 * kk), sw128_desc(vaddr + 16 * 128 * kk), idPV,
+                  (jp > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&vempty[stp]);
+        umma_commit(pv_done);
+      }
+      __syncwarp();
+      return true;
+    };
+    while (!dead) {
+      const int sl = it & 1;
+      if (!mbar_wait_bounded(&item_full[sl], (it >> 1) & 1, a.st)) dead = true;
+      dead = __any_sync(0xffffffffu, dead);
+      if (dead) break;
+      const ShItem I = s_item[sl];
+      if (I.nblk == 0) break;
+      if (!mbar_wait_bounded(q_full, it & 1, a.st)) dead = true;
+      dead = __any_sync(0xffffffffu, dead);
+      if (dead) break;
+      for (int j = 0; j < I.nblk; ++j) {
+        const uint32_t gj = g + j;
+        const int st = int(gj % SH_NST);
+        // S_j overwrites S_{j-1}: after the softmax threads loaded it
+        if (gj >= 1 && !mbar_wait_bounded(s_free, (gj - 1) & 1, a.st)) dead = true;
+        if (!dead && !mbar_wait_bounded(&kfull[st], (gj / SH_NST) & 1, a.st)) dead = true;
+        dead = __any_sync(0xffffffffu, dead);
+        if (dead) break;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint32_t kaddr = smem_u32(kst + size_t(st) * TC_KTILE);
+#pragma unroll
+          for (int kk = 0; kk < TC_D / 16; ++kk)
+            umma_ss(tbase, sw128_desc(q_addr + 32 * kk), sw128_desc(kaddr + 32 * kk), idS, kk > 0);
+          umma_commit(s_full);
+          umma_commit(&kempty[st]);
+          if (j == I.nblk - 1) umma_commit(q_empty);  // the item's last read of its query tile
+        }
+        __syncwarp();
+        if (j >= 1 && !pv(gj - 1, j - 1, I)) {
+          dead = true;
+          break;
+        }
+      }
+      if (dead) break;
+      if (!pv(g + I.nblk - 1, I.nblk - 1, I)) {
+        dead = true;
+        break;
+      }
+      if (lane == 0) mbar_arrive(&item_empty[sl]);
+      g += I.nblk;
+      ++it;
+    }
+    // every MMA issued above has completed before TMEM is freed
+    if (lane == 0) {
+      umma_commit(drain);
+      mbar_wait_bounded(drain, 0, a.st);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax warps
+    const int q4 = warp & 3;       // TMEM lane quarter this warp may access
+    const int r = q4 * 32 + lane;  // this thread's row: token r / G, query head r % G of the item's group
+    const uint32_t lane_off = uint32_t(q4 * 32) << 16;
+    const float sl2 = a.scale_log2;
+    const float sc = sl2 > 0.f ? sl2 : 1.f;  // the scale still to apply after masking (log2 units)
+    unsigned char* prow = pbuf + r * 128;
+    uint32_t g = 0;
+    int it = 0;
+    bool dead = false;
+    while (!dead) {
+      const int sl = it & 1;
+      if (!mbar_wait_bounded(&item_full[sl], (it >> 1) & 1, a.st)) dead = true;
+      dead = __any_sync(0xffffffffu, dead);
+      if (dead) break;
+      const int nblk = s_item[sl].nblk;
+      if (nblk == 0) break;
+      const int nt = s_item[sl].nt;
+      // last key of the range this row sees (a row past the tile's tokens: none)
+      const int lim = r / G < nt ? s_item[sl].lim0 + s_item[sl].causal * (r / G) : -1;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nblk; ++j) {
+        const uint32_t gj = g + j;
+        if (!mbar_wait_bounded(s_full, gj & 1, a.st)) dead = true;
+        dead = __any_sync(0xffffffffu, dead);
+        if (dead) break;
+        tc_fence_after();
+        uint32_t sr[64];
+        tmem_ld64(tbase + lane_off, sr);
+        tc_fence_before();
+        mbar_arrive(s_free);  // S_{j+1} may overwrite S now
+        const int kb0 = j * TC_KB;
+        if (sl2 <= 0.f) {  // a non-positive scale: scale first so the masked -inf stays the minimum
+#pragma unroll
+          for (int i = 0; i < 64; ++i) sr[i] = __float_as_uint(__uint_as_float(sr[i]) * sl2);
+        }
+        if (kb0 + TC_KB - 1 > lim) {  // the block reaches past this row's last visible key
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (kb0 + i > lim) sr[i] = __float_as_uint(-INFINITY);
+        }
+        float mx;
+        {
+          float t[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) t[u] = __uint_as_float(sr[u]);
+#pragma unroll
+          for (int i = 8; i < 64; i += 2)
+            t[(i >> 1) & 7] = max3f(t[(i >> 1) & 7], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+          mx = max3f(max3f(t[0], t[1], t[2]), max3f(t[3], t[4], t[5]), fmaxf(t[6], t[7]));
+        }
+        mx = mx * sc;  // -inf stays -inf (sc > 0)
+        const float mn = fmaxf(m, mx);
+        float m_new = m;
+        if (mn != -INFINITY && (m == -INFINITY || mn > m + TC_RESCALE)) m_new = mn;
+        const bool resc = (m_new != m) && (m != -INFINITY);  // earlier blocks already added to O
+        const float alpha = resc ? ex2(m - m_new) : 1.f;
+        l *= alpha;
+        m = m_new;
+        // P.V_{j-1} done: the P tile is free and O holds every earlier block
+        if (gj >= 1 && !mbar_wait_bounded(pv_done, (gj - 1) & 1, a.st)) dead = true;
+        dead = __any_sync(0xffffffffu, dead);
+        if (dead) break;
+        const float mu = m == -INFINITY ? 0.f : m;
+        tl_exp64_smem<T>(sr, f32x2(sc, sc), f32x2(-mu, -mu), l, prow, r);
+        fence_proxy_async_smem();  // P (generic-proxy stores) -> the P.V MMA (async proxy)
+        if (__any_sync(0xffffffffu, resc)) {
+          tc_fence_after();
+          tl_rescale_o(tO + lane_off, alpha);
+        }
+        tc_fence_before();
+        mbar_arrive(p_full);
+      }
+      if (dead) break;
+      // ---- epilogue: O / l of the item -> its piece rows in fp32 (or out in the
+      // pool dtype), staged through this warp's own rows of the P tile (the
+      // item's last P.V completed) 32 columns at a time, so that the stores are
+      // whole 128-byte lines
+      const uint32_t gl = g + nblk - 1;
+      if (!mbar_wait_bounded(pv_done, gl & 1, a.st)) dead = true;
+      dead = __any_sync(0xffffffffu, dead);
+      if (dead) break;
+      tc_fence_after();
+      const int h = s_item[sl].h, t0 = s_item[sl].t0, piece = s_item[sl].piece;
+      const bool zero = s_item[sl].zero != 0;
+      const float inv = (l > 0.f && !zero) ? 1.f / l : 0.f;
+      uint32_t o[64];
+      tmem_ld64(tO + lane_off, o);
+      tc_fence_before();
+      mbar_arrive(o_free);           // O read: the next item's first P.V may overwrite it
+      mbar_arrive(&item_empty[sl]);  // and the item's fields
+#pragma unroll
+      for (int i = 0; i < 64; ++i)  // rows that saw nothing, or a bad page: zeros
+        o[i] = __float_as_uint(inv == 0.f ? 0.f : __uint_as_float(o[i]) * inv);
+      if (piece >= 0) {
+        if (r / G < nt)
+          __stcg(a.part_ml + int64_t(piece + r / G) * a.n_heads + h * G + r % G,
+                 make_float2(m == -INFINITY || zero ? -1e30f : m, zero ? 0.f : l));
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) =
+                make_uint4(o[half * 32 + c * 4], o[half * 32 + c * 4 + 1], o[half * 32 + c * 4 + 2],
+                           o[half * 32 + c * 4 + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const int rw = q4 * 32 + 4 * kk + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(pbuf + rw * 128 + (((lane & 7) ^ (rw & 7)) << 4));
+            if (rw / G < nt)
+              __stcg(reinterpret_cast<uint4*>(a.part_o + (int64_t(piece + rw / G) * a.n_heads + h * G + rw % G) * TC_D +
+                                              half * 32) + (lane & 7), v);
+          }
+          __syncwarp();
+        }
+      } else {
+        T* out = static_cast<T*>(a.out);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int e = c * 8;
+          uint4 v;
+          v.x = MmaOp<T>::pack(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+          v.y = MmaOp<T>::pack(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+          v.z = MmaOp<T>::pack(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]));
+          v.w = MmaOp<T>::pack(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
+          *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = v;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const int rw = q4 * 32 + 4 * kk + (lane >> 3);
+          const uint4 v = *reinterpret_cast<const uint4*>(pbuf + rw * 128 + (((lane & 7) ^ (rw & 7)) << 4));
+          if (rw / G < nt)
+            reinterpret_cast<uint4*>(out + (int64_t(t0 + rw / G) * a.n_heads + h * G + rw % G) * TC_D)[lane & 7] = v;
+        }
+        __syncwarp();
+      }
+      g += nblk;
+      ++it;
+    }
+  }
+
+  // ---- free tensor memory once every role is done with it
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(SH_TMEM_COLS)
+                 : "memory");
+  }
+  if (threadIdx.x == 0) tl_count_exit(a.claim);
+}
+
+size_t sh_smem() { return 1024 + 2 * size_t(TC_QTILE) + size_t(2 * SH_NST) * TC_KTILE + 256; }
+
+// ---------------------------------------------------------------- merge
+// Rows of several-token sequences of shared groups: one warp per (token, query
+// head) merges the row's prefix pieces and its own.
+template <typename T>
+__global__ void __launch_bounds__(256) shared_merge_kernel(const int4* fold, const int4* rest, const float* part_o,
+                                                           const float2* part_ml, void* out, int n_tokens,
+                                                           int n_heads) {
+  const int64_t w = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (w >= int64_t(n_tokens) * n_heads) {
+    pdl_wait();
+    return;
+  }
+  const int t = int(w / n_heads), hh = int(w % n_heads);
+  const int4 b = __ldcg(rest + t);  // the plan's: complete before any kernel of the step started
+  const int4 f = __ldcg(fold + t);
+  pdl_wait();
+  if (b.y <= 0) return;  // a one-token row or one written straight to out
+  float M = -1e30f, L = 0.f, y0 = 0.f, y1 = 0.f;
+  for (int i = 0; i < f.y + b.y; ++i) {
+    const int64_t p = i < f.y ? int64_t(f.x) + int64_t(i) * f.z : int64_t(b.x) + int64_t(i - f.y) * b.z;
+    const float2 ml = __ldcg(part_ml + p * n_heads + hh);
+    const float2 v = __ldcg(reinterpret_cast<const float2*>(part_o + (p * n_heads + hh) * TC_D) + lane);
+    const float Mn = fmaxf(M, ml.x);
+    const float c = ex2(M - Mn), k = ml.y * ex2(ml.x - Mn);
+    y0 = y0 * c + k * v.x;
+    y1 = y1 * c + k * v.y;
+    L = L * c + k;
+    M = Mn;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  reinterpret_cast<uint32_t*>(static_cast<T*>(out) + (int64_t(t) * n_heads + hh) * TC_D)[lane] =
+      MmaOp<T>::pack(y0 * inv, y1 * inv);
+}
+
+// ---------------------------------------------------------------- host
+int check_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* b) {
+  if (int rc = check_pool(pool)) return rc;
+  if (!b) return fail(PKV_ERR_ARG, "batch descriptor is NULL");
+  if (n_heads <= 0 || n_heads % pool->n_kv_heads)
+    return fail(PKV_ERR_ARG, "n_heads must be a positive multiple of n_kv_heads");
+  if (!decode_fold_supported(*pool, n_heads))
+    return fail(PKV_ERR_UNSUPPORTED, "shared-prefix attention takes fp16 / bf16 pools, head_dim 64, 16-token pages, "
+                                     "up to 8 KV heads and 1, 2, 4 or 8 query heads per KV head");
+  if (b->n_seqs <= 0) return fail(PKV_ERR_ARG, "batch has no sequences");
+  if (b->n_tokens < 0 || b->total_pages < 0 || b->total_pages >= (int64_t(1) << 31) || b->n_seqs >= (1 << 24))
+    return fail(PKV_ERR_ARG, "bad batch sizes");
+  if (!b->cu_query_lens || !b->kv_indptr || !b->kv_last_page_len || (b->total_pages && !b->kv_indices))
+    return fail(PKV_ERR_ARG, "batch CSR pointers must be non-NULL");
+  return PKV_OK;
+}
+
+template <typename T, int G>
+int launch_shared_t(const CUtensorMap& tm, const CUtensorMap& qm, const ShArgs& a, int grid, cudaStream_t s) {
+  static std::mutex mu;
+  static std::vector<char> ready;
+  int dev = 0;
+  PKV_CUDA_RET(cudaGetDevice(&dev));
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if ((int)ready.size() <= dev) ready.resize(dev + 1, 0);
+    if (!ready[dev]) {
+      PKV_CUDA_RET(cudaFuncSetAttribute(shared_tc_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        int(sh_smem())));
+      // three CTAs of ~67 KiB need the whole shared-memory carveout
+      PKV_CUDA_RET(cudaFuncSetAttribute(shared_tc_kernel<T, G>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                        int(cudaSharedmemCarveoutMaxShared)));
+      ready[dev] = 1;
+    }
+  }
+  PKV_CUDA_RET(launch_kernel(shared_tc_kernel<T, G>, dim3(grid), dim3(TC_THREADS), sh_smem(), s, true, tm, qm, a));
+  return PKV_OK;
+}
+
+template <typename T>
+int launch_shared_g(int groups, const CUtensorMap& tm, const CUtensorMap& qm, const ShArgs& a, int grid,
+                    cudaStream_t s) {
+  switch (groups) {
+    case 1: return launch_shared_t<T, 1>(tm, qm, a, grid, s);
+    case 2: return launch_shared_t<T, 2>(tm, qm, a, grid, s);
+    case 4: return launch_shared_t<T, 4>(tm, qm, a, grid, s);
+    case 8: return launch_shared_t<T, 8>(tm, qm, a, grid, s);
+  }
+  return fail(PKV_ERR_UNSUPPORTED, "shared-prefix attention: unsupported GQA group size");
+}
+
+}  // namespace
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" size_t pkv_shared_workspace_size(const pkv_pool* pool, int32_t n_heads, int32_t n_seqs, int32_t n_tokens,
+                                            int64_t total_pages) {
+  if (!pool || pool->n_kv_heads <= 0 || n_heads < pool->n_kv_heads || n_seqs <= 0 || n_tokens < 0 || total_pages < 0)
+    return 0;
+  return sh_layout(n_heads, std::min(8, n_heads / pool->n_kv_heads), n_seqs, n_tokens, total_pages).total;
+}
+
+extern "C" int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* batch, int32_t n_groups,
+                               const int32_t* group_indptr, const int32_t* prefix_pages, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (int rc = check_shared(pool, n_heads, batch)) return rc;
+  if (n_groups <= 0 || n_groups > batch->n_seqs)
+    return fail(PKV_ERR_ARG, "n_groups must be between 1 and the number of sequences");
+  if (!group_indptr || !prefix_pages) return fail(PKV_ERR_ARG, "group_indptr and prefix_pages must be non-NULL");
+  const int groups = n_heads / pool->n_kv_heads;
+  const ShLayout w = sh_layout(n_heads, groups, batch->n_seqs, batch->n_tokens, batch->total_pages);
+  if (!workspace || workspace_bytes < w.total)
+    return fail(PKV_ERR_ARG, "workspace too small: need " + std::to_string(w.total) + " bytes");
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(PKV_ERR_ARG, "workspace must be 256-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  PlanArgs a;
+  a.cu_q = batch->cu_query_lens;
+  a.kv_lens = batch->kv_lens;
+  a.kv_indptr = batch->kv_indptr;
+  a.kv_indices = batch->kv_indices;
+  a.last_page_len = batch->kv_last_page_len;
+  a.group_indptr = group_indptr;
+  a.prefix_pages = prefix_pages;
+  a.st = batch->dev_status;
+  a.num_blocks = pool->num_blocks;
+  a.total_pages = batch->total_pages;
+  a.n_seqs = batch->n_seqs;
+  a.n_tokens = batch->n_tokens;
+  a.n_groups = n_groups;
+  a.n_kv = pool->n_kv_heads;
+  a.tpt = TC_ROWS / groups;
+  a.slots = SH_MINB * num_sms();
+  a.splits_cap = split_cap(batch->n_tokens);
+  a.pieces_cap = w.pieces;
+  a.items_cap = w.items_cap;
+  a.ctl = reinterpret_cast<ShCtl*>(ws + w.ctl);
+  a.rows = reinterpret_cast<int32_t*>(ws + w.rows);
+  a.seq_np = reinterpret_cast<int32_t*>(ws + w.seq_np);
+  a.group_bad = reinterpret_cast<int32_t*>(ws + w.group_bad);
+  a.ents = reinterpret_cast<ShEnt*>(ws + w.ents);
+  a.items = reinterpret_cast<int4*>(ws + w.items);
+  a.fold = reinterpret_cast<int4*>(ws + w.fold);
+  a.rest = reinterpret_cast<int4*>(ws + w.rest);
+  a.desc = reinterpret_cast<int4*>(ws + w.dec.page_desc);
+  a.counters = reinterpret_cast<int32_t*>(ws + w.dec.counters);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  PKV_CUDA_RET(cudaMemsetAsync(a.group_bad, 0, sizeof(int32_t) * size_t(batch->n_seqs), s));
+  shared_check_kernel<<<unsigned(batch->n_seqs), 128, 0, s>>>(a);
+  PKV_CUDA_RET(cudaGetLastError());
+  shared_plan_kernel<<<1, 1024, 0, s>>>(a);
+  PKV_CUDA_RET(cudaGetLastError());
+  return PKV_OK;
+}
+
+extern "C" int pkv_attend_shared_planned(const pkv_pool* pool, int32_t layer, int32_t n_heads, const void* q,
+                                         void* out, float scale, const pkv_batch* batch, int32_t decode_hint,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_shared(pool, n_heads, batch)) return rc;
+  const pkv_pool& p = *pool;
+  if (layer < 0 || layer >= p.num_layers)
+    return fail(PKV_ERR_ARG, "layer_idx " + std::to_string(layer) + " out of range [0, " +
+                                 std::to_string(p.num_layers) + ")");
+  if (batch->n_tokens == 0) return PKV_OK;
+  if (!q || !out) return fail(PKV_ERR_ARG, "q and out must be non-NULL");
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
+    return fail(PKV_ERR_ARG, "q and out must be 16-byte aligned");
+  const int groups = n_heads / p.n_kv_heads;
+  const ShLayout w = sh_layout(n_heads, groups, batch->n_seqs, batch->n_tokens, batch->total_pages);
+  if (!workspace || workspace_bytes < w.total)
+    return fail(PKV_ERR_ARG, "workspace too small: need " + std::to_string(w.total) + " bytes");
+  char* ws = static_cast<char*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CUtensorMap tm, qm;
+  if (int rc = pool_tmap_head(p, &tm)) return rc;
+  if (int rc = q_tmap(p.dtype, q, batch->n_tokens, n_heads, groups, &qm)) return rc;
+  ShArgs a;
+  a.out = out;
+  a.ctl = reinterpret_cast<const ShCtl*>(ws + w.ctl);
+  a.claim = reinterpret_cast<ShCtl*>(ws + w.ctl)->claim;
+  a.ents = reinterpret_cast<const ShEnt*>(ws + w.ents);
+  a.items = reinterpret_cast<const int4*>(ws + w.items);
+  a.kv_indices = batch->kv_indices;
+  a.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+  a.st = batch->dev_status;
+  a.num_blocks = p.num_blocks;
+  a.n_heads = n_heads;
+  a.n_kv = p.n_kv_heads;
+  a.layer = layer;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const int grid = int(std::min<int64_t>(w.items_cap * p.n_kv_heads, int64_t(SH_MINB) * num_sms()));
+  int rc = p.dtype == PKV_F16 ? launch_shared_g<__half>(groups, tm, qm, a, grid, s)
+                              : launch_shared_g<__nv_bfloat16>(groups, tm, qm, a, grid, s);
+  if (rc) return rc;
+  const int4* fold = reinterpret_cast<const int4*>(ws + w.fold);
+  const int4* rest = reinterpret_cast<const int4*>(ws + w.rest);
+  if (decode_hint != 2) {  // one-token sequences
+    rc = decode_fold(p, layer, n_heads, q, out, scale, *batch, ws, reinterpret_cast<const int32_t*>(ws + w.rows),
+                     &a.ctl->p_dec, fold, a.part_o, a.part_ml, s);
+    if (rc) return rc;
+  }
+  if (decode_hint != 1) {  // several-token sequences
+    const int64_t warps = int64_t(batch->n_tokens) * n_heads;
+    const int64_t blocks = (warps * 32 + 255) / 256;
+    if (blocks >= (int64_t(1) << 31)) return fail(PKV_ERR_ARG, "too many tokens for one call");
+    auto kern = p.dtype == PKV_F16 ? shared_merge_kernel<__half> : shared_merge_kernel<__nv_bfloat16>;
+    PKV_CUDA_RET(launch_kernel(kern, dim3(unsigned(blocks)), dim3(256), 0, s, true, fold, rest,
+                               static_cast<const float*>(a.part_o), static_cast<const float2*>(a.part_ml), out,
+                               batch->n_tokens, n_heads));
+  }
+  return PKV_OK;
+}
