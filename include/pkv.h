@@ -252,16 +252,21 @@ PKV_API int pkv_page_index_rebuild(const pkv_pool* pool, const pkv_page_index* i
  * listed pages up to the query's position (pages read as given when not
  * selected; entries outside the sequence's pages up to the query's own are
  * skipped, a page listed twice counts twice, nothing listed gives zeros).
- * fp16, bf16 or fp32 pools, head_dim up to 256; batch_indices [n_tokens] is
- * BatchMeta's; max_pages bounds the pages of any sequence of the batch
- * (PKV_DEV_META_BAD and zeros for a longer one; PKV_ERR_UNSUPPORTED when a
- * list does not fit in shared memory, about 50000 pages). One launch. */
+ * fp16, bf16 or fp32 pools, head_dim up to 256. One launch; `rows` is the
+ * step's plan (every layer uses it): int4 [n_tokens], device, 16-byte aligned,
+ * written by pkv_plan_sparse, where batch_indices [n_tokens] is BatchMeta's and
+ * max_pages bounds the pages of any sequence of the batch (tokens of a longer
+ * one, or of one whose tables are inconsistent, set PKV_DEV_META_BAD, and
+ * their rows are zeros and -1; PKV_ERR_UNSUPPORTED when a list does not fit in
+ * shared memory, about 50000 pages). */
 #define PKV_SPARSE_SELECT 1
 #define PKV_SPARSE_ATTEND 2
+PKV_API int pkv_plan_sparse(const pkv_pool* pool, const pkv_batch* batch, const int32_t* batch_indices,
+                            int32_t max_pages, void* rows, void* stream);
 PKV_API int pkv_attend_sparse(const pkv_pool* pool, const pkv_page_index* index, int32_t layer, int32_t n_heads,
                               const void* q, void* out, int32_t* pages, float scale, int32_t budget, int32_t sink,
-                              int32_t recent, const pkv_batch* batch, const int32_t* batch_indices,
-                              int32_t max_pages, int32_t mode, void* stream);
+                              int32_t recent, const pkv_batch* batch, const void* rows, int32_t max_pages,
+                              int32_t mode, void* stream);
 
 /* ---- shared-prefix attention --------------------------------------------------
  * pkv_attend for a batch whose sequences come in n_groups consecutive groups
@@ -272,17 +277,16 @@ PKV_API int pkv_attend_sparse(const pkv_pool* pool, const pkv_page_index* index,
  * kv_len - query_len; page lists that disagree are computed without sharing and
  * set PKV_DEV_META_BAD. The plan is made once per step and reused by every
  * layer with the same batch and workspace (device, 256-byte aligned, of
- * pkv_shared_workspace_size bytes). decode_hint as pkv_attend: 1 every query
- * length is 1, 2 none is, 0 unknown. Geometry of the decode kernel only
- * (PKV_ERR_UNSUPPORTED otherwise: use pkv_attend). */
+ * pkv_shared_workspace_size bytes). Two launches per layer. Geometry of the
+ * decode kernel only (PKV_ERR_UNSUPPORTED otherwise: use pkv_attend). */
 PKV_API size_t pkv_shared_workspace_size(const pkv_pool* pool, int32_t n_heads, int32_t n_seqs, int32_t n_tokens,
                                          int64_t total_pages);
 PKV_API int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* batch, int32_t n_groups,
                             const int32_t* group_indptr, const int32_t* prefix_pages, void* workspace,
                             size_t workspace_bytes, void* stream);
 PKV_API int pkv_attend_shared_planned(const pkv_pool* pool, int32_t layer, int32_t n_heads, const void* q, void* out,
-                                      float scale, const pkv_batch* batch, int32_t decode_hint, void* workspace,
-                                      size_t workspace_bytes, void* stream);
+                                      float scale, const pkv_batch* batch, void* workspace, size_t workspace_bytes,
+                                      void* stream);
 
 /* Which kernel pkv_attend_planned runs for a batch of this shape and hint
  * (host only, nothing touches the device): PKV_KERNEL_GENERIC,

@@ -34,7 +34,7 @@ class SharedPlan:
     used by every layer of the step. Holds the step's tables and a workspace of
     its own (``workspace`` may be passed on to the next step's plan)."""
 
-    __slots__ = ("meta", "n_tokens", "hint", "batch", "batch_ref", "tensors", "workspace", "ws_ptr", "ws_bytes")
+    __slots__ = ("meta", "n_tokens", "batch", "batch_ref", "tensors", "workspace", "ws_ptr", "ws_bytes")
 
 
 class SparsePlan:
@@ -42,7 +42,7 @@ class SparsePlan:
     used by every layer of the step."""
 
     __slots__ = ("index", "budget", "sink", "recent", "max_pages", "n_tokens", "batch", "batch_ref", "tensors",
-                 "batch_indices_ptr")
+                 "rows_ptr")
 
 
 class B200PagedBackend:
@@ -318,71 +318,87 @@ class B200PagedBackend:
         ``interleaved``. Same bits as ``rope`` followed by ``append_kv``.
         ``index`` (a ``PageIndex`` of this backend): the entries of the pages
         this step completes are written too. fp16, bf16 or fp32 pools."""
-        cos, sin = self._rope_tables(rope, None)
-        rotary = 2 * cos.shape[1]
-        if rotary > self.head_dim:
-            raise ValueError(f"the rope tables turn {rotary} dims of heads of {self.head_dim}")
-        self._check_layer(layer_idx)
-        if getattr(meta, "slot_mapping", None) is None or getattr(meta, "positions", None) is None:
+        # the checks of every call in their cheapest form; the tables' refusal is worded by a helper
+        dev, D, Hk = self._dev_index, self.head_dim, self.n_kv_heads
+        try:
+            cos, sin = rope
+            rows, half = shape = cos.shape
+            ok = (half > 0 and rows > 0 and sin.shape == shape and cos.dtype is sin.dtype is torch.float32
+                  and cos.get_device() == sin.get_device() == dev and cos.is_contiguous() and sin.is_contiguous())
+        except (TypeError, ValueError, AttributeError):
+            ok = False
+        if not ok:
+            self._refuse_rope_tables(rope)
+        if 2 * half > D:
+            raise ValueError(f"the rope tables turn {2 * half} dims of heads of {D}")
+        if layer_idx is None or not 0 <= layer_idx < self.num_layers:
+            self._check_layer(layer_idx)
+        slots, pos = meta.slot_mapping, meta.positions
+        if slots is None or pos is None:
             raise ValueError("rope_append requires meta.slot_mapping and meta.positions")
-        tokens = k.shape[0]
-        if k.shape != (tokens, self.n_kv_heads, self.head_dim):
-            raise ValueError(f"k has shape {tuple(k.shape)}, expected ({tokens}, {self.n_kv_heads}, {self.head_dim})")
-        if v.shape != k.shape:
-            raise ValueError(f"v shape {tuple(v.shape)} != k shape {tuple(k.shape)}")
-        if q is not None and q.shape != (tokens, self.n_heads, self.head_dim):
-            raise ValueError(f"q has shape {tuple(q.shape)}, expected ({tokens}, {self.n_heads}, {self.head_dim})")
-        for name in ("slot_mapping", "positions"):
-            if getattr(meta, name).shape != (tokens,):
-                raise ValueError(f"{name} has {getattr(meta, name).shape[0]} entries but {tokens} tokens were supplied")
+        shape = k.shape
+        tokens = shape[0]
+        if shape != (tokens, Hk, D):
+            raise ValueError(f"k has shape {tuple(shape)}, expected ({tokens}, {Hk}, {D})")
+        if v.shape != shape:
+            raise ValueError(f"v shape {tuple(v.shape)} != k shape {tuple(shape)}")
+        if slots.shape != (tokens,) or pos.shape != (tokens,):
+            raise ValueError(f"slot_mapping has {slots.shape[0]} entries and positions {pos.shape[0]} but {tokens} "
+                             "tokens were supplied")
         if index is not None and index.backend is not self:
             raise ValueError("index belongs to another backend")
-        k, v = self._rows(k), self._rows(v)
+        k, k_stride = self._rows(k, Hk * D)
+        v, v_stride = self._rows(v, Hk * D)
+        q_ptr = qo_ptr = None
+        q_stride = heads = 0
         if q is not None:
-            q = self._rows(q)
+            heads = self.n_heads
+            if q.shape != (tokens, heads, D):
+                raise ValueError(f"q has shape {tuple(q.shape)}, expected ({tokens}, {heads}, {D})")
+            q, q_stride = self._rows(q, heads * D)
             if q_out is None:
-                q_out = torch.empty((tokens, self.n_heads, self.head_dim), dtype=self.dtype, device=self.device)
-            elif (q_out.shape != q.shape or q_out.dtype != self.dtype or not q_out.is_cuda
-                  or q_out.get_device() != self._dev_index or not q_out.is_contiguous()):
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            elif (q_out.shape != q.shape or q_out.dtype != self.dtype or q_out.get_device() != dev
+                  or not q_out.is_contiguous()):
                 raise ValueError(f"q_out must be a contiguous {tuple(q.shape)} {self.dtype} tensor on {self.device}")
             elif _overlap(q_out, q) and not (q_out.data_ptr() == q.data_ptr() and q.is_contiguous()):
                 raise ValueError("q_out overlaps q without being q")
+            q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out given without q")
-        if tokens == 0:
+        if not tokens:
             return q_out
-        slots, pos = self._i32(meta.slot_mapping), self._own(meta.positions, torch.int64)
-        N.check(self._lib.pkv_rope_append(
-            self._pdesc, layer_idx, N.ptr(q), 0 if q is None else q.stride(0), N.ptr(q_out),
-            0 if q is None else self.n_heads, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slots.data_ptr(),
-            pos.data_ptr(), tokens, cos.data_ptr(), sin.data_ptr(), cos.shape[0], rotary, int(interleaved),
-            None if index is None else index._pdesc, self._status_ptr, N.raw_stream(self._dev_index)), "rope_append")
+        slots, pos = self._dev_vec(slots, torch.int32), self._dev_vec(pos, torch.int64)
+        rc = self._lib.pkv_rope_append(
+            self._pdesc, layer_idx, q_ptr, q_stride, qo_ptr, heads, k.data_ptr(), k_stride, v.data_ptr(), v_stride,
+            slots.data_ptr(), pos.data_ptr(), tokens, cos.data_ptr(), sin.data_ptr(), rows, 2 * half, interleaved,
+            None if index is None else index._pdesc, self._status_ptr, N.raw_stream(self._dev_index))
+        if rc:
+            N.check(rc, "rope_append")
         return q_out
 
-    def _rope_tables(self, rope, half):
+    def _refuse_rope_tables(self, rope):
         try:
             cos, sin = rope
         except (TypeError, ValueError):
             raise ValueError("rope must be a (cos, sin) pair of tensors") from None
-        for t, name in ((cos, "cos"), (sin, "sin")):
-            if (not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] < 1 or t.shape[1] < 1
-                    or (half is not None and t.shape[1] != half) or t.dtype != torch.float32 or not t.is_cuda
-                    or t.get_device() != self._dev_index or not t.is_contiguous()):
-                raise ValueError(f"rope {name} must be a contiguous float32 [max_pos, dims] tensor on {self.device}")
-        if cos.shape != sin.shape:
-            raise ValueError(f"rope cos {tuple(cos.shape)} and sin {tuple(sin.shape)} differ in shape")
-        return cos, sin
+        raise ValueError(f"rope cos and sin must be contiguous float32 [max_pos, rotary_dim // 2] tensors of one shape "
+                         f"on {self.device}")
 
-    def _rows(self, t: torch.Tensor) -> torch.Tensor:
-        """t on this device in the pool dtype with each token's row contiguous
-        (no op for slices of a fused projection)."""
-        if (t.is_cuda and t.dtype == self.dtype and t.get_device() == self._dev_index and t.stride(2) == 1
-                and (t.stride(1) == t.shape[2] or t.shape[1] == 1)
-                and (t.stride(0) >= t.shape[1] * t.shape[2] or t.shape[0] <= 1)):
-            if t.shape[0] <= 1 and t.stride(0) < t.shape[1] * t.shape[2]:
-                return t.contiguous()
+    def _rows(self, t: torch.Tensor, row: int) -> tuple[torch.Tensor, int]:
+        """t ``(T, heads, head_dim)`` on this device in the pool dtype with each
+        token's ``row`` elements contiguous (no copy for slices of a fused
+        projection), and the elements from token to token."""
+        st = t.stride()
+        if t.dtype is self.dtype and t.get_device() == self._dev_index and st[2] == 1 and st[0] >= row \
+                and (st[1] == self.head_dim or row == self.head_dim):
+            return t, st[0]
+        return t.to(device=self.device, dtype=self.dtype).contiguous(), row
+
+    def _dev_vec(self, t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+        if t.dtype is dtype and t.get_device() == self._dev_index and t.is_contiguous():
             return t
-        return t.to(device=self.device, dtype=self.dtype).contiguous()
+        return t.to(device=self.device, dtype=dtype).contiguous()
 
     def _rope_args(self, rope, meta):
         try:
@@ -482,12 +498,9 @@ class B200PagedBackend:
             raise ValueError(f"the groups hold {shared.n_seqs} sequences but the batch has {n}")
         plan = SharedPlan()
         self._plan_batch(plan, meta)
-        mql, mnql = getattr(meta, "max_query_len", None), getattr(meta, "min_query_len", None)
-        plan.hint = 1 if plan.n_tokens == n and mql == 1 else (2 if mnql is not None and int(mnql) > 1 else 0)
         plan.meta = None
         if self.validate == "host":
-            decode, hint = self._host_validate(meta, n, int(meta.kv_indices.shape[0]))
-            plan.hint = hint
+            self._host_validate(meta, n, int(meta.kv_indices.shape[0]))
             self._validate_shared(meta, shared)
         bounds = [0]
         for size in shared.group_sizes:
@@ -517,15 +530,17 @@ class B200PagedBackend:
         ``attend`` itself."""
         if plan.meta is not None:
             return self.attend(q, layer_idx, scale, plan.meta, out=out)
-        self._check_layer(layer_idx)
-        self._check_q(q, plan.n_tokens)
-        q = self._own(q, self.dtype)
-        out = self._out(q, out)
-        if plan.n_tokens == 0:
+        if layer_idx is None or not 0 <= layer_idx < self.num_layers:
+            self._check_layer(layer_idx)
+        q = self._query(q, plan.n_tokens)
+        out = torch.empty_like(q) if out is None else self._out(q, out)
+        if not plan.n_tokens:
             return out
-        N.check(self._lib.pkv_attend_shared_planned(
-            self._pdesc, layer_idx, self.n_heads, q.data_ptr(), out.data_ptr(), float(scale), plan.batch_ref,
-            plan.hint, plan.ws_ptr, plan.ws_bytes, N.raw_stream(self._dev_index)), "attend_shared")
+        rc = self._lib.pkv_attend_shared_planned(
+            self._pdesc, layer_idx, self.n_heads, q.data_ptr(), out.data_ptr(), scale, plan.batch_ref,
+            plan.ws_ptr, plan.ws_bytes, N.raw_stream(self._dev_index))
+        if rc:
+            N.check(rc, "attend_shared")
         self.n_runs += 1
         self.last_kernel = "shared"
         return out
@@ -566,8 +581,6 @@ class B200PagedBackend:
             self._host_validate(meta, int(meta.query_lens.shape[0]), int(meta.kv_indices.shape[0]))
         if getattr(meta, "batch_indices", None) is None or meta.batch_indices.shape != (plan.n_tokens,):
             raise ValueError(f"plan_sparse needs meta.batch_indices with {plan.n_tokens} entries")
-        plan.tensors["bi"] = self._copy_i32(meta.batch_indices)
-        plan.batch_indices_ptr = plan.tensors["bi"].data_ptr()
         if max_pages is None:
             ip = plan.tensors["ip"]
             max_pages = int((ip[1:] - ip[:-1]).max())
@@ -575,6 +588,11 @@ class B200PagedBackend:
             raise ValueError(f"max_pages must be positive, got {max_pages}")
         plan.index, plan.budget, plan.sink, plan.recent = index, budget, sink, recent
         plan.max_pages = int(max_pages)
+        bi = self._i32(meta.batch_indices)
+        rows = plan.tensors["rows"] = torch.empty((plan.n_tokens, 4), dtype=torch.int32, device=self.device)
+        plan.rows_ptr = rows.data_ptr()
+        N.check(self._lib.pkv_plan_sparse(self._pdesc, plan.batch_ref, bi.data_ptr(), plan.max_pages, plan.rows_ptr,
+                                          N.raw_stream(self._dev_index)), "plan_sparse")
         return plan
 
     def attend_sparse(self, q: torch.Tensor, layer_idx: int, scale: float, plan: SparsePlan, *,
@@ -600,24 +618,28 @@ class B200PagedBackend:
         return self._sparse(q, layer_idx, scale, plan, out, pages, N.SPARSE_ATTEND)[0]
 
     def _sparse(self, q, layer_idx, scale, plan, out, pages, mode):
-        self._check_layer(layer_idx)
-        self._check_q(q, plan.n_tokens)
-        q = self._own(q, self.dtype)
-        shape = (plan.n_tokens, self.n_kv_heads, plan.budget)
+        if layer_idx is None or not 0 <= layer_idx < self.num_layers:
+            self._check_layer(layer_idx)
+        q = self._query(q, plan.n_tokens)
         if pages is None and mode & N.SPARSE_SELECT:
-            pages = torch.empty(shape, dtype=torch.int32, device=self.device)
-        elif (pages is None or pages.shape != shape or pages.dtype != torch.int32 or not pages.is_cuda
-              or pages.get_device() != self._dev_index or not pages.is_contiguous()):
-            raise ValueError(f"pages must be a contiguous int32 {shape} tensor on {self.device}")
+            pages = torch.empty((plan.n_tokens, self.n_kv_heads, plan.budget), dtype=torch.int32, device=self.device)
+        elif (pages is None or pages.shape != (plan.n_tokens, self.n_kv_heads, plan.budget)
+              or pages.dtype != torch.int32 or pages.get_device() != self._dev_index or not pages.is_contiguous()):
+            raise ValueError(f"pages must be a contiguous int32 {(plan.n_tokens, self.n_kv_heads, plan.budget)} "
+                             f"tensor on {self.device}")
+        out_ptr = None
         if mode & N.SPARSE_ATTEND:
-            out = self._out(q, out)
-        if plan.n_tokens == 0:
+            out = torch.empty_like(q) if out is None else self._out(q, out)
+            out_ptr = out.data_ptr()
+        if not plan.n_tokens:
             return out, pages
-        N.check(self._lib.pkv_attend_sparse(
-            self._pdesc, plan.index._pdesc, layer_idx, self.n_heads, q.data_ptr(), N.ptr(out), pages.data_ptr(),
-            float(scale), plan.budget, plan.sink, plan.recent, plan.batch_ref, plan.batch_indices_ptr, plan.max_pages,
-            mode, N.raw_stream(self._dev_index)), "attend_sparse")
-        if mode & N.SPARSE_ATTEND:
+        rc = self._lib.pkv_attend_sparse(
+            self._pdesc, plan.index._pdesc, layer_idx, self.n_heads, q.data_ptr(), out_ptr, pages.data_ptr(), scale,
+            plan.budget, plan.sink, plan.recent, plan.batch_ref, plan.rows_ptr, plan.max_pages, mode,
+            N.raw_stream(self._dev_index))
+        if rc:
+            N.check(rc, "attend_sparse")
+        if out_ptr:
             self.n_runs += 1
             self.last_kernel = "sparse"
         return out, pages
@@ -642,9 +664,13 @@ class B200PagedBackend:
             t["ix"].data_ptr() if total_pages else None, t["lp"].data_ptr(), self._status_ptr)
         plan.batch_ref = ctypes.byref(plan.batch)
 
-    def _check_q(self, q: torch.Tensor, tokens: int) -> None:
+    def _query(self, q: torch.Tensor, tokens: int) -> torch.Tensor:
+        """q checked against the plan's tokens, contiguous in the pool dtype on this device."""
         if q.shape != (tokens, self.n_heads, self.head_dim):
             raise ValueError(f"q has shape {tuple(q.shape)}, expected ({tokens}, {self.n_heads}, {self.head_dim})")
+        if q.dtype is self.dtype and q.get_device() == self._dev_index and q.is_contiguous():
+            return q
+        return q.to(device=self.device, dtype=self.dtype).contiguous()
 
     def _copy_i32(self, t: torch.Tensor) -> torch.Tensor:
         return t.to(device=self.device, dtype=torch.int32, copy=True).contiguous()

@@ -39,6 +39,7 @@ struct RopeAppendArgs {
   int64_t n_tokens, n_slots, max_pos;
   int hq, hkv, d, half;  // half = rotated pairs per head
   int wpt;               // warps per token
+  int cols;              // lanes side by side on a head's columns (vectors): a power of two
 };
 
 template <typename T>
@@ -58,106 +59,120 @@ __device__ __forceinline__ uint4 pack_vec(const float (&f)[16 / sizeof(T)]) {
     return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
 }
 
-// VE elements per unit (16 bytes, or 1 where alignment or sizes do not allow
-// vectors). A token's units: for each rotated head VE pairs at a time, the
-// pass-through dims, then v; wpt warps share a token's units.
+// One token's work, shared by wpt warps. VECTOR: 16-byte vectors of VE
+// elements; a lane owns one column of VE pairs (its cosines and sines stay in
+// registers) and steps over the heads, UB of them loaded before the first is
+// stored, so that a token's rows travel together. Otherwise single elements.
 template <typename T, bool VECTOR, bool INTER>
 __global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a) {
   constexpr int VE = VECTOR ? 16 / int(sizeof(T)) : 1;
+  constexpr int UB = 4;
+  using V = typename std::conditional<VECTOR, uint4, T>::type;
   pdl_trigger();
   pdl_wait();  // q, k, v, positions and slots may come from the kernels just before
   const int lane = threadIdx.x & 31;
   const int64_t warp = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int64_t t = warp / a.wpt;
   if (t >= a.n_tokens) return;
-  const int u0 = int(warp % a.wpt) * 32 + lane, du = a.wpt * 32;
+  const int u0 = int(warp - t * a.wpt) * 32 + lane, du = a.wpt * 32;
   const int64_t pos = a.positions[t], slot = a.slots[t];
   const bool turn = pos >= 0 && pos < a.max_pos;
   const bool store = slot >= 0 && slot < a.n_slots;
+  const int d = a.d, half = a.half, heads = a.hq + a.hkv;
+  const int64_t row = int64_t(a.hkv) * d * sizeof(T);
+  const T* q = reinterpret_cast<const T*>(a.q + t * a.q_stride);
+  const T* k = reinterpret_cast<const T*>(a.k + t * a.k_stride);
+  T* qo = reinterpret_cast<T*>(a.q_out + t * a.qo_stride);
+  T* ko = reinterpret_cast<T*>(a.k_slab + (store ? slot * row : 0));
+  // the token's v: its first vectors are loaded now and stored last
+  const V* vs = reinterpret_cast<const V*>(a.v + t * a.v_stride);
+  const int nv = a.hkv * d / VE;
+  V vv[UB];
+#pragma unroll
+  for (int b = 0; b < UB; ++b)
+    if (u0 + b * du < nv) vv[b] = vs[u0 + b * du];
   if (u0 == 0) {
     if (!turn) flag(a.st, PKV_DEV_META_BAD);
     if (!store) flag(a.st, PKV_DEV_SLOT_OOB);
   }
-  const int d = a.d, half = a.half;
-  const int64_t row = int64_t(a.hkv) * d * sizeof(T);
-  const T* q = reinterpret_cast<const T*>(a.q + t * a.q_stride);
-  const T* k = reinterpret_cast<const T*>(a.k + t * a.k_stride);
-  const T* v = reinterpret_cast<const T*>(a.v + t * a.v_stride);
-  T* qo = reinterpret_cast<T*>(a.q_out + t * a.qo_stride);
-  T* ko = reinterpret_cast<T*>(a.k_slab + slot * row);
-  T* vo = reinterpret_cast<T*>(a.v_slab + slot * row);
   const float* cs = a.cs + (turn ? pos : 0) * half;
   const float* sn = a.sn + (turn ? pos : 0) * half;
-  // the head's source and destination (NULL: a key whose slot is outside the pool)
-  auto head = [&](int hh, const T*& x, T*& y) {
-    const bool isq = hh < a.hq;
-    x = isq ? q + hh * d : k + (hh - a.hq) * d;
-    y = isq ? qo + hh * d : (store ? ko + (hh - a.hq) * d : nullptr);
-  };
+  auto src = [&](int hh) -> const T* { return hh < a.hq ? q + hh * d : k + (hh - a.hq) * d; };
+  // NULL: a key whose slot is outside the pool
+  auto dst = [&](int hh) -> T* { return hh < a.hq ? qo + hh * d : (store ? ko + (hh - a.hq) * d : nullptr); };
 
-  const int cols = half / VE;  // units of VE pairs per head (host: half % VE == 0)
-  const int n_rot = (a.hq + a.hkv) * cols;
-#pragma unroll 2
-  for (int u = u0; u < n_rot; u += du) {
-    const int hh = u / cols, i = (u - hh * cols) * VE;
-    const T* x;
-    T* y;
-    head(hh, x, y);
-    if constexpr (VECTOR) {
-      // half-split: elements i.. and half + i..; interleaved: the 2 VE elements from 2 i
-      const int e0 = INTER ? 2 * i : i, e1 = INTER ? 2 * i + VE : half + i;
-      const uint4 xa = *reinterpret_cast<const uint4*>(x + e0), xb = *reinterpret_cast<const uint4*>(x + e1);
-      float c[VE], s[VE], p[VE], r[VE];
+  if constexpr (VECTOR) {
+    const int cols = half / VE;  // <= a.cols, a power of two <= 32
+    const int i = (lane & (a.cols - 1)) * VE, step = du / a.cols;
+    // half-split: elements i.. and half + i..; interleaved: the 2 VE elements from 2 i
+    const int e0 = INTER ? 2 * i : i, e1 = INTER ? 2 * i + VE : half + i;
+    const int h0 = i < cols * VE ? u0 / a.cols : heads;
+    float c[VE], s[VE];
 #pragma unroll
-      for (int e = 0; e < VE; e += 4) {
-        const float4 cv = __ldg(reinterpret_cast<const float4*>(cs + i + e));
-        const float4 sv = __ldg(reinterpret_cast<const float4*>(sn + i + e));
-        c[e] = cv.x; c[e + 1] = cv.y; c[e + 2] = cv.z; c[e + 3] = cv.w;
-        s[e] = sv.x; s[e + 1] = sv.y; s[e + 2] = sv.z; s[e + 3] = sv.w;
-      }
-      unpack_vec<T>(xa, p);
-      unpack_vec<T>(xb, r);
-      if (turn) {
-        if constexpr (INTER) {
+    for (int e = 0; e < VE; e += 4) {
+      const float4 cv = h0 < heads ? __ldg(reinterpret_cast<const float4*>(cs + i + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 sv = h0 < heads ? __ldg(reinterpret_cast<const float4*>(sn + i + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      c[e] = cv.x; c[e + 1] = cv.y; c[e + 2] = cv.z; c[e + 3] = cv.w;
+      s[e] = sv.x; s[e + 1] = sv.y; s[e + 2] = sv.z; s[e + 3] = sv.w;
+    }
+    for (int hb = h0; hb < heads; hb += UB * step) {
+      uint4 xa[UB], xb[UB];
 #pragma unroll
-          for (int e = 0; e < VE; e += 2) rope_pair(p[e], p[e + 1], c[e / 2], s[e / 2]);
+      for (int b = 0; b < UB; ++b)
+        if (hb + b * step < heads) {
+          const T* x = src(hb + b * step);
+          xa[b] = *reinterpret_cast<const uint4*>(x + e0);
+          xb[b] = *reinterpret_cast<const uint4*>(x + e1);
+        }
 #pragma unroll
-          for (int e = 0; e < VE; e += 2) rope_pair(r[e], r[e + 1], c[VE / 2 + e / 2], s[VE / 2 + e / 2]);
-        } else {
+      for (int b = 0; b < UB; ++b) {
+        if (hb + b * step >= heads) continue;
+        float p[VE], r[VE];
+        unpack_vec<T>(xa[b], p);
+        unpack_vec<T>(xb[b], r);
+        if (turn) {
+          if constexpr (INTER) {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) rope_pair(p[e], r[e], c[e], s[e]);
+            for (int e = 0; e < VE; e += 2) {
+              rope_pair(p[e], p[e + 1], c[e / 2], s[e / 2]);
+              rope_pair(r[e], r[e + 1], c[VE / 2 + e / 2], s[VE / 2 + e / 2]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) rope_pair(p[e], r[e], c[e], s[e]);
+          }
+        }
+        if (T* y = dst(hb + b * step)) {
+          *reinterpret_cast<uint4*>(y + e0) = pack_vec<T>(p);
+          *reinterpret_cast<uint4*>(y + e1) = pack_vec<T>(r);
         }
       }
-      if (y) {
-        *reinterpret_cast<uint4*>(y + e0) = pack_vec<T>(p);
-        *reinterpret_cast<uint4*>(y + e1) = pack_vec<T>(r);
-      }
-    } else {
+    }
+  } else {
+    for (int u = u0; u < heads * half; u += du) {
+      const int hh = u / half, i = u - hh * half;
       const int e0 = INTER ? 2 * i : i, e1 = INTER ? 2 * i + 1 : half + i;
+      const T* x = src(hh);
       float p = to_f<T>(x[e0]), r = to_f<T>(x[e1]);
       if (turn) rope_pair(p, r, cs[i], sn[i]);
-      if (y) {
+      if (T* y = dst(hh)) {
         y[e0] = from_f<T>(p);
         y[e1] = from_f<T>(r);
       }
     }
   }
-  using V = typename std::conditional<VECTOR, uint4, T>::type;
   const int pass = (d - 2 * half) / VE;  // pass-through vectors per head
-  for (int u = u0; u < (a.hq + a.hkv) * pass; u += du) {
+  for (int u = u0; u < heads * pass; u += du) {
     const int hh = u / pass, e = 2 * half + (u - hh * pass) * VE;
-    const T* x;
-    T* y;
-    head(hh, x, y);
-    const V w = *reinterpret_cast<const V*>(x + e);
-    if (y) *reinterpret_cast<V*>(y + e) = w;
+    const V w = *reinterpret_cast<const V*>(src(hh) + e);
+    if (T* y = dst(hh)) *reinterpret_cast<V*>(y + e) = w;
   }
   if (store) {
-    const V* src = reinterpret_cast<const V*>(v);
-    V* dst = reinterpret_cast<V*>(vo);
-    const int n = a.hkv * d / VE;
-#pragma unroll 2
-    for (int u = u0; u < n; u += du) dst[u] = src[u];
+    V* vo = reinterpret_cast<V*>(a.v_slab + slot * row);
+#pragma unroll
+    for (int b = 0; b < UB; ++b)
+      if (u0 + b * du < nv) vo[u0 + b * du] = vv[b];
+    for (int u = u0 + UB * du; u < nv; u += du) vo[u] = vs[u];
   }
 }
 
@@ -222,11 +237,73 @@ __device__ __forceinline__ void index_entry(const IndexArgs& a, int layer, int64
   if (lane == 0) a.scales[entry] = scale;
 }
 
-// layer >= 0: one CTA per 32 tokens; the pages whose last slot one of them
-// fills are indexed, its warps taking the KV heads. layer < 0: one CTA per
-// (block, layer).
-template <typename T>
+// The same for heads of LPR 16-byte vectors (8, 16 or 32): LPR lanes on a key,
+// 32 / LPR keys at a time, up to 8 loads in flight; a lane keeps VE dims.
+template <typename T, int LPR>
+__device__ __forceinline__ void index_entry_vec(const IndexArgs& a, int layer, int64_t blk, int h, int lane) {
+  constexpr int VE = 16 / int(sizeof(T)), D = LPR * VE, RPI = 32 / LPR;
+  const T* k = reinterpret_cast<const T*>(a.k_base + int64_t(2) * layer * a.slab_bytes) +
+               (blk * a.page * a.hkv + h) * D + (lane % LPR) * VE;
+  const int64_t row = int64_t(a.hkv) * D;
+  float lo[VE], hi[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    lo[e] = INFINITY;
+    hi[e] = -INFINITY;
+  }
+#pragma unroll 8
+  for (int r = lane / LPR; r < a.page; r += RPI) {
+    float x[VE];
+    unpack_vec<T>(*reinterpret_cast<const uint4*>(k + r * row), x);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      lo[e] = fminf(lo[e], x[e]);
+      hi[e] = fmaxf(hi[e], x[e]);
+    }
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+#pragma unroll
+    for (int off = LPR; off < 32; off <<= 1) {
+      lo[e] = fminf(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], off));
+      hi[e] = fmaxf(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], off));
+    }
+    top = fmaxf(top, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+  }
+#pragma unroll
+  for (int off = 1; off < LPR; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const float scale = __fmul_rn(top, 1.0f / 127.0f);
+  const int64_t entry = (int64_t(layer) * a.num_blocks + blk) * a.hkv + h;
+  if (lane < LPR) {
+    int8_t c[2][VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float x = scale > 0.f ? floorf(__fdiv_rn(lo[e], scale)) : 0.f;
+      const float y = scale > 0.f ? ceilf(__fdiv_rn(hi[e], scale)) : 0.f;
+      c[0][e] = int8_t(fminf(fmaxf(x, -127.f), 127.f));
+      c[1][e] = int8_t(fminf(fmaxf(y, -127.f), 127.f));
+    }
+    int8_t* out = a.codes + entry * 2 * D + lane * VE;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int w = 0; w < VE / 4; ++w)
+        reinterpret_cast<char4*>(out + b * D)[w] = make_char4(c[b][4 * w], c[b][4 * w + 1], c[b][4 * w + 2], c[b][4 * w + 3]);
+  }
+  if (lane == 0) a.scales[entry] = scale;
+}
+
+// layer >= 0: one CTA per IX_TOKENS tokens; the pages whose last slot one of
+// them fills are indexed, its warps taking the KV heads. layer < 0: one CTA per
+// (block, layer). LPR 0: any head size.
+constexpr int IX_TOKENS = 16;
+template <typename T, int LPR>
 __global__ void __launch_bounds__(256) page_index_kernel(const IndexArgs a) {
+  auto index_one = [&](int layer, int64_t blk, int h, int ln) {
+    if constexpr (LPR == 0) index_entry<T>(a, layer, blk, h, ln);
+    else index_entry_vec<T, LPR>(a, layer, blk, h, ln);
+  };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   pdl_trigger();
   pdl_wait();  // the keys were written by the append just before
@@ -238,11 +315,11 @@ __global__ void __launch_bounds__(256) page_index_kernel(const IndexArgs a) {
       if (threadIdx.x == 0 && layer == 0) flag(a.st, PKV_DEV_SLOT_OOB);
       return;
     }
-    for (int h = warp; h < a.hkv; h += nw) index_entry<T>(a, layer, blk, h, lane);
+    for (int h = warp; h < a.hkv; h += nw) index_one(layer, blk, h, lane);
     return;
   }
-  const int64_t t = int64_t(blockIdx.x) * 32 + lane;
-  const int64_t slot = t < a.n ? a.ids[t] : -1;
+  const int64_t t = int64_t(blockIdx.x) * IX_TOKENS + lane;
+  const int64_t slot = lane < IX_TOKENS && t < a.n ? a.ids[t] : -1;
   // a slot outside the pool was flagged by the append
   const bool done = slot >= 0 && slot < a.num_blocks * a.page && slot % a.page == a.page - 1;
   uint32_t todo = __ballot_sync(0xffffffffu, done);
@@ -250,14 +327,17 @@ __global__ void __launch_bounds__(256) page_index_kernel(const IndexArgs a) {
     const int l = __ffs(todo) - 1;
     todo &= todo - 1;
     const int64_t blk = __shfl_sync(0xffffffffu, slot, l) / a.page;
-    for (int h = warp; h < a.hkv; h += nw) index_entry<T>(a, a.layer, blk, h, lane);
+    for (int h = warp; h < a.hkv; h += nw) index_one(a.layer, blk, h, lane);
   }
 }
 
 template <typename T>
 int launch_index(const IndexArgs& a, int64_t grid, cudaStream_t s) {
-  PKV_CUDA_RET(launch_kernel(page_index_kernel<T>, dim3(unsigned(grid)), dim3(unsigned(32 * std::min(a.hkv, 8))), 0, s,
-                             true, a));
+  // pool rows of whole 16-byte vectors (the base is 16-byte aligned): the vector forms
+  const int lpr = (a.d * int(sizeof(T))) % 16 == 0 ? a.d * int(sizeof(T)) / 16 : 0;
+  auto kern = lpr == 8 ? page_index_kernel<T, 8> : lpr == 16 ? page_index_kernel<T, 16>
+              : lpr == 32 ? page_index_kernel<T, 32> : page_index_kernel<T, 0>;
+  PKV_CUDA_RET(launch_kernel(kern, dim3(unsigned(grid)), dim3(unsigned(32 * std::min(a.hkv, 8))), 0, s, true, a));
   return PKV_OK;
 }
 
@@ -277,7 +357,7 @@ int run_index(const pkv_pool& p, const pkv_page_index* ix, int layer, const int3
   a.hkv = p.n_kv_heads;
   a.d = p.head_dim;
   a.page = p.block_size;
-  const int64_t grid = layer >= 0 ? (n + 31) / 32 : n * p.num_layers;
+  const int64_t grid = layer >= 0 ? (n + IX_TOKENS - 1) / IX_TOKENS : n * p.num_layers;
   if (grid >= (int64_t(1) << 31)) return fail(PKV_ERR_ARG, "too many blocks for one call");
   switch (p.dtype) {
     case PKV_F16: return launch_index<__half>(a, grid, s);
@@ -393,7 +473,9 @@ extern "C" int pkv_rope_append(const pkv_pool* pool, int32_t layer, const void* 
                  reinterpret_cast<uintptr_t>(rope_sin) | uintptr_t(slab_bytes(p));
   if (n_heads > 0)
     al |= reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | uintptr_t(a.q_stride);
-  const bool vec = (al & 15) == 0 && a.half % ve == 0;
+  a.cols = 1;
+  while (a.cols < a.half / ve) a.cols *= 2;
+  const bool vec = (al & 15) == 0 && a.half % ve == 0 && a.cols <= 32;
   // one warp per token once that fills the SMs' warp slots, else up to 8
   const int64_t want = int64_t(num_sms()) * 32;
   a.wpt = n_tokens >= want ? 1 : (2 * n_tokens >= want ? 2 : (4 * n_tokens >= want ? 4 : 8));

@@ -164,13 +164,6 @@ struct DecodeArgs {
   const float* rcos = nullptr;
   const float* rsin = nullptr;
   int64_t rmax = 0;
-  // Pieces computed before (FOLD variant): row r's attention over keys outside
-  // its listed pages, as fold[r] = {first piece row, pieces, stride}: piece i
-  // of head hh is O / l at fold_o[((first + i * stride) * n_heads + hh) * 64] and
-  // (m, l) at fold_ml[...]; the sequence's first piece here starts from them.
-  const int4* fold = nullptr;
-  const float* fold_o = nullptr;
-  const float2* fold_ml = nullptr;
   int64_t total_pages;   // capacity of desc (and the page count when p_dev is NULL)
   int n_seqs;
   int n_rows;            // rows of q / out
@@ -385,52 +378,6 @@ __device__ __forceinline__ void attend_pages(const uint32_t (&kb)[U], const uint
   }
 }
 
-// The (m, l, O) state of one warp's KV head after the pieces fold[row] lists
-// (FOLD variant), in attend_pages' fragment layout: dims mt * 16 + g (+ 8) of
-// heads 2 c4 and 2 c4 + 1; a row's l is summed over the lanes g, so one lane
-// holds it.
-template <int GROUPS>
-__device__ __forceinline__ void fold_pieces(const DecodeArgs& a, int row, int h, int g, int c4, float (&o)[4][4],
-                                            float& m0, float& m1, float& l0, float& l1) {
-  const int4 f = __ldcg(a.fold + row);
-  const int nh = a.n_heads;
-  const int j0 = min(2 * c4, GROUPS - 1), j1 = min(2 * c4 + 1, GROUPS - 1);
-  float L0 = 0.f, L1 = 0.f;
-#pragma unroll 2
-  for (int i = 0; i < f.y; ++i) {
-    const int64_t e = (int64_t(f.x) + int64_t(i) * f.z) * nh + h * GROUPS;
-    const float2 ml0 = __ldcg(a.fold_ml + e + j0), ml1 = __ldcg(a.fold_ml + e + j1);
-    const float* p0 = a.fold_o + (e + j0) * DK_D + g;
-    const float* p1 = a.fold_o + (e + j1) * DK_D + g;
-    float v[4][4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      v[mt][0] = __ldcg(p0 + mt * 16);
-      v[mt][1] = __ldcg(p1 + mt * 16);
-      v[mt][2] = __ldcg(p0 + mt * 16 + 8);
-      v[mt][3] = __ldcg(p1 + mt * 16 + 8);
-    }
-    const float n0 = fmaxf(m0, ml0.x), n1 = fmaxf(m1, ml1.x);
-    const float k0 = ex2(m0 - n0), k1 = ex2(m1 - n1);
-    const float w0 = ml0.y * ex2(ml0.x - n0), w1 = ml1.y * ex2(ml1.x - n1);
-    m0 = n0;
-    m1 = n1;
-    L0 = L0 * k0 + w0;
-    L1 = L1 * k1 + w1;
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      o[mt][0] = o[mt][0] * k0 + w0 * v[mt][0];
-      o[mt][2] = o[mt][2] * k0 + w0 * v[mt][2];
-      o[mt][1] = o[mt][1] * k1 + w1 * v[mt][1];
-      o[mt][3] = o[mt][3] * k1 + w1 * v[mt][3];
-    }
-  }
-  if (g == 0) {
-    l0 = L0;
-    l1 = L1;
-  }
-}
-
 // One CTA = one consumer warp per KV head + one producer warp. The producer
 // streams whole pages: one TMA box per page for K and one for V, each the full
 // contiguous 16 KiB [16 tok][8 heads][64] page, read through a permuted view of
@@ -447,9 +394,7 @@ __device__ __forceinline__ void fold_pieces(const DecodeArgs& a, int row, int h,
 // per sequence and, if that completed the count, merges the sequence.
 // FUSE: the variant with the KV-append folded in (DecodeArgs::knew set); a
 // separate instantiation, so the plain decode kernel carries none of its code.
-// FOLD: the variant whose sequences start from pieces computed before
-// (DecodeArgs::fold set; pkv_shared.cu).
-template <typename T, int GROUPS, int NST, bool FUSE, bool FOLD = false>
+template <typename T, int GROUPS, int NST, bool FUSE>
 __global__ void __maxnreg__(DK_MAXNREG) decode_kernel(const __grid_constant__ CUtensorMap tmap,
                                                       const DecodeArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -839,9 +784,6 @@ __global__ void __maxnreg__(DK_MAXNREG) decode_kernel(const __grid_constant__ CU
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[mt][e] = 0.f;
     float m0 = -1e30f, m1 = -1e30f, l0 = 0.f, l1 = 0.f;
-    if constexpr (FOLD) {
-      if (seen_first) fold_pieces<GROUPS>(a, row, h, g, c4, o, m0, m1, l0, l1);
-    }
     for (int j = 0; j < n; j += DK_U) {
       const int cnt = min(DK_U, n - j);
       slide_to(i + j);
@@ -1185,7 +1127,7 @@ int decode_ctas_per_sm_cap() {
 
 // CTAs of the decode kernel resident per SM, cached per (device, n_kv_heads);
 // also raises the kernel's dynamic shared-memory limit on first use per device.
-template <typename T, int GROUPS, int NST, bool FUSE, bool FOLD = false>
+template <typename T, int GROUPS, int NST, bool FUSE>
 int decode_grid_limit(int n_kv_heads) {
   static std::mutex mu;
   static std::vector<std::array<int, 9>> occ;
@@ -1195,7 +1137,7 @@ int decode_grid_limit(int n_kv_heads) {
   if ((int)occ.size() <= dev) occ.resize(dev + 1, std::array<int, 9>{});
   int& o = occ[dev][n_kv_heads];
   if (!o) {
-    auto fn = decode_kernel<T, GROUPS, NST, FUSE, FOLD>;
+    auto fn = decode_kernel<T, GROUPS, NST, FUSE>;
     const size_t sm = decode_smem(n_kv_heads, GROUPS, NST);
     // the limit is the function's, not this geometry's: a pool of fewer KV heads
     // must not lower it under a launch for more
@@ -1214,15 +1156,15 @@ int decode_grid_limit(int n_kv_heads) {
 
 int max_decode_grid() { return num_sms() * 8; }
 
-template <typename T, int GROUPS, int NST, bool FUSE, bool FOLD = false>
+template <typename T, int GROUPS, int NST, bool FUSE>
 int launch_decode_f(const pkv_pool& p, const CUtensorMap& tm, DecodeArgs& a, int64_t total_pages,
                     cudaStream_t s) {
-  int limit = decode_grid_limit<T, GROUPS, NST, FUSE, FOLD>(p.n_kv_heads);
+  int limit = decode_grid_limit<T, GROUPS, NST, FUSE>(p.n_kv_heads);
   if (limit <= 0) return PKV_ERR_CUDA;  // message already set
   limit = std::min(limit, max_decode_grid());
   const int grid = int(std::max<int64_t>(1, std::min<int64_t>(limit, total_pages)));
   a.prefetch = decode_prefetch();
-  PKV_CUDA_RET(launch_kernel(decode_kernel<T, GROUPS, NST, FUSE, FOLD>, dim3(grid), dim3(32 * (p.n_kv_heads + 2)),
+  PKV_CUDA_RET(launch_kernel(decode_kernel<T, GROUPS, NST, FUSE>, dim3(grid), dim3(32 * (p.n_kv_heads + 2)),
                              decode_smem(p.n_kv_heads, GROUPS, NST), s, true, tm, a));
   return PKV_OK;
 }
@@ -1277,67 +1219,7 @@ WsLayout step_layout(const pkv_pool* pool, int n_heads, int n_seqs, int64_t tota
   return ws_layout(n_heads, n_seqs, total_pages, max_decode_grid(), d, cap);
 }
 
-// The FOLD variant: the ring as deep as shared memory allows, 5 or 6 stages.
-template <typename T, int GROUPS>
-int launch_decode_fold_n(const pkv_pool& p, const CUtensorMap& tm, DecodeArgs& a, int64_t tp, cudaStream_t s) {
-  if (decode_smem(p.n_kv_heads, GROUPS, 6) <= size_t(DK_SMEM_MAX)) return launch_decode_f<T, GROUPS, 6, false, true>(p, tm, a, tp, s);
-  return launch_decode_f<T, GROUPS, 5, false, true>(p, tm, a, tp, s);
-}
-
-template <typename T>
-int launch_decode_fold_g(const pkv_pool& p, int groups, const CUtensorMap& tm, DecodeArgs& a, int64_t tp,
-                         cudaStream_t s) {
-  switch (groups) {
-    case 1: return launch_decode_fold_n<T, 1>(p, tm, a, tp, s);
-    case 2: return launch_decode_fold_n<T, 2>(p, tm, a, tp, s);
-    case 4: return launch_decode_fold_n<T, 4>(p, tm, a, tp, s);
-    case 8: return launch_decode_fold_n<T, 8>(p, tm, a, tp, s);
-  }
-  return fail(PKV_ERR_UNSUPPORTED, "decode kernel: unsupported GQA group size");
-}
-
 }  // namespace
-
-bool decode_fold_supported(const pkv_pool& p, int n_heads) { return decode_supported(p, n_heads); }
-
-DecodeListLayout decode_list_layout(int n_heads, int n_seqs, int64_t total_pages) {
-  const WsLayout w = ws_layout(n_heads, n_seqs, total_pages, max_decode_grid(), DK_D);
-  return DecodeListLayout{w.page_desc, w.counters, w.total};
-}
-
-int decode_fold(const pkv_pool& p, int layer, int n_heads, const void* q, void* out, float scale, const pkv_batch& b,
-                char* ws, const int32_t* rows, const int64_t* p_dec, const int4* fold, const float* fold_o,
-                const float2* fold_ml, cudaStream_t s) {
-  const WsLayout w = ws_layout(n_heads, b.n_seqs, b.total_pages, max_decode_grid(), DK_D);
-  CUtensorMap tm;
-  if (int rc = get_tmap(p, &tm, p.n_kv_heads)) return rc;
-  DecodeArgs a;
-  a.q = q;
-  a.out = out;
-  a.desc = reinterpret_cast<const int4*>(ws + w.page_desc);
-  a.partial_o = reinterpret_cast<float*>(ws + w.partial_o);
-  a.partial_ml = reinterpret_cast<float2*>(ws + w.partial_ml);
-  a.counters = reinterpret_cast<int32_t*>(ws + w.counters);
-  a.st = b.dev_status;
-  a.rows = rows;
-  a.p_dev = p_dec;
-  a.knew = a.vnew = nullptr;
-  a.slots = nullptr;
-  a.k_slab = a.v_slab = nullptr;
-  a.n_slots = 0;
-  a.fold = fold;
-  a.fold_o = fold_o;
-  a.fold_ml = fold_ml;
-  a.total_pages = b.total_pages;
-  a.n_seqs = b.n_seqs;
-  a.n_rows = b.n_tokens;
-  a.n_heads = n_heads;
-  a.layer = layer;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  const int groups = n_heads / p.n_kv_heads;
-  if (p.dtype == PKV_F16) return launch_decode_fold_g<__half>(p, groups, tm, a, b.total_pages, s);
-  return launch_decode_fold_g<__nv_bfloat16>(p, groups, tm, a, b.total_pages, s);
-}
 
 int pool_tmap(const pkv_pool& p, CUtensorMap* out) { return get_tmap(p, out, p.n_kv_heads); }
 int pool_tmap_head(const pkv_pool& p, CUtensorMap* out) { return get_tmap(p, out, 1); }

@@ -104,19 +104,6 @@ int prefill_tc_attend(const pkv_pool& p, int layer, int n_heads, const void* q, 
                       const pkv_batch& b, const int2* tiles, const int32_t* n_tiles, int64_t tiles_cap,
                       cudaStream_t s);
 
-// The decode kernel over listed q_len == 1 rows whose sequences start from
-// pieces computed before (pkv_attn.cu, for shared-prefix attention). The list
-// (descriptors, zeroed split-K counters) lies in `ws` as decode_list_layout says;
-// rows / p_dec as in PrefillMixedPlan, fold / fold_o / fold_ml as DecodeArgs'.
-struct DecodeListLayout {
-  size_t page_desc, counters, total;
-};
-bool decode_fold_supported(const pkv_pool& p, int n_heads);
-DecodeListLayout decode_list_layout(int n_heads, int n_seqs, int64_t total_pages);
-int decode_fold(const pkv_pool& p, int layer, int n_heads, const void* q, void* out, float scale, const pkv_batch& b,
-                char* ws, const int32_t* rows, const int64_t* p_dec, const int4* fold, const float* fold_o,
-                const float2* fold_ml, cudaStream_t s);
-
 // ---------------------------------------------------------------- device side
 // PDL: let the next kernel in the stream be scheduled now; wait until the
 // kernels before this one completed and their writes are visible.
@@ -250,6 +237,17 @@ __device__ __forceinline__ void tma_prefetch_l2_4d(const CUtensorMap* map, int c
                    reinterpret_cast<uint64_t>(map)),
                "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
+}
+
+// 16 bytes global -> shared (cp.async), or 16 zero bytes when !ok
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // warp-level tensor-core helpers (fp16 / bf16 operands, fp32 accumulate) ----

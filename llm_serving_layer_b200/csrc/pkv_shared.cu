@@ -12,18 +12,22 @@
 //
 //   shared_check_kernel  once per step: verifies that a group's page lists agree
 //   shared_plan_kernel   once per step: the work items, the pieces each row
-//                        merges, and the decode kernel's page list of the rest
-//   shared_tc_kernel     tcgen05 tiles of 128 rows (128 / G tokens of the group
-//                        x the G query heads of a KV head) over a range of A's
-//                        64-key blocks -> pieces (O, m, l) in fp32. Also the rest
-//                        B of sequences with several new tokens (causal).
-//   decode kernel        the rest B of sequences with one new token; starts from
-//                        the row's pieces (decode_fold, pkv_attn.cu)
-//   shared_merge_kernel  the pieces of rows of several-token sequences -> out
+//                        merges, and the list of the one-token sequences' rest
+//   shared_kernel        one persistent launch, three CTAs per SM, two roles:
+//                        tiles  tcgen05 tiles of 128 rows (128 / G tokens of the
+//                               group x the G query heads of a KV head) over a
+//                               range of A's 64-key blocks, and the rest B of
+//                               sequences with several new tokens (causal)
+//                        stream one warp per KV head walks the pages of the rest
+//                               B of sequences with one new token (mma.sync on
+//                               16-key pages, as the decode kernel)
+//                        each leaves pieces (O, m, l) in fp32
+//   shared_merge_kernel  the pieces of a row -> out
 //
-// A's keys are read once per 128 rows instead of once per sequence; its
-// arithmetic is 4 D flops per (row, key) on the tensor cores. The range length
-// of an item is chosen on the device so that the items fill the SMs.
+// A's keys are read once per 128 rows instead of once per sequence: its
+// 4 D flops per (row, key) are bound by the tensor cores and the exponentials,
+// the rest by HBM. So the roles run side by side on every SM: some CTAs stream
+// while the others compute, and the streaming CTAs take tiles when they are done.
 #include <algorithm>
 #include <mutex>
 #include <string>
@@ -35,11 +39,22 @@
 namespace pkv {
 namespace {
 
-constexpr int SH_MINB = 3;          // CTAs per SM of the tile kernel
+constexpr int SH_MINB = 3;          // CTAs per SM
 constexpr int SH_NST = 2;           // slots of the K ring and of the V ring
 constexpr int SH_TMEM_COLS = 128;   // S in columns 0-63, O in 64-127
-constexpr int SH_PIECES = 16384;    // token pieces the workspace holds at most (x n_heads x 264 bytes)
-constexpr int SH_OVERHEAD = 4;      // cost of an item besides its blocks, in blocks (set-up, piece written and read)
+constexpr int SH_PIECES = 16384;    // tile piece rows the workspace holds at most (x n_heads x 264 bytes)
+#ifndef SH_OVERHEAD
+#define SH_OVERHEAD 4
+#endif
+// SH_OVERHEAD: cost of an item besides its blocks, in blocks (set-up, piece written and read)
+constexpr int SH_WARPS = TC_THREADS / 32;
+#ifndef SH_SST_
+#define SH_SST_ 3
+#endif
+constexpr int SH_SST = SH_SST_;                         // ring stages of a streaming warp
+constexpr int SH_TILE = TC_P * TC_D * 2;          // one 16-token K or V tile of a head
+constexpr int SH_STAGE = 2 * SH_TILE;
+constexpr size_t SH_RING = size_t(SH_WARPS) * SH_SST * SH_STAGE;
 
 // Rows (consecutive tokens) against a page range of one list.
 struct ShEnt {
@@ -55,34 +70,50 @@ struct ShEnt {
   int item0;       // first item
 };
 
+// A work item of the tile role, without its KV head.
+struct ShItem {
+  int t0, nt;        // first token, tokens of the tile
+  int pg_at, n_pg;   // first entry in kv_indices, pages of the range
+  int nblk;          // 64-key blocks
+  int lim0, causal;  // last key (counted from the range's first) the first token sees; 1: token i sees i more
+  int tail_pg, lpl;  // page of the range with only lpl written tokens (-1: none)
+  int piece;         // piece row of the first token (-1: straight to out)
+  int h, zero;       // (published) KV head; a page id outside the pool: the item's rows are zeros
+};
+static_assert(sizeof(ShItem) == 3 * sizeof(int4), "items are read as three int4");
+
 struct ShCtl {
   int n_items;
-  int claim[2];    // next item, CTAs finished
-  int chunk;       // blocks per range
-  int64_t p_dec;   // pages listed for the decode kernel
-  int n_ents;
-  int n_shared;    // groups whose prefix is shared
+  int claim[2];    // items claimed, CTAs finished
+  int n_stream;    // CTAs that stream first
+  int n_ranges;    // ranges the listed pages are cut into (one warp per range and KV head)
+  int listed;      // pages listed
+  int chunk;       // blocks per range of a tile item
+  int n_ents, n_shared;
 };
 
 struct ShLayout {
-  DecodeListLayout dec;
-  size_t ctl, rows, seq_np, group_bad, ents, items, fold, rest, part_o, part_ml, total;
-  int64_t pieces, items_cap;
+  size_t ctl, rows, list, seq_np, group_bad, ents, items, desc, fold, rest, part_o, part_ml, total;
+  int64_t pieces, items_cap, slots;
 };
 
 inline size_t al256(size_t x) { return (x + 255) & ~size_t(255); }
 
 int split_cap(int n_tokens) { return std::max(1, std::min(64, 4096 / std::max(n_tokens, 1))); }
 
-ShLayout sh_layout(int n_heads, int groups, int n_seqs, int n_tokens, int64_t total_pages) {
+// Ranges of the listed pages there can be: every warp of the launch streaming.
+int max_ranges(int n_kv) { return SH_MINB * num_sms() * SH_WARPS / n_kv; }
+
+ShLayout sh_layout(int n_heads, int n_kv, int n_seqs, int n_tokens, int64_t total_pages) {
   ShLayout w;
-  w.dec = decode_list_layout(n_heads, n_seqs, total_pages);
-  size_t off = al256(w.dec.total);
+  size_t off = 0;
   const int cap = split_cap(n_tokens);
-  const int tpt = TC_ROWS / groups;
+  const int tpt = TC_ROWS / std::max(1, std::min(8, n_heads / n_kv));
   w.pieces = std::min<int64_t>(int64_t(2) * n_tokens * cap, SH_PIECES);
   // every entity's last tile may be partial; an entity is a group or a sequence
   w.items_cap = (int64_t(2) * ((n_tokens + tpt - 1) / tpt) + 2 * int64_t(n_seqs)) * cap;
+  // piece rows: the tiles', then one per (range, sequence) a streaming warp meets
+  w.slots = w.pieces + n_seqs + max_ranges(n_kv);
   auto take = [&](size_t bytes) {
     const size_t at = off;
     off = al256(off + bytes);
@@ -90,14 +121,16 @@ ShLayout sh_layout(int n_heads, int groups, int n_seqs, int n_tokens, int64_t to
   };
   w.ctl = take(sizeof(ShCtl));
   w.rows = take(sizeof(int32_t) * n_seqs);
+  w.list = take(sizeof(int2) * n_seqs);
   w.seq_np = take(sizeof(int32_t) * n_seqs);
   w.group_bad = take(sizeof(int32_t) * n_seqs);
   w.ents = take(sizeof(ShEnt) * 2 * n_seqs);
-  w.items = take(sizeof(int4) * w.items_cap);
+  w.items = take(sizeof(ShItem) * w.items_cap);
+  w.desc = take(sizeof(int2) * size_t(std::max<int64_t>(total_pages, 1)));
   w.fold = take(sizeof(int4) * std::max(n_tokens, 1));
   w.rest = take(sizeof(int4) * std::max(n_tokens, 1));
-  w.part_o = take(sizeof(float) * size_t(w.pieces) * n_heads * TC_D);
-  w.part_ml = take(sizeof(float2) * size_t(w.pieces) * n_heads);
+  w.part_o = take(sizeof(float) * size_t(w.slots) * n_heads * TC_D);
+  w.part_ml = take(sizeof(float2) * size_t(w.slots) * n_heads);
   w.total = off;
   return w;
 }
@@ -113,18 +146,18 @@ struct PlanArgs {
   const int32_t* prefix_pages;  // [n_groups]
   int32_t* st;
   int64_t num_blocks, total_pages;
-  int n_seqs, n_tokens, n_groups, n_kv, tpt, slots, splits_cap;
+  int n_seqs, n_tokens, n_groups, n_kv, tpt, sms, splits_cap, grid;
   int64_t pieces_cap, items_cap;
   ShCtl* ctl;
-  int32_t* rows;
-  int32_t* seq_np;
+  int32_t* rows;   // row of each listed one-token sequence
+  int2* list;      // its first page in the list, its pages
+  int32_t* seq_np; // shared pages of each sequence
   int32_t* group_bad;
   ShEnt* ents;
-  int4* items;
-  int4* fold;
-  int4* rest;
-  int4* desc;
-  int32_t* counters;
+  ShItem* items;
+  int2* desc;      // listed page {block, index of its sequence in the list << 7 | first << 6 | last << 5 | tokens}
+  int4* fold;      // a row's pieces over the shared keys {first piece row, pieces, stride}
+  int4* rest;      // ... over its own
 };
 
 struct SeqInfo {
@@ -188,15 +221,12 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   if (tid == 0) {
     s_bad = (a.cu_q[0] != 0 || a.cu_q[a.n_seqs] != a.n_tokens || a.group_indptr[0] != 0 ||
              a.group_indptr[a.n_groups] != a.n_seqs) ? 1 : 0;
-    a.ctl->n_items = 0;
-    a.ctl->claim[0] = a.ctl->claim[1] = 0;
-    a.ctl->p_dec = 0;
+    *a.ctl = ShCtl{};
   }
   for (int t = tid; t < a.n_tokens; t += blockDim.x) a.fold[t] = a.rest[t] = make_int4(0, 0, 0, 0);
   __syncthreads();
   if (s_bad) {
     if (tid == 0) flag(a.st, PKV_DEV_META_BAD);
-    for (int d = tid; d < a.n_seqs; d += blockDim.x) a.rows[d] = -1;
     __threadfence();
     return;
   }
@@ -289,7 +319,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
       if (x.base >= 0) pieces += int64_t(x.nt) * sp;
     }
     fits &= pieces <= a.pieces_cap;
-    const float est = (work + n_it * SH_OVERHEAD) * a.n_kv / a.slots + cand + SH_OVERHEAD;
+    const float est = (work + n_it * SH_OVERHEAD) * a.n_kv / (SH_MINB * a.sms) + cand + SH_OVERHEAD;
     if (tid == 0) s_best = ~0ull;
     __syncthreads();
     if (fits && (tid == 0 || (tid + 1) * step < maxblk + step))
@@ -329,23 +359,37 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   if (tid == 0) s_tot = item0 <= a.items_cap ? 1 : 0;
   __syncthreads();
   const bool room = s_tot != 0;  // the capacity covers every case: kept as a check
+  if (tid == 0) s_maxblk = 0;
+  __syncthreads();
   for (int i = warp; room && i < n_ents; i += 32) {
     const ShEnt x = a.ents[i];
-    for (int k = lane; k < x.tiles * x.splits; k += 32)
-      a.items[x.item0 + k] = make_int4(i, k / x.splits, k % x.splits, 0);
+    for (int k = lane; k < x.tiles * x.splits; k += 32) {
+      const int i0 = k / x.splits * a.tpt, sp = k % x.splits;
+      ShItem I{};
+      I.t0 = x.t0 + i0;
+      I.nt = min(a.tpt, x.nt - i0);
+      const int first = x.pg0 + (x.base < 0 ? 0 : sp * chunk * TC_PPB);
+      const int last = x.base < 0 ? x.pg1 : min(x.pg1, first + chunk * TC_PPB);
+      I.pg_at = x.pa + first;
+      I.lim0 = x.lim0 + x.causal * i0 - first * TC_P;
+      I.causal = x.causal;
+      const int seen = I.lim0 + x.causal * (I.nt - 1);  // last key any of its rows sees
+      I.n_pg = seen < 0 ? 0 : min(last - first, seen / TC_P + 1);
+      I.nblk = max(1, (I.n_pg + TC_PPB - 1) / TC_PPB);  // a range no row sees: one block, all masked
+      I.tail_pg = x.lpl < TC_P && x.pg1 - 1 - first < I.n_pg ? x.pg1 - 1 - first : -1;
+      I.lpl = x.lpl;
+      I.piece = x.base < 0 ? -1 : x.base + sp * x.nt + i0;
+      a.items[x.item0 + k] = I;
+      atomicAdd(&s_maxblk, I.nblk);
+    }
     if (x.base >= 0) {
       int4* to = x.causal ? a.rest : a.fold;
       for (int k = lane; k < x.nt; k += 32) to[x.t0 + k] = make_int4(x.base + k, x.splits, x.nt, 0);
     }
   }
-  if (tid == 0) {
-    if (!room) flag(a.st, PKV_DEV_WORKSPACE);
-    a.ctl->n_items = room ? item0 : 0;
-    a.ctl->chunk = chunk;
-    a.ctl->n_ents = n_ents;
-    a.ctl->n_shared = n_shared;
-  }
-  // ---- the decode kernel's list: one-token sequences, their pages after the shared ones
+  __syncthreads();
+  const int n_items = room ? item0 : 0, blocks = s_maxblk;
+  // ---- the one-token sequences' list: their pages after the shared ones
   int base_seq = 0, base_pg = 0;
   for (int c0 = 0; c0 < a.n_seqs; c0 += blockDim.x) {
     const int s = c0 + tid;
@@ -363,73 +407,299 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     const int off = base_pg + block_excl_scan(np, warp_sum, &tot_pg);
     if (is) {
       a.rows[d] = q.q0;
-      a.counters[d] = 0;
+      a.list[d] = make_int2(off, np);
     }
-    // the warp writes its sequences' descriptors one sequence at a time
+    // the warp writes its sequences' pages one sequence at a time
     for (int l = 0; l < 32; ++l) {
       if (!__shfl_sync(0xffffffffu, is, l)) continue;
       const int dn = __shfl_sync(0xffffffffu, d, l), on = __shfl_sync(0xffffffffu, off, l);
       const int nn = __shfl_sync(0xffffffffu, np, l), lp = __shfl_sync(0xffffffffu, q.lpl, l);
       const int from = __shfl_sync(0xffffffffu, q.pa + q.pages - np, l);
       for (int p = lane; p < nn && int64_t(on) + nn <= a.total_pages; p += 32) {
-        const int id = a.kv_indices[from + p];
-        if (id < 0 || id >= a.num_blocks) flag(a.st, PKV_DEV_SLOT_OOB);
+        int id = a.kv_indices[from + p];
+        if (id < 0 || id >= a.num_blocks) {
+          flag(a.st, PKV_DEV_SLOT_OOB);
+          id = -1;  // no keys
+        }
         const int first = p == 0, last = p == nn - 1;
-        a.desc[on + p] = make_int4(id, (dn << 7) | (first << 6) | (last << 5) | (last ? lp : TC_P), on, on + nn);
+        a.desc[on + p] = make_int2(id, (dn << 7) | (first << 6) | (last << 5) | (last ? lp : TC_P));
       }
     }
     base_seq += tot_seq;
     base_pg += tot_pg;
   }
-  for (int d = base_seq + tid; d < a.n_seqs; d += blockDim.x) a.rows[d] = -1;
+  // overlapping page lists (some indptr entry runs backwards) list more pages
+  // than there are: nothing is streamed
+  const bool over = base_pg > a.total_pages;
+  const int P = over ? 0 : base_pg;
+  // Streaming CTAs: all when there are no tiles, else one per SM, or two where
+  // the pages' time at the copy rate is the larger part (a page of one KV head:
+  // 4 KiB; a block of a tile: 820 cycles of its SM)
+  const float t_stream = float(P) * a.n_kv * 4096.f / 6.4e6f, t_tiles = float(blocks) * a.n_kv / a.sms * 0.43f;  // us
+  int n_stream = P == 0 ? 0 : n_items == 0 ? a.grid : min(a.grid, t_stream > 1.5f * t_tiles ? 2 * a.sms : a.sms);
+#ifdef SH_FORCE
+  if (P > 0 && n_items > 0) n_stream = SH_FORCE * a.sms;
+#endif
+  n_stream = min(n_stream, (P * a.n_kv + SH_WARPS - 1) / SH_WARPS);
+  const int ranges = P == 0 ? 0 : max(1, min(P, n_stream * SH_WARPS / a.n_kv));
+  __syncthreads();
+  for (int d = tid; d < base_seq; d += blockDim.x) {
+    const int2 r = a.list[d];
+    // ranges [r P / ranges, (r + 1) P / ranges) that hold its pages; (range, sequence) is piece range + d
+    const int r0 = P ? int((int64_t(r.x + 1) * ranges + P - 1) / P) - 1 : 0;
+    const int r1 = P ? int((int64_t(r.x + r.y) * ranges + P - 1) / P) - 1 : -1;
+    a.rest[a.rows[d]] = make_int4(int(a.pieces_cap) + d + r0, r1 - r0 + 1, 1, 0);
+  }
   if (tid == 0) {
-    // overlapping page lists (some indptr entry runs backwards) list more pages
-    // than there are: nothing is decoded
-    if (base_pg > a.total_pages) flag(a.st, PKV_DEV_META_BAD);
-    a.ctl->p_dec = base_pg > a.total_pages ? 0 : base_pg;
+    if (!room) flag(a.st, PKV_DEV_WORKSPACE);
+    if (over) flag(a.st, PKV_DEV_META_BAD);
+    a.ctl->n_items = n_items;
+    a.ctl->chunk = chunk;
+    a.ctl->n_ents = n_ents;
+    a.ctl->n_shared = n_shared;
+    a.ctl->n_stream = n_stream;
+    a.ctl->n_ranges = ranges;
+    a.ctl->listed = P;
   }
   // read by later kernels before their griddepcontrol.wait (this kernel never
   // triggers its dependents early): visible at GPU scope before the block exits
   __threadfence();
 }
 
-// ---------------------------------------------------------------- tile kernel
+// ---------------------------------------------------------------- roles
 struct ShArgs {
+  const void* q;
   void* out;
   const ShCtl* ctl;
   int32_t* claim;
-  const ShEnt* ents;
-  const int4* items;
+  const ShItem* items;
+  const int2* desc;
+  const int32_t* rows;
   const int32_t* kv_indices;
+  const char* k_slab;
+  const char* v_slab;
   float* part_o;
   float2* part_ml;
   int32_t* st;
   int64_t num_blocks;
-  int n_heads, n_kv, layer;
+  int stream_piece0;  // first piece row of the streaming warps
+  int n_heads, n_kv, layer, n_tokens, n_seqs;
   float scale_log2;
 };
 
-// A work item as the producer publishes it (nblk = 0: no more items).
-struct ShItem {
-  int h, t0, nt;     // KV head, first token, tokens of the tile
-  int n_pg, nblk;    // pages and 64-key blocks of the range
-  int lim0, causal;  // last key (counted from the range's first) the first token sees
-  int tail_pg, lpl;  // page of the range with only lpl written tokens (-1: none)
-  int piece;         // piece row of the first token (-1: straight to out)
-  int zero;          // a page id outside the pool: the item's rows are zeros
-};
-
-// The tile pipeline of prefill_tc_lean_kernel (pkv_prefill_tc.cu) over the
-// plan's items: three persistent CTAs per SM; warp 0 claims items and loads the
-// query tile and the K / V blocks by TMA, warp 1 issues S = Q K^T and O += P V
-// (tcgen05, accumulators in TMEM), warps 2-5 hold one row a thread: running
-// maximum and sum, P to shared memory, lazy rescale of O. The epilogue writes
-// the row as a piece: O / l in fp32 and (m, l).
+// Stream role, one warp: KV head h over the listed pages [p0, p1) (range `r`).
+// Each sequence it meets leaves the piece (O / l, m, l) of its pages in the
+// range. Pages come through the warp's ring of SH_SST stages (cp.async, 128-byte
+// rows swizzled for ldmatrix); S^T = K q^T and O^T += V^T P^T on 16-key tiles with
+// fp32 online softmax; keys past a page's tokens are neither read nor counted.
 template <typename T, int G>
-__global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_tc_kernel(
+__device__ __forceinline__ void stream_range(const ShArgs& a, unsigned char* ring, int h, int r, int p0, int p1,
+                                             int lane) {
+  const int g = lane >> 2, c4 = lane & 3;
+  const T* q = static_cast<const T*>(a.q);
+  const int n = p1 - p0;
+  const uint32_t ring0 = smem_u32(ring);
+  const int64_t row_b = int64_t(a.n_kv) * TC_D * 2;
+  const int r0 = lane >> 3, ch = lane & 7;  // this lane's chunk of the rows r0, r0 + 4, ... it copies
+  const int64_t lane_off = int64_t(r0) * row_b + int64_t(h) * TC_D * 2 + ch * 16;
+  // descriptors: lane j holds pages wb + j (cur) and wb + 32 + j (nxt)
+  int wb = 0;
+  int2 cur = lane < n ? __ldcg(a.desc + p0 + lane) : make_int2(-1, 0);
+  int2 nxt = 32 + lane < n ? __ldcg(a.desc + p0 + 32 + lane) : make_int2(-1, 0);
+  auto desc_at = [&](int i) -> int2 {  // uniform i in [wb, wb + 64)
+    const bool in_cur = i < wb + 32;
+    return make_int2(__shfl_sync(0xffffffffu, in_cur ? cur.x : nxt.x, i & 31),
+                     __shfl_sync(0xffffffffu, in_cur ? cur.y : nxt.y, i & 31));
+  };
+  auto slide_to = [&](int i) {  // make [i, i + 32) resident
+    if (i >= wb + 32) {
+      wb += 32;
+      cur = nxt;
+      nxt = wb + 32 + lane < n ? __ldcg(a.desc + p0 + wb + 32 + lane) : make_int2(-1, 0);
+    }
+  };
+  auto load = [&](int i) {  // page i of the range
+    const int2 d = desc_at(i);
+    const int valid = d.x < 0 ? 0 : d.y & 31;
+    const uint32_t dst = ring0 + (i % SH_SST) * SH_STAGE;
+    const int64_t off0 = int64_t(d.x) * TC_P * row_b + lane_off;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int rr = 4 * c + r0;
+      const bool ok = rr < valid;
+      const int64_t off = ok ? off0 + 4 * c * row_b : 0;
+      const uint32_t sw = rr * 128 + ((ch ^ (rr & 7)) << 4);
+      cp_async16(dst + sw, a.k_slab + off, ok);
+      cp_async16(dst + SH_TILE + sw, a.v_slab + off, ok);
+    }
+  };
+  auto load_q = [&](int sq, uint32_t (&qb)[4][2]) {  // B operand of list entry sq's queries of this KV head
+    const int row = sq < a.n_seqs ? __ldcg(a.rows + sq) : -1;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) qb[ks][0] = qb[ks][1] = 0u;
+    if (g < G && row >= 0 && row < a.n_tokens) {
+      const T* qr = q + (int64_t(row) * a.n_heads + h * G + g) * TC_D + 2 * c4;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        qb[ks][0] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16));
+        qb[ks][1] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8));
+      }
+    }
+  };
+  const int k_tok = lane & 15, k_chk = lane >> 4;
+  const int v_tok = (lane & 7) + ((lane >> 4) << 3), v_chk = (lane >> 3) & 1;
+#pragma unroll
+  for (int i = 0; i < SH_SST - 1; ++i) {
+    if (i < n) load(i);
+    cp_async_commit();
+  }
+  int sq = desc_at(0).y >> 7;
+  const int sq_last = __ldcg(&a.desc[p1 - 1].y) >> 7;
+  uint32_t qb[4][2], qn[4][2];
+  load_q(sq, qb);
+  if (sq < sq_last) load_q(sq + 1, qn);
+  float o[4][4];
+  float m0 = -1e30f, m1 = -1e30f, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[mt][e] = 0.f;
+  for (int i = 0; i < n; ++i) {
+    slide_to(i);
+    if (i + SH_SST - 1 < n) load(i + SH_SST - 1);
+    cp_async_commit();
+    cp_async_wait<SH_SST - 1>();
+    __syncwarp();
+    const int2 d = desc_at(i);
+    const int valid = d.x < 0 ? 0 : d.y & 31;
+    const uint32_t src = ring0 + (i % SH_SST) * SH_STAGE;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      uint32_t af[4];
+      const int chunk = 2 * ks + k_chk;
+      ldsm_x4(af[0], af[1], af[2], af[3], src + k_tok * 128 + ((chunk ^ (k_tok & 7)) << 4));
+      MmaOp<T>::run(s, af, qb[ks][0], qb[ks][1]);
+    }
+    const bool a0 = g < valid, a1 = g + 8 < valid;
+    s[0] = a0 ? s[0] * a.scale_log2 : -INFINITY;
+    s[1] = a0 ? s[1] * a.scale_log2 : -INFINITY;
+    s[2] = a1 ? s[2] * a.scale_log2 : -INFINITY;
+    s[3] = a1 ? s[3] * a.scale_log2 : -INFINITY;
+    float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+    }
+    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+    const float al0 = ex2(m0 - n0), al1 = ex2(m1 - n1);
+    m0 = n0;
+    m1 = n1;
+    const float p00 = ex2(s[0] - n0), p01 = ex2(s[1] - n1);
+    const float p10 = ex2(s[2] - n0), p11 = ex2(s[3] - n1);
+    l0 = l0 * al0 + (p00 + p10);
+    l1 = l1 * al1 + (p01 + p11);
+    const uint32_t pb0 = movmatrix_t(MmaOp<T>::pack(p00, p01)), pb1 = movmatrix_t(MmaOp<T>::pack(p10, p11));
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      o[mt][0] *= al0;
+      o[mt][2] *= al0;
+      o[mt][1] *= al1;
+      o[mt][3] *= al1;
+      uint32_t af[4];
+      const int chunk = 2 * mt + v_chk;
+      ldsm_x4_t(af[0], af[1], af[2], af[3], src + SH_TILE + v_tok * 128 + ((chunk ^ (v_tok & 7)) << 4));
+      MmaOp<T>::run(o[mt], af, pb0, pb1);
+    }
+    if (((d.y >> 5) & 1) || i == n - 1) {
+      // the sequence's last page of the range: its piece, then the next sequence's queries
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+      }
+      const float i0 = l0 > 0.f ? 1.f / l0 : 0.f, i1 = l1 > 0.f ? 1.f / l1 : 0.f;
+      const int64_t e = int64_t(a.stream_piece0 + r + sq) * a.n_heads + h * G;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        if (2 * c4 < G) {
+          float* po = a.part_o + (e + 2 * c4) * TC_D + mt * 16 + g;
+          __stcg(po, o[mt][0] * i0);
+          __stcg(po + 8, o[mt][2] * i0);
+        }
+        if (2 * c4 + 1 < G) {
+          float* po = a.part_o + (e + 2 * c4 + 1) * TC_D + mt * 16 + g;
+          __stcg(po, o[mt][1] * i1);
+          __stcg(po + 8, o[mt][3] * i1);
+        }
+      }
+      if (g == 0) {
+        if (2 * c4 < G) __stcg(a.part_ml + e + 2 * c4, make_float2(m0, l0));
+        if (2 * c4 + 1 < G) __stcg(a.part_ml + e + 2 * c4 + 1, make_float2(m1, l1));
+      }
+      ++sq;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        qb[ks][0] = qn[ks][0];
+        qb[ks][1] = qn[ks][1];
+      }
+      if (sq < sq_last) load_q(sq + 1, qn);
+      m0 = m1 = -1e30f;
+      l0 = l1 = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[mt][x] = 0.f;
+    }
+    __syncwarp();  // every lane has read the stage before its slot is filled again
+  }
+  cp_async_wait<0>();
+}
+
+// Tile role: the pipeline of prefill_tc_lean_kernel (pkv_prefill_tc.cu) over the
+// plan's items: warp 0 claims items and loads the query tile and the K / V blocks
+// by TMA, warp 1 issues S = Q K^T and O += P V (tcgen05, accumulators in TMEM),
+// warps 2-5 hold one row a thread: running maximum and sum, P to shared memory,
+// lazy rescale of O. The epilogue writes the row as a piece: O / l in fp32 and
+// (m, l). The first item of the CTAs that start with tiles is their own number.
+template <typename T, int G>
+__global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
     const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap qmap, const ShArgs a) {
-  constexpr int TPT = TC_ROWS / G;  // tokens per tile
   extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ int s_first;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  // the plan completed before this kernel could start and fenced its stores
+  const int n_items = __ldcg(&a.ctl->n_items) * a.n_kv;
+  const int n_stream = __ldcg(&a.ctl->n_stream);
+  const int n_tile = int(gridDim.x) - n_stream;  // CTAs [0, n_tile) start with tiles
+  const bool streams = int(blockIdx.x) >= n_tile;
+  if (!streams && int(blockIdx.x) >= n_items) {  // nothing for this CTA (uniform over the CTA)
+    pdl_wait();                                  // the counters belong to the previous launch until it completed
+    if (threadIdx.x == 0) tl_count_exit(a.claim);
+    return;
+  }
+  if (streams) {
+    const int ranges = __ldcg(&a.ctl->n_ranges), P = __ldcg(&a.ctl->listed);
+    pdl_wait();  // q and this layer's appended K/V rows are written by earlier kernels
+    const int w = (int(blockIdx.x) - n_tile) * SH_WARPS + warp;
+    for (int u = w; u < ranges * a.n_kv; u += n_stream * SH_WARPS) {
+      const int h = u % a.n_kv, r = u / a.n_kv;
+      const int p0 = int(int64_t(r) * P / ranges), p1 = int(int64_t(r + 1) * P / ranges);
+      if (p0 < p1) stream_range<T, G>(a, smem_raw + size_t(warp) * SH_SST * SH_STAGE, h, r, p0, p1, lane);
+    }
+    // the ring's generic-proxy accesses before the tiles' TMA writes
+    fence_proxy_async_smem();
+    if (threadIdx.x == 0) s_first = n_items > 0 ? n_tile + atomicAdd(a.claim, 1) : 0;
+    __syncthreads();
+    if (s_first >= n_items) {
+      if (threadIdx.x == 0) tl_count_exit(a.claim);
+      return;
+    }
+  } else if (threadIdx.x == 0) {
+    s_first = blockIdx.x;
+  }
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* qbuf = smem;                             // [128 rows][128 B], 128B swizzle
@@ -453,15 +723,6 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_tc_kernel(
   __shared__ uint32_t s_tmem;
   __shared__ ShItem s_item[2];
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
-  // the plan completed before this kernel could start and fenced its stores
-  const int n_items = __ldcg(&a.ctl->n_items) * a.n_kv;
-  if (int(blockIdx.x) >= n_items) {  // no item for this CTA (uniform over the CTA)
-    pdl_wait();                      // the counters belong to the previous launch until it completed
-    if (threadIdx.x == 0) tl_count_exit(a.claim);
-    return;
-  }
   if (threadIdx.x == 0) {
     prefetch_tmap(&tmap);
     prefetch_tmap(&qmap);
@@ -502,36 +763,19 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_tc_kernel(
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     const int kvc = 2 * a.layer;
-    const int chunk_pg = a.ctl->chunk * TC_PPB;
     uint32_t kiss = 0, viss = 0;  // K / V slots filled so far
     int it = 0;                   // items published
     bool dead = false;
+    int w = s_first;
     while (!dead) {
-      int w = 0;
-      if (lane == 0) w = atomicAdd(a.claim, 1);
-      w = __shfl_sync(0xffffffffu, w, 0);
       const bool end = w >= n_items;
       ShItem I{};
-      int pg_at = 0;  // first entry of the range in kv_indices
       if (!end) {
-        const int4 d = a.items[w / a.n_kv];
-        const ShEnt e = a.ents[d.x];
-        I.h = w % a.n_kv;
-        const int i0 = d.y * TPT;  // first token of the tile within the entity
-        I.t0 = e.t0 + i0;
-        I.nt = min(TPT, e.nt - i0);
-        const int first = e.pg0 + (e.base < 0 ? 0 : d.z * chunk_pg);
-        const int last = e.base < 0 ? e.pg1 : min(e.pg1, first + chunk_pg);
-        I.lim0 = e.lim0 + e.causal * i0 - first * TC_P;
-        I.causal = e.causal;
-        const int seen = I.lim0 + e.causal * (I.nt - 1);  // last key any of its rows sees
-        I.n_pg = seen < 0 ? 0 : min(last - first, seen / TC_P + 1);
-        I.nblk = max(1, (I.n_pg + TC_PPB - 1) / TC_PPB);  // a range no row sees: one block, all masked
-        I.tail_pg = e.lpl < TC_P && e.pg1 - 1 - first < I.n_pg ? e.pg1 - 1 - first : -1;
-        I.lpl = e.lpl;
-        I.piece = e.base < 0 ? -1 : e.base + d.z * e.nt + i0;
-        pg_at = e.pa + first;
+        const int4* d = reinterpret_cast<const int4*>(a.items + w / a.n_kv);
+        const int4 x = __ldg(d), y = __ldg(d + 1), z = __ldg(d + 2);
+        I = ShItem{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, w % a.n_kv, 0};
       }
+      const int pg_at = I.pg_at;
       bool pg_bad = false;
       for (int pg = lane; pg < I.n_pg; pg += 32) {
         const int id = a.kv_indices[pg_at + pg];
@@ -588,6 +832,8 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_tc_kernel(
       }
       dead = __shfl_sync(0xffffffffu, dead, 0);
       ++it;
+      if (lane == 0) w = n_tile + atomicAdd(a.claim, 1);
+      w = __shfl_sync(0xffffffffu, w, 0);
     }
     if (dead && lane == 0) {
       // let this CTA's own copies land before its shared memory can be released
@@ -837,11 +1083,12 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_tc_kernel(
   if (threadIdx.x == 0) tl_count_exit(a.claim);
 }
 
-size_t sh_smem() { return 1024 + 2 * size_t(TC_QTILE) + size_t(2 * SH_NST) * TC_KTILE + 256; }
+// the tile role's buffers (1 KiB to align them), or the streaming warps' rings
+size_t sh_smem() { return std::max(1024 + 2 * size_t(TC_QTILE) + size_t(2 * SH_NST) * TC_KTILE + 256, SH_RING); }
 
 // ---------------------------------------------------------------- merge
-// Rows of several-token sequences of shared groups: one warp per (token, query
-// head) merges the row's prefix pieces and its own.
+// One warp per (token, query head): its pieces over the shared keys and over its
+// own -> out. Two dims a lane, four pieces' loads in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) shared_merge_kernel(const int4* fold, const int4* rest, const float* part_o,
                                                            const float2* part_ml, void* out, int n_tokens,
@@ -857,18 +1104,29 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const int4* fold, con
   const int4 b = __ldcg(rest + t);  // the plan's: complete before any kernel of the step started
   const int4 f = __ldcg(fold + t);
   pdl_wait();
-  if (b.y <= 0) return;  // a one-token row or one written straight to out
+  if (b.y <= 0) return;  // written straight to out, or its tables are inconsistent
+  const int n = f.y + b.y;
+  constexpr int U = 4;
   float M = -1e30f, L = 0.f, y0 = 0.f, y1 = 0.f;
-  for (int i = 0; i < f.y + b.y; ++i) {
-    const int64_t p = i < f.y ? int64_t(f.x) + int64_t(i) * f.z : int64_t(b.x) + int64_t(i - f.y) * b.z;
-    const float2 ml = __ldcg(part_ml + p * n_heads + hh);
-    const float2 v = __ldcg(reinterpret_cast<const float2*>(part_o + (p * n_heads + hh) * TC_D) + lane);
-    const float Mn = fmaxf(M, ml.x);
-    const float c = ex2(M - Mn), k = ml.y * ex2(ml.x - Mn);
-    y0 = y0 * c + k * v.x;
-    y1 = y1 * c + k * v.y;
-    L = L * c + k;
-    M = Mn;
+  for (int i0 = 0; i0 < n; i0 += U) {
+    float2 ml[U], v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      const int64_t p = i < f.y ? int64_t(f.x) + int64_t(i) * f.z : int64_t(b.x) + int64_t(i - f.y) * b.z;
+      ml[u] = i < n ? __ldcg(part_ml + p * n_heads + hh) : make_float2(-1e30f, 0.f);
+      v[u] = i < n ? __ldcg(reinterpret_cast<const float2*>(part_o + (p * n_heads + hh) * TC_D) + lane)
+                   : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float Mn = fmaxf(M, ml[u].x);
+      const float c = ex2(M - Mn), k = ml[u].y * ex2(ml[u].x - Mn);
+      y0 = y0 * c + k * v[u].x;
+      y1 = y1 * c + k * v[u].y;
+      L = L * c + k;
+      M = Mn;
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   reinterpret_cast<uint32_t*>(static_cast<T*>(out) + (int64_t(t) * n_heads + hh) * TC_D)[lane] =
@@ -881,7 +1139,9 @@ int check_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* b) {
   if (!b) return fail(PKV_ERR_ARG, "batch descriptor is NULL");
   if (n_heads <= 0 || n_heads % pool->n_kv_heads)
     return fail(PKV_ERR_ARG, "n_heads must be a positive multiple of n_kv_heads");
-  if (!decode_fold_supported(*pool, n_heads))
+  const int g = n_heads / pool->n_kv_heads;
+  if ((pool->dtype != PKV_F16 && pool->dtype != PKV_BF16) || pool->head_dim != TC_D || pool->block_size != TC_P ||
+      pool->n_kv_heads > 8 || (g != 1 && g != 2 && g != 4 && g != 8))
     return fail(PKV_ERR_UNSUPPORTED, "shared-prefix attention takes fp16 / bf16 pools, head_dim 64, 16-token pages, "
                                      "up to 8 KV heads and 1, 2, 4 or 8 query heads per KV head");
   if (b->n_seqs <= 0) return fail(PKV_ERR_ARG, "batch has no sequences");
@@ -902,15 +1162,15 @@ int launch_shared_t(const CUtensorMap& tm, const CUtensorMap& qm, const ShArgs& 
     std::lock_guard<std::mutex> lock(mu);
     if ((int)ready.size() <= dev) ready.resize(dev + 1, 0);
     if (!ready[dev]) {
-      PKV_CUDA_RET(cudaFuncSetAttribute(shared_tc_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      PKV_CUDA_RET(cudaFuncSetAttribute(shared_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         int(sh_smem())));
-      // three CTAs of ~67 KiB need the whole shared-memory carveout
-      PKV_CUDA_RET(cudaFuncSetAttribute(shared_tc_kernel<T, G>, cudaFuncAttributePreferredSharedMemoryCarveout,
+      // three CTAs of ~73 KiB need the whole shared-memory carveout
+      PKV_CUDA_RET(cudaFuncSetAttribute(shared_kernel<T, G>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                         int(cudaSharedmemCarveoutMaxShared)));
       ready[dev] = 1;
     }
   }
-  PKV_CUDA_RET(launch_kernel(shared_tc_kernel<T, G>, dim3(grid), dim3(TC_THREADS), sh_smem(), s, true, tm, qm, a));
+  PKV_CUDA_RET(launch_kernel(shared_kernel<T, G>, dim3(grid), dim3(TC_THREADS), sh_smem(), s, true, tm, qm, a));
   return PKV_OK;
 }
 
@@ -935,7 +1195,7 @@ extern "C" size_t pkv_shared_workspace_size(const pkv_pool* pool, int32_t n_head
                                             int64_t total_pages) {
   if (!pool || pool->n_kv_heads <= 0 || n_heads < pool->n_kv_heads || n_seqs <= 0 || n_tokens < 0 || total_pages < 0)
     return 0;
-  return sh_layout(n_heads, std::min(8, n_heads / pool->n_kv_heads), n_seqs, n_tokens, total_pages).total;
+  return sh_layout(n_heads, pool->n_kv_heads, n_seqs, n_tokens, total_pages).total;
 }
 
 extern "C" int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* batch, int32_t n_groups,
@@ -946,7 +1206,7 @@ extern "C" int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_
     return fail(PKV_ERR_ARG, "n_groups must be between 1 and the number of sequences");
   if (!group_indptr || !prefix_pages) return fail(PKV_ERR_ARG, "group_indptr and prefix_pages must be non-NULL");
   const int groups = n_heads / pool->n_kv_heads;
-  const ShLayout w = sh_layout(n_heads, groups, batch->n_seqs, batch->n_tokens, batch->total_pages);
+  const ShLayout w = sh_layout(n_heads, pool->n_kv_heads, batch->n_seqs, batch->n_tokens, batch->total_pages);
   if (!workspace || workspace_bytes < w.total)
     return fail(PKV_ERR_ARG, "workspace too small: need " + std::to_string(w.total) + " bytes");
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(PKV_ERR_ARG, "workspace must be 256-byte aligned");
@@ -967,20 +1227,21 @@ extern "C" int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_
   a.n_groups = n_groups;
   a.n_kv = pool->n_kv_heads;
   a.tpt = TC_ROWS / groups;
-  a.slots = SH_MINB * num_sms();
+  a.sms = num_sms();
+  a.grid = SH_MINB * num_sms();
   a.splits_cap = split_cap(batch->n_tokens);
   a.pieces_cap = w.pieces;
   a.items_cap = w.items_cap;
   a.ctl = reinterpret_cast<ShCtl*>(ws + w.ctl);
   a.rows = reinterpret_cast<int32_t*>(ws + w.rows);
+  a.list = reinterpret_cast<int2*>(ws + w.list);
   a.seq_np = reinterpret_cast<int32_t*>(ws + w.seq_np);
   a.group_bad = reinterpret_cast<int32_t*>(ws + w.group_bad);
   a.ents = reinterpret_cast<ShEnt*>(ws + w.ents);
-  a.items = reinterpret_cast<int4*>(ws + w.items);
+  a.items = reinterpret_cast<ShItem*>(ws + w.items);
+  a.desc = reinterpret_cast<int2*>(ws + w.desc);
   a.fold = reinterpret_cast<int4*>(ws + w.fold);
   a.rest = reinterpret_cast<int4*>(ws + w.rest);
-  a.desc = reinterpret_cast<int4*>(ws + w.dec.page_desc);
-  a.counters = reinterpret_cast<int32_t*>(ws + w.dec.counters);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   PKV_CUDA_RET(cudaMemsetAsync(a.group_bad, 0, sizeof(int32_t) * size_t(batch->n_seqs), s));
   shared_check_kernel<<<unsigned(batch->n_seqs), 128, 0, s>>>(a);
@@ -991,8 +1252,8 @@ extern "C" int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_
 }
 
 extern "C" int pkv_attend_shared_planned(const pkv_pool* pool, int32_t layer, int32_t n_heads, const void* q,
-                                         void* out, float scale, const pkv_batch* batch, int32_t decode_hint,
-                                         void* workspace, size_t workspace_bytes, void* stream) {
+                                         void* out, float scale, const pkv_batch* batch, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
   if (int rc = check_shared(pool, n_heads, batch)) return rc;
   const pkv_pool& p = *pool;
   if (layer < 0 || layer >= p.num_layers)
@@ -1003,7 +1264,7 @@ extern "C" int pkv_attend_shared_planned(const pkv_pool* pool, int32_t layer, in
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
     return fail(PKV_ERR_ARG, "q and out must be 16-byte aligned");
   const int groups = n_heads / p.n_kv_heads;
-  const ShLayout w = sh_layout(n_heads, groups, batch->n_seqs, batch->n_tokens, batch->total_pages);
+  const ShLayout w = sh_layout(n_heads, pool->n_kv_heads, batch->n_seqs, batch->n_tokens, batch->total_pages);
   if (!workspace || workspace_bytes < w.total)
     return fail(PKV_ERR_ARG, "workspace too small: need " + std::to_string(w.total) + " bytes");
   char* ws = static_cast<char*>(workspace);
@@ -1012,12 +1273,19 @@ extern "C" int pkv_attend_shared_planned(const pkv_pool* pool, int32_t layer, in
   if (int rc = pool_tmap_head(p, &tm)) return rc;
   if (int rc = q_tmap(p.dtype, q, batch->n_tokens, n_heads, groups, &qm)) return rc;
   ShArgs a;
+  a.q = q;
   a.out = out;
   a.ctl = reinterpret_cast<const ShCtl*>(ws + w.ctl);
   a.claim = reinterpret_cast<ShCtl*>(ws + w.ctl)->claim;
-  a.ents = reinterpret_cast<const ShEnt*>(ws + w.ents);
-  a.items = reinterpret_cast<const int4*>(ws + w.items);
+  a.items = reinterpret_cast<const ShItem*>(ws + w.items);
+  a.desc = reinterpret_cast<const int2*>(ws + w.desc);
+  a.rows = reinterpret_cast<const int32_t*>(ws + w.rows);
   a.kv_indices = batch->kv_indices;
+  a.k_slab = static_cast<const char*>(p.base) + int64_t(2) * layer * slab_bytes(p);
+  a.v_slab = a.k_slab + slab_bytes(p);
+  a.stream_piece0 = int(w.pieces);
+  a.n_tokens = batch->n_tokens;
+  a.n_seqs = batch->n_seqs;
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
   a.st = batch->dev_status;
@@ -1026,25 +1294,16 @@ extern "C" int pkv_attend_shared_planned(const pkv_pool* pool, int32_t layer, in
   a.n_kv = p.n_kv_heads;
   a.layer = layer;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const int grid = int(std::min<int64_t>(w.items_cap * p.n_kv_heads, int64_t(SH_MINB) * num_sms()));
+  const int grid = SH_MINB * num_sms();
   int rc = p.dtype == PKV_F16 ? launch_shared_g<__half>(groups, tm, qm, a, grid, s)
                               : launch_shared_g<__nv_bfloat16>(groups, tm, qm, a, grid, s);
   if (rc) return rc;
-  const int4* fold = reinterpret_cast<const int4*>(ws + w.fold);
-  const int4* rest = reinterpret_cast<const int4*>(ws + w.rest);
-  if (decode_hint != 2) {  // one-token sequences
-    rc = decode_fold(p, layer, n_heads, q, out, scale, *batch, ws, reinterpret_cast<const int32_t*>(ws + w.rows),
-                     &a.ctl->p_dec, fold, a.part_o, a.part_ml, s);
-    if (rc) return rc;
-  }
-  if (decode_hint != 1) {  // several-token sequences
-    const int64_t warps = int64_t(batch->n_tokens) * n_heads;
-    const int64_t blocks = (warps * 32 + 255) / 256;
-    if (blocks >= (int64_t(1) << 31)) return fail(PKV_ERR_ARG, "too many tokens for one call");
-    auto kern = p.dtype == PKV_F16 ? shared_merge_kernel<__half> : shared_merge_kernel<__nv_bfloat16>;
-    PKV_CUDA_RET(launch_kernel(kern, dim3(unsigned(blocks)), dim3(256), 0, s, true, fold, rest,
-                               static_cast<const float*>(a.part_o), static_cast<const float2*>(a.part_ml), out,
-                               batch->n_tokens, n_heads));
-  }
+  const int64_t blocks = (int64_t(batch->n_tokens) * n_heads * 32 + 255) / 256;
+  if (blocks >= (int64_t(1) << 31)) return fail(PKV_ERR_ARG, "too many tokens for one call");
+  auto kern = p.dtype == PKV_F16 ? shared_merge_kernel<__half> : shared_merge_kernel<__nv_bfloat16>;
+  PKV_CUDA_RET(launch_kernel(kern, dim3(unsigned(blocks)), dim3(256), 0, s, true,
+                             reinterpret_cast<const int4*>(ws + w.fold), reinterpret_cast<const int4*>(ws + w.rest),
+                             static_cast<const float*>(a.part_o), static_cast<const float2*>(a.part_ml), out,
+                             batch->n_tokens, n_heads));
   return PKV_OK;
 }

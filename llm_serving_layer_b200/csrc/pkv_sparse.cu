@@ -19,12 +19,17 @@
 // fp32 online softmax) with the pages spread over its warps and merged at the
 // end.
 #include <algorithm>
+#include <mutex>
+#include <string>
 #include <type_traits>
+#include <vector>
 
 #include "pkv_common.cuh"
 
 namespace pkv {
 namespace {
+
+struct Row;
 
 struct SparseArgs {
   const void* q;
@@ -34,53 +39,61 @@ struct SparseArgs {
   const float* scales;   // [num_blocks][n_kv]
   const char* k_slab;
   const char* v_slab;
-  const int32_t* cu_q;
-  const int32_t* kv_lens;
-  const int32_t* kv_indptr;
+  const Row* rows;       // [n_tokens], the plan's
   const int32_t* kv_indices;
-  const int32_t* last_page_len;
-  const int32_t* batch_indices;
   int32_t* st;
-  int64_t num_blocks, total_pages;
-  int n_seqs, n_tokens, n_heads, n_kv, groups, d, page;
+  int64_t num_blocks;
+  int n_tokens, n_heads, n_kv, groups, d, page;
   int budget, sink, recent, max_pages;
   int mode;              // PKV_SPARSE_SELECT | PKV_SPARSE_ATTEND
   float scale_log2;
 };
 
-constexpr uint32_t KEY_FORCED = 0xffffffffu;  // first / last pages, always listed
-
 // unsigned order = order of the scores; not a number above every number
 __device__ __forceinline__ uint32_t score_key(float x) {
-  if (x != x) return 0xfffffffeu;
+  if (x != x) return 0xffffffffu;
   const uint32_t b = __float_as_uint(x + 0.f);  // -0 counts as 0
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// What a CTA works on: query t's sequence, its page list, its position.
+// What a CTA works on, one entry per query token, written by the plan: first
+// entry of its sequence's page list, its position, and whether the step's tables
+// are consistent for it (0: the row is zeros).
 struct Row {
-  bool ok;
-  int64_t pa;   // first entry of its page list
-  int mine;     // page (of the list) that holds the query's own token
-  int pos;      // the query's position
+  int pa, pos, ok, unused;
 };
-__device__ __forceinline__ Row find_row(const SparseArgs& a, int t) {
-  Row r{false, 0, 0, 0};
+static_assert(sizeof(Row) == sizeof(int4), "the plan's rows are int4");
+
+struct RowArgs {
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  const int32_t* kv_indptr;
+  const int32_t* last_page_len;
+  const int32_t* batch_indices;
+  int32_t* st;
+  Row* rows;
+  int64_t total_pages;
+  int n_seqs, n_tokens, page, max_pages;
+};
+__global__ void __launch_bounds__(256) sparse_plan_kernel(const RowArgs a) {
+  const int t = blockIdx.x * blockDim.x + threadIdx.x;
+  if (t >= a.n_tokens) return;
+  Row r{0, 0, 0, 0};
   const int s = a.batch_indices[t];
-  if (s < 0 || s >= a.n_seqs) return r;
-  const int q0 = a.cu_q[s], q1 = a.cu_q[s + 1];
-  const int64_t pa = a.kv_indptr[s], pb = a.kv_indptr[s + 1];
-  const int lpl = a.last_page_len[s];
-  const int64_t kv = (pb - pa - 1) * a.page + lpl;
-  if (t < q0 || t >= q1 || pa < 0 || pb <= pa || pb > a.total_pages || lpl < 1 || lpl > a.page ||
-      kv < q1 - q0 || kv >= 0x7fffffff || pb - pa > a.max_pages)
-    return r;
-  if (a.kv_lens && a.kv_lens[s] != kv) return r;
-  r.ok = true;
-  r.pa = pa;
-  r.pos = int(kv) - (q1 - t);
-  r.mine = r.pos / a.page;
-  return r;
+  if (s >= 0 && s < a.n_seqs) {
+    const int q0 = a.cu_q[s], q1 = a.cu_q[s + 1];
+    const int64_t pa = a.kv_indptr[s], pb = a.kv_indptr[s + 1];
+    const int lpl = a.last_page_len[s];
+    const int64_t kv = (pb - pa - 1) * a.page + lpl;
+    if (t >= q0 && t < q1 && pa >= 0 && pb > pa && pb <= a.total_pages && lpl >= 1 && lpl <= a.page &&
+        kv >= q1 - q0 && kv < 0x7fffffff && pb - pa <= a.max_pages && (!a.kv_lens || a.kv_lens[s] == kv)) {
+      r.pa = int(pa);
+      r.pos = int(kv) - (q1 - t);
+      r.ok = 1;
+    }
+  }
+  if (!r.ok) flag(a.st, PKV_DEV_META_BAD);
+  a.rows[t] = r;
 }
 
 // q8 of the KV head's query heads into q8s [groups][2 d] (negative parts, then
@@ -106,117 +119,117 @@ __device__ __forceinline__ void quantise_query(const SparseArgs& a, const T* q, 
 }
 
 struct SelectSmem {
-  uint32_t hist[256];
-  uint32_t wsum[2][32];
-  uint32_t prefix, need, ties;
+  uint32_t hist[3][256];  // reversed bins: entry 255 - b counts bin b
+  uint32_t cnt[2][32];    // per warp: keys above the threshold, keys equal to it
+  uint32_t lo, hi;        // range of the scored keys
 };
 
-// The `budget` largest of keys[0..n) (n > budget), ties to the lowest index,
-// into list[0..budget) ascending. Radix selection of the threshold, 8 bits a
-// pass, ending as soon as a prefix holds exactly what is still needed, then one
-// ordered compaction pass. All threads of the CTA call it.
-__device__ __forceinline__ void select_top(const uint32_t* keys, int n, int budget, int* list, SelectSmem& sm) {
+// Before the scores: an empty range and histogram (a barrier follows).
+__device__ __forceinline__ void select_init(SelectSmem& sm) {
+  for (int i = threadIdx.x; i < 256; i += blockDim.x) sm.hist[0][i] = 0;
+  if (threadIdx.x == 0) {
+    sm.lo = 0xffffffffu;
+    sm.hi = 0u;
+  }
+}
+// Pages [f0, f1) of n are scored; the first and the last are listed anyway.
+__device__ __forceinline__ int first_scored(const SparseArgs& a, int n) { return min(a.sink, n); }
+__device__ __forceinline__ int end_scored(const SparseArgs& a, int n) { return max(min(a.sink, n), n - a.recent); }
+
+// The query's `a.budget` pages out of n > budget: the unscored ones and the
+// highest keys[p] of the others, ties to the lowest page; put(i, p) gets the
+// i-th of them in ascending order. sm.lo / sm.hi hold the scored keys' range.
+// Threshold search by 256-bin histograms over the keys' range (scores lie close
+// together: equal-width bins over their range separate them in one or two
+// passes, where fixed digits spend the first on common leading bits), until the
+// threshold's bin is listed whole or holds one value: one barrier a pass, since
+// every warp scans the bins itself. Then each warp counts and writes a
+// contiguous share of the pages. All threads call it.
+template <typename Put>
+__device__ __forceinline__ void select_top(const SparseArgs& a, const uint32_t* keys, int n, SelectSmem& sm, Put put) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
-  uint32_t prefix = 0, mask = 0, need = budget;
-  bool ties = true;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += nt) sm.hist[i] = 0;
-    __syncthreads();
-    for (int p = tid; p < n; p += nt) {
+  const int f0 = first_scored(a, n), f1 = end_scored(a, n);
+  uint32_t lo = sm.lo, hi = sm.hi;
+  uint32_t need = uint32_t(a.budget - f0 - (n - f1));  // scored pages to list (fewer than there are)
+  int buf = 0;
+  while (need > 0 && lo < hi) {
+    const int shift = max(0, 24 - __clz(hi - lo));  // (hi - lo) >> shift < 256
+    for (int p = f0 + tid; p < f1; p += nt) {
       const uint32_t k = keys[p];
-      if ((k & mask) == prefix) atomicAdd(&sm.hist[(k >> shift) & 255u], 1u);
+      if (k >= lo && k <= hi) atomicAdd(&sm.hist[buf][255 - ((k - lo) >> shift)], 1u);
     }
+    // the next pass's bins, last read two passes ago: every warp has since met a barrier
+    const int next = buf == 2 ? 0 : buf + 1;
+    for (int i = tid; i < 256; i += nt) sm.hist[next][i] = 0;
     __syncthreads();
-    if (warp == 0) {  // lane l: bins 255 - 8 l .. 248 - 8 l
-      uint32_t c[8], sum = 0;
+    // lane l: bins 255 - 8 l .. 248 - 8 l
+    const uint4 x = reinterpret_cast<const uint4*>(sm.hist[buf])[2 * lane];
+    const uint4 y = reinterpret_cast<const uint4*>(sm.hist[buf])[2 * lane + 1];
+    const uint32_t c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    const uint32_t sum = (x.x + x.y) + (x.z + x.w) + ((y.x + y.y) + (y.z + y.w));
+    uint32_t incl = sum;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        c[u] = sm.hist[255 - 8 * lane - u];
-        sum += c[u];
-      }
-      uint32_t incl = sum;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += x;
-      }
-      const uint32_t before = incl - sum;
-      if (before < need && incl >= need) {  // exactly one lane
-        uint32_t above = before;
-        int u = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (u == j && above + c[j] < need) {
-            above += c[j];
-            u = j + 1;
-          }
-        sm.prefix = prefix | (uint32_t(255 - 8 * lane - u) << shift);
-        sm.need = need - above;
-        sm.ties = (sm.hist[255 - 8 * lane - u] != need - above) ? 1u : 0u;
-      }
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
     }
-    __syncthreads();
-    prefix = sm.prefix;
-    need = sm.need;
-    ties = sm.ties != 0;
-    mask |= 0xffu << shift;
-    if (!ties) break;
+    // the first lane whose bins reach `need`, then its first such bin
+    const int src = __ffs(__ballot_sync(0xffffffffu, incl >= need)) - 1;
+    uint32_t above = incl - sum, u = 0, cu = c[0];
+#pragma unroll
+    for (int v = 1; v < 8; ++v)
+      if (u == uint32_t(v - 1) && above + cu < need) {
+        above += cu;
+        u = v;
+        cu = c[v];
+      }
+    above = __shfl_sync(0xffffffffu, above, src);
+    cu = __shfl_sync(0xffffffffu, cu, src);
+    const uint32_t b = 255u - 8u * src - __shfl_sync(0xffffffffu, u, src);
+    need -= above;
+    const uint32_t top = lo + (((b + 1) << shift) - 1);  // wraps where the bin reaches past the last key
+    const uint32_t bin_lo = lo + (b << shift);
+    hi = min(hi, top < lo ? 0xffffffffu : top);
+    lo = bin_lo;
+    if (cu == need) break;  // every key of [lo, hi] is listed
+    buf = next;
   }
-  // listed: key above the threshold prefix, or (no excess ties) equal to it, or the first `need` equal ones
-  uint32_t base_sel = 0, base_eq = 0;
-  for (int p0 = 0; p0 < n; p0 += nt) {
-    const int p = p0 + tid;
-    const uint32_t k = p < n ? keys[p] & mask : 0u;
-    const bool eq = p < n && k == prefix;
-    bool sel = p < n && k > prefix;
-    const uint32_t beq = __ballot_sync(0xffffffffu, eq);
-    if (ties) {
-      if (lane == 0) sm.wsum[0][warp] = __popc(beq);
-      __syncthreads();
-      uint32_t before = base_eq, all = 0;
-      for (int w = 0; w < nw; ++w) {
-        const uint32_t c = sm.wsum[0][w];
-        if (w < warp) before += c;
-        all += c;
-      }
-      base_eq += all;
-      if (eq && before + __popc(beq & ((1u << lane) - 1u)) < need) sel = true;
-    } else {
-      sel = sel || eq;
-    }
+  // listed: keys above hi, then `need` of those in [lo, hi] in page order (all of them, or they are equal)
+  const int seg = (n + nw * 32 - 1) / (nw * 32) * 32;
+  const int p0 = min(n, warp * seg), p1 = min(n, p0 + seg);
+  auto judge = [&](int p, bool& gt, bool& eq) {
+    const uint32_t k = p < p1 ? keys[p] : 0u;
+    gt = p < p1 && (p < f0 || p >= f1 || k > hi);
+    eq = p < p1 && !gt && need > 0 && k >= lo;
+  };
+  uint32_t n_gt = 0, n_eq = 0;
+#pragma unroll 4
+  for (int q = p0; q < p1; q += 32) {
+    bool gt, eq;
+    judge(q + lane, gt, eq);
+    n_gt += gt;
+    n_eq += eq;
+  }
+  n_gt = __reduce_add_sync(0xffffffffu, n_gt);
+  n_eq = __reduce_add_sync(0xffffffffu, n_eq);
+  if (lane == 0) {
+    sm.cnt[0][warp] = n_gt;
+    sm.cnt[1][warp] = n_eq;
+  }
+  __syncthreads();
+  uint32_t eq_before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.cnt[1][lane] : 0u);
+  uint32_t at = __reduce_add_sync(0xffffffffu, lane < warp ? sm.cnt[0][lane] : 0u) + min(eq_before, need);
+#pragma unroll 2
+  for (int q = p0; q < p1; q += 32) {
+    bool gt, eq;
+    judge(q + lane, gt, eq);
+    const uint32_t beq = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1u;
+    const bool sel = gt || (eq && eq_before + __popc(beq & below) < need);
     const uint32_t b = __ballot_sync(0xffffffffu, sel);
-    if (lane == 0) sm.wsum[1][warp] = __popc(b);
-    __syncthreads();
-    uint32_t before = base_sel, all = 0;
-    for (int w = 0; w < nw; ++w) {
-      const uint32_t c = sm.wsum[1][w];
-      if (w < warp) before += c;
-      all += c;
-    }
-    base_sel += all;
-    if (sel) list[before + __popc(b & ((1u << lane) - 1u))] = p;
-    __syncthreads();
+    if (sel) put(int(at + __popc(b & below)), q + lane);
+    at += __popc(b);
+    eq_before += __popc(beq);
   }
-}
-
-__device__ __forceinline__ bool forced_page(const SparseArgs& a, int p, int mine) {
-  return p < a.sink || p > mine - a.recent;
-}
-
-// list[0..len): the query's pages, ascending (a given list: as given); writes
-// the pages row of a selection. keys is scratch of n entries.
-__device__ __forceinline__ int finish_list(const SparseArgs& a, uint32_t* keys, int n, int* list, int32_t* prow,
-                                           SelectSmem& sm) {
-  int len = n;
-  if (n > a.budget) {
-    select_top(keys, n, a.budget, list, sm);
-    len = a.budget;
-  } else {
-    for (int p = threadIdx.x; p < n; p += blockDim.x) list[p] = p;
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < a.budget; i += blockDim.x) prow[i] = i < len ? list[i] : -1;
-  return len;
 }
 
 __device__ __forceinline__ void imma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -227,102 +240,189 @@ __device__ __forceinline__ void imma_s8(int (&d)[4], uint32_t a0, uint32_t a1, u
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes global -> shared, or 16 zero bytes when !ok
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  const int n = ok ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // ---------------------------------------------------------------- 16-bit kernel
-template <int D>
-constexpr int sp_tps() { return D == 64 ? 2 : 1; }  // 16-token tiles per ring stage (8 KiB of K and V)
-constexpr int SP_NST = 3;                            // ring stages per warp
+// Ring of one warp: NST stages of one 16-token K and V tile; reused for the
+// warps' merge pieces.
+template <int D, int NW, int NST>
+constexpr size_t sp_ring_bytes() {
+  constexpr size_t ring = size_t(NW) * NST * 2 * 16 * D * 2, merge = size_t(NW) * 8 * (D + 4) * 4;
+  return ring > merge ? ring : merge;
+}
 
-template <int D, int NW>
-constexpr size_t sp_ring_bytes() { return size_t(NW) * SP_NST * sp_tps<D>() * 2 * 16 * D * 2; }
+// Thread-block clusters: a row's CTAs (1 when the launch has no cluster).
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// address of this CTA's shared variable in the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void red_cluster_min(uint32_t addr, uint32_t v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.min.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void red_cluster_max(uint32_t addr, uint32_t v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 
-template <typename T, int D, int NW>
-__global__ void __launch_bounds__(NW * 32) sparse_kernel(const SparseArgs a) {
-  constexpr int TPS = sp_tps<D>();
+// One row (query, KV head) per cluster of `cs` CTAs (1: no cluster): the CTAs
+// share the row's scoring and its listed pages; rank 0 selects.
+// SU: groups of 32 pages a warp scores at a time; MINB: CTAs per SM.
+template <typename T, int D, int NW, int NST, int SU, int MINB>
+__global__ void __launch_bounds__(NW * 32, MINB) sparse_kernel(const SparseArgs a, int cs) {
   constexpr int TILE = 16 * D * 2;       // bytes of one 16-token K or V tile
-  constexpr int STAGE = TPS * 2 * TILE;
+  constexpr int STAGE = 2 * TILE;
   constexpr int CH = D / 8;              // 16-byte chunks per row
   constexpr int KS = D / 16;             // 16-dim steps
   constexpr int Q8S = 2 * D + 16;
+  constexpr int PS = D + 4;
   extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char* ring = smem;                                      // aliases keys (scores end before the ring starts)
+  unsigned char* ring = smem;                          // aliases keys (scores end before the ring starts)
   uint32_t* keys = reinterpret_cast<uint32_t*>(smem);
-  __shared__ int8_t q8s[8 * Q8S];
-  __shared__ float qs[8];
+  __shared__ __align__(16) int8_t q8s[8 * Q8S];
   __shared__ SelectSmem sel;
   __shared__ float2 ml_all[NW][8];
-  __shared__ int tile_valid[NW][SP_NST][TPS];  // visible tokens of each staged tile
-  const size_t big = max(sp_ring_bytes<D, NW>(), (size_t(a.max_pages) * 4 + 15) & ~size_t(15));
-  int* list = reinterpret_cast<int*>(smem + big);
+  __shared__ __align__(8) float2 ml_cta[8];
+  __shared__ int tile_valid[NW][NST];               // visible tokens of each staged tile
+  const size_t big = max(sp_ring_bytes<D, NW, NST>(), (size_t(a.max_pages) * 4 + 15) & ~size_t(15));
+  int* list = reinterpret_cast<int*>(smem + big);      // pages within the sequence
+  int* blks = list + a.budget;                         // their blocks (-1: outside the pool)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
-  const int t = int(blockIdx.x / unsigned(a.n_kv)), h = int(blockIdx.x % unsigned(a.n_kv));
+  const uint32_t rank = cs > 1 ? cluster_rank() : 0u;
+  const unsigned row_id = blockIdx.x / unsigned(cs);
+  const int t = int(row_id / unsigned(a.n_kv)), h = int(row_id % unsigned(a.n_kv));
   pdl_trigger();
   pdl_wait();  // q, the pool's new rows and the index may come from the kernels just before
-  const Row row = find_row(a, t);
+  const int4 row4 = __ldg(reinterpret_cast<const int4*>(a.rows + t));
   const int G = a.groups;
   const int64_t q0 = (int64_t(t) * a.n_heads + int64_t(h) * G) * D;
   const T* q = static_cast<const T*>(a.q) + q0;
+  // this lane's part of the queries as the score products' B operand, loaded
+  // while the row travels
+  uint32_t qb[KS][2];
+  if (g < G) {
+    const T* qr = q + g * D + 2 * c4;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qb[ks][0] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16));
+      qb[ks][1] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8));
+    }
+  } else {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qb[ks][0] = qb[ks][1] = 0u;
+  }
+  const struct { int64_t pa; int pos, mine; bool ok; } row{row4.x, row4.y, row4.y / a.page, row4.z != 0};
   T* out = static_cast<T*>(a.out) + q0;
   int32_t* prow = a.pages + (int64_t(t) * a.n_kv + h) * a.budget;
-  if (!row.ok) {
-    if (threadIdx.x == 0) flag(a.st, PKV_DEV_META_BAD);
-    if (a.mode & PKV_SPARSE_SELECT)
-      for (int i = threadIdx.x; i < a.budget; i += NW * 32) prow[i] = -1;
-    if (a.mode & PKV_SPARSE_ATTEND)
-      for (int i = threadIdx.x; i < G * D; i += NW * 32) out[i] = from_f<T>(0.f);
+  if (!row.ok) {  // uniform over the cluster
+    if (rank == 0) {
+      if (a.mode & PKV_SPARSE_SELECT)
+        for (int i = threadIdx.x; i < a.budget; i += NW * 32) prow[i] = -1;
+      if (a.mode & PKV_SPARSE_ATTEND)
+        for (int i = threadIdx.x; i < G * D; i += NW * 32) out[i] = from_f<T>(0.f);
+    }
     return;
   }
   int len = a.budget;
-  if (a.mode & PKV_SPARSE_SELECT) {
-    const int n = row.mine + 1;
-    if (n > a.budget) {
-      for (int i = threadIdx.x; i < 8 * Q8S; i += NW * 32) q8s[i] = 0;
-      if (threadIdx.x < 8) qs[threadIdx.x] = 0.f;
-      __syncthreads();
-      quantise_query<T>(a, q, q8s, Q8S, qs, warp, NW, lane);
-      __syncthreads();
-      // this lane's columns of B: head g, bytes 64 j + 16 c4 .. +15 of its 2 D
-      constexpr int J = 2 * D / 64;
-      uint4 b[J];
+  const int n = row.mine + 1;
+  if ((a.mode & PKV_SPARSE_SELECT) && n > a.budget) {
+    const int stride = cs * NW * 32 * SU;
+    int p0 = (int(rank) * NW + warp) * 32 * SU, id[SU];
 #pragma unroll
-      for (int j = 0; j < J; ++j) b[j] = *reinterpret_cast<const uint4*>(q8s + g * Q8S + 64 * j + 16 * c4);
-      const float s0 = qs[2 * c4], s1 = qs[2 * c4 + 1];
-      const bool v0 = 2 * c4 < G, v1 = 2 * c4 + 1 < G;
-      for (int p0 = warp * 32; p0 < n; p0 += NW * 32) {
-        const int pl = p0 + lane;
-        int id = pl < n ? a.kv_indices[row.pa + pl] : 0;
-        const bool oob = id < 0 || id >= a.num_blocks;
-        if (oob) {
+    for (int u = 0; u < SU; ++u) id[u] = p0 + 32 * u + lane < n ? a.kv_indices[row.pa + p0 + 32 * u + lane] : 0;
+    // int8 query: the lanes (g, c4) hold head g's elements; the scale by a
+    // maximum over the head's four lanes, the bytes through shared memory into
+    // B's layout (head g, bytes 64 j + 16 c4 .. +15 of its 2 D)
+    float top = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 x = unpack2<T>(qb[ks][e]);
+        top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float q_scale = __fmul_rn(top, 1.0f / 127.0f);
+    select_init(sel);
+    if (cs > 1) cluster_arrive();  // waited for before the first remote store
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks % NW != warp) continue;  // the warps share the 16-dim steps
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 x = unpack2<T>(qb[ks][e]);
+        int8_t* d8 = q8s + g * Q8S + ks * 16 + e * 8 + 2 * c4;
+        float y0 = q_scale > 0.f ? rintf(__fdiv_rn(x.x, q_scale)) : 0.f;
+        float y1 = q_scale > 0.f ? rintf(__fdiv_rn(x.y, q_scale)) : 0.f;
+        y0 = fminf(fmaxf(y0, -127.f), 127.f);
+        y1 = fminf(fmaxf(y1, -127.f), 127.f);
+        *reinterpret_cast<char2*>(d8) = make_char2(int8_t(fminf(y0, 0.f)), int8_t(fminf(y1, 0.f)));
+        *reinterpret_cast<char2*>(d8 + D) = make_char2(int8_t(fmaxf(y0, 0.f)), int8_t(fmaxf(y1, 0.f)));
+      }
+    }
+    __syncthreads();
+    constexpr int J = 2 * D / 64;
+    uint4 b[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) b[j] = *reinterpret_cast<const uint4*>(q8s + g * Q8S + 64 * j + 16 * c4);
+    // scales of this lane's columns, heads 2 c4 and 2 c4 + 1
+    const float s0 = __shfl_sync(0xffffffffu, q_scale, 8 * c4), s1 = __shfl_sync(0xffffffffu, q_scale, 8 * c4 + 4);
+    const bool v0 = 2 * c4 < G, v1 = 2 * c4 + 1 < G;
+    const uint32_t keys0 = cs > 1 ? map_rank(smem_u32(keys), 0) : smem_u32(keys);
+    if (cs > 1) cluster_wait();
+    const int f0 = first_scored(a, n), f1 = end_scored(a, n);
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    for (; p0 < n; p0 += stride) {
+      // SU groups of 32 pages: all their index loads are in flight together
+      uint4 w[SU][4][J];
+      float bs[SU];
+      bool oob[SU];
+#pragma unroll
+      for (int u = 0; u < SU; ++u) {
+        oob[u] = id[u] < 0 || id[u] >= a.num_blocks;
+        if (oob[u]) {
           flag(a.st, PKV_DEV_SLOT_OOB);
-          id = 0;
+          id[u] = 0;
         }
-        const float bs = a.scales[int64_t(id) * a.n_kv + h];
+        bs[u] = a.scales[int64_t(id[u]) * a.n_kv + h];
         // 4 rows of A per lane: pages g, g + 8, g + 16, g + 24 of the 32
-        uint4 w[4][J];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int64_t idr = __shfl_sync(0xffffffffu, id, g + 8 * r);
+          const int64_t idr = __shfl_sync(0xffffffffu, id[u], g + 8 * r);
           const uint4* src = reinterpret_cast<const uint4*>(a.codes + (idr * a.n_kv + h) * (2 * D)) + c4;
 #pragma unroll
-          for (int j = 0; j < J; ++j) w[r][j] = __ldg(src + 4 * j);
+          for (int j = 0; j < J; ++j) w[u][r][j] = __ldg(src + 4 * j);
         }
+      }
+#pragma unroll
+      for (int u = 0; u < SU; ++u) {
+        const int pn = p0 + stride + 32 * u + lane;
+        id[u] = pn < n ? a.kv_indices[row.pa + pn] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < SU; ++u) {
+        const int pl = p0 + 32 * u + lane;
         uint32_t mykey = 0;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           int acc[4] = {0, 0, 0, 0};
 #pragma unroll
           for (int j = 0; j < J; ++j) {
-            const uint4 &x = w[2 * half][j], &y = w[2 * half + 1][j];
+            const uint4 &x = w[u][2 * half][j], &y = w[u][2 * half + 1][j];
             imma_s8(acc, x.x, y.x, x.y, y.y, b[j].x, b[j].y);
             imma_s8(acc, x.z, y.z, x.w, y.w, b[j].z, b[j].w);
           }
@@ -335,71 +435,102 @@ __global__ void __launch_bounds__(NW * 32) sparse_kernel(const SparseArgs a) {
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             // row g of (half, r) = page 16 half + 8 r + g: hand it to that lane
             const float mm = __shfl_sync(0xffffffffu, m, (lane & 7) * 4);
-            if ((lane >> 3) == 2 * half + r) mykey = score_key(__fmul_rn(mm, bs));
+            if ((lane >> 3) == 2 * half + r) mykey = score_key(__fmul_rn(mm, bs[u]));
           }
         }
-        if (pl < n) keys[pl] = forced_page(a, pl, row.mine) ? KEY_FORCED : (oob ? 0u : mykey);
+        if (oob[u]) mykey = 0u;
+        if (pl >= f0 && pl < f1) {
+          lo = min(lo, mykey);
+          hi = max(hi, mykey);
+        }
+        if (pl < n) {
+          if (cs > 1) st_cluster(keys0 + 4 * pl, mykey);
+          else keys[pl] = mykey;
+        }
       }
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0 && lo <= hi) {  // this warp scored something: into rank 0's range
+      if (cs > 1) {
+        red_cluster_min(map_rank(smem_u32(&sel.lo), 0), lo);
+        red_cluster_max(map_rank(smem_u32(&sel.hi), 0), hi);
+      } else {
+        atomicMin(&sel.lo, lo);
+        atomicMax(&sel.hi, hi);
+      }
+    }
+    if (cs > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
       __syncthreads();
     }
-    len = finish_list(a, keys, n, list, prow, sel);
+  }
+  // ---- the list: pages, their blocks (-1 for what is not attended)
+  const bool attend = (a.mode & PKV_SPARSE_ATTEND) != 0;
+  auto block_of = [&](int p) -> int {
+    if (p < 0 || p > row.mine) return -1;
+    const int id = a.kv_indices[row.pa + p];
+    if (id >= 0 && id < a.num_blocks) return id;
+    flag(a.st, PKV_DEV_SLOT_OOB);
+    return -1;
+  };
+  if (a.mode & PKV_SPARSE_SELECT) {
+    len = min(n, a.budget);
+    if (n > a.budget) {
+      if (rank == 0)
+        select_top(a, keys, n, sel, [&](int i, int p) {
+          prow[i] = p;
+          if (!attend) return;
+          list[i] = p;
+          for (int r = 1; r < cs; ++r) st_cluster(map_rank(smem_u32(list + i), r), uint32_t(p));
+        });
+      if (cs > 1) {
+        cluster_arrive();
+        cluster_wait();  // rank 0's list is in every CTA
+      } else {
+        __syncthreads();
+      }
+    } else {
+      for (int i = threadIdx.x; i < a.budget; i += NW * 32) {
+        if (rank == 0) prow[i] = i < n ? i : -1;
+        if (i < n) list[i] = i;
+      }
+    }
   } else {
     for (int i = threadIdx.x; i < a.budget; i += NW * 32) list[i] = prow[i];
   }
+  if (!attend) return;
+  for (int i = threadIdx.x; i < len; i += NW * 32) blks[i] = block_of(list[i]);  // unselected lists: own entries
   __syncthreads();
-  if (!(a.mode & PKV_SPARSE_ATTEND)) return;
 
   // ---- attention over the listed pages, the tiles dealt to the warps in turn
   const int tpp = a.page / 16;
   const int n_tiles = len * tpp;
-  uint32_t qb[KS][2];
-  if (g < G) {
-    const T* qr = q + g * D + 2 * c4;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      qb[ks][0] = *reinterpret_cast<const uint32_t*>(qr + ks * 16);
-      qb[ks][1] = *reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8);
-    }
-  } else {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qb[ks][0] = qb[ks][1] = 0u;
-  }
-  const int n_stages = (n_tiles + TPS - 1) / TPS;
-  const int mine_stages = n_stages > warp ? (n_stages - warp + NW - 1) / NW : 0;
-  unsigned char* myring = ring + size_t(warp) * SP_NST * STAGE;
+  const int w0 = int(rank) * NW + warp, dw = cs * NW;  // this warp's tiles: w0, w0 + dw, ...
+  const int my_tiles = n_tiles > w0 ? (n_tiles - w0 + dw - 1) / dw : 0;
+  unsigned char* myring = ring + size_t(warp) * NST * STAGE;
   const uint32_t ring0 = smem_u32(myring);
   const int64_t row_b = int64_t(a.n_kv) * D * 2;
-  // valid tokens of tile i (0: not listed, past the query, outside the pool) and its block
-  auto tile = [&](int i, int64_t& tok0) -> int {
-    if (i >= n_tiles) return 0;
-    const int p = list[i / tpp];
-    if (p < 0 || p > row.mine) return 0;
-    const int first = p * a.page + (i % tpp) * 16;
-    if (first > row.pos) return 0;
-    const int id = a.kv_indices[row.pa + p];
-    if (id < 0 || id >= a.num_blocks) {
-      flag(a.st, PKV_DEV_SLOT_OOB);
-      return 0;
-    }
-    tok0 = int64_t(id) * a.page + (i % tpp) * 16;
-    return min(16, row.pos - first + 1);
-  };
-  auto load = [&](int k) {  // this warp's k-th stage
-    const uint32_t dst = ring0 + (k % SP_NST) * STAGE;
+  const int r0 = lane / CH, ch = lane % CH;  // this lane's chunk of each row it copies
+  const int64_t lane_off = int64_t(r0) * row_b + int64_t(h) * D * 2 + ch * 16;
+  auto load = [&](int k) {  // this warp's k-th tile
+    const uint32_t dst = ring0 + (k % NST) * STAGE;
+    const int i = w0 + k * dw;
+    const int e = tpp == 1 ? i : i / tpp, sub = tpp == 1 ? 0 : (i - e * tpp) * 16;
+    const int blk = blks[e];
+    const int valid = blk < 0 ? 0 : max(0, min(16, row.pos - (list[e] * a.page + sub) + 1));
+    if (lane == 0) tile_valid[warp][k % NST] = valid;
+    const int64_t off0 = (int64_t(blk) * a.page + sub) * row_b + lane_off;
 #pragma unroll
-    for (int u = 0; u < TPS; ++u) {
-      int64_t tok0 = 0;
-      const int valid = tile((warp + k * NW) * TPS + u, tok0);
-      if (lane == 0) tile_valid[warp][k % SP_NST][u] = valid;
-#pragma unroll
-      for (int c = 0; c < 16 * CH / 32; ++c) {
-        const int idx = c * 32 + lane, r = idx / CH, ch = idx % CH;
-        const int64_t off = (tok0 + r) * row_b + int64_t(h) * D * 2 + ch * 16;
-        const bool ok = r < valid;  // rows past the query's position are never read: zeros
-        const uint32_t sw = r * (D * 2) + ((ch ^ (r & 7)) << 4);
-        cp_async16(dst + (2 * u) * TILE + sw, a.k_slab + (ok ? off : 0), ok);
-        cp_async16(dst + (2 * u + 1) * TILE + sw, a.v_slab + (ok ? off : 0), ok);
-      }
+    for (int c = 0; c < 16 * CH / 32; ++c) {
+      const int r = c * (32 / CH) + r0;
+      const bool ok = r < valid;  // rows past the query's position are never read: zeros
+      const int64_t off = ok ? off0 + c * (32 / CH) * row_b : 0;
+      const uint32_t sw = r * (D * 2) + ((ch ^ (r & 7)) << 4);
+      cp_async16(dst + sw, a.k_slab + off, ok);
+      cp_async16(dst + TILE + sw, a.v_slab + off, ok);
     }
   };
   float o[KS][4];
@@ -411,44 +542,31 @@ __global__ void __launch_bounds__(NW * 32) sparse_kernel(const SparseArgs a) {
   const int k_tok = lane & 15, k_chk = lane >> 4;
   const int v_tok = (lane & 7) + ((lane >> 4) << 3), v_chk = (lane >> 3) & 1;
 #pragma unroll
-  for (int k = 0; k < SP_NST - 1; ++k) {
-    if (k < mine_stages) load(k);
+  for (int k = 0; k < NST - 1; ++k) {
+    if (k < my_tiles) load(k);
     cp_async_commit();
   }
-  for (int k = 0; k < mine_stages; ++k) {
-    if (k + SP_NST - 1 < mine_stages) load(k + SP_NST - 1);
+  for (int k = 0; k < my_tiles; ++k) {
+    if (k + NST - 1 < my_tiles) load(k + NST - 1);
     cp_async_commit();
-    cp_async_wait<SP_NST - 1>();
+    cp_async_wait<NST - 1>();
     __syncwarp();
-    const uint32_t src = ring0 + (k % SP_NST) * STAGE;
-    float s[TPS][4];
-    int valid[TPS];
+    const uint32_t src = ring0 + (k % NST) * STAGE;
+    const int valid = tile_valid[warp][k % NST];
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < TPS; ++u) {
-      valid[u] = tile_valid[warp][k % SP_NST][u];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[u][e] = 0.f;
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t af[4];
+      const int chunk = 2 * ks + k_chk;
+      ldsm_x4(af[0], af[1], af[2], af[3], src + k_tok * (D * 2) + ((chunk ^ (k_tok & 7)) << 4));
+      MmaOp<T>::run(s, af, qb[ks][0], qb[ks][1]);
     }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int u = 0; u < TPS; ++u) {
-        uint32_t af[4];
-        const int chunk = 2 * ks + k_chk;
-        ldsm_x4(af[0], af[1], af[2], af[3], src + (2 * u) * TILE + k_tok * (D * 2) + ((chunk ^ (k_tok & 7)) << 4));
-        MmaOp<T>::run(s[u], af, qb[ks][0], qb[ks][1]);
-      }
-    float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < TPS; ++u) {
-      const bool a0 = g < valid[u], a1 = g + 8 < valid[u];
-      s[u][0] = a0 ? s[u][0] * a.scale_log2 : -INFINITY;
-      s[u][1] = a0 ? s[u][1] * a.scale_log2 : -INFINITY;
-      s[u][2] = a1 ? s[u][2] * a.scale_log2 : -INFINITY;
-      s[u][3] = a1 ? s[u][3] * a.scale_log2 : -INFINITY;
-      x0 = fmaxf(x0, fmaxf(s[u][0], s[u][2]));
-      x1 = fmaxf(x1, fmaxf(s[u][1], s[u][3]));
-    }
+    const bool a0 = g < valid, a1 = g + 8 < valid;
+    s[0] = a0 ? s[0] * a.scale_log2 : -INFINITY;
+    s[1] = a0 ? s[1] * a.scale_log2 : -INFINITY;
+    s[2] = a1 ? s[2] * a.scale_log2 : -INFINITY;
+    s[3] = a1 ? s[3] * a.scale_log2 : -INFINITY;
+    float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
       x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
@@ -458,33 +576,21 @@ __global__ void __launch_bounds__(NW * 32) sparse_kernel(const SparseArgs a) {
     const float al0 = ex2(m0 - n0), al1 = ex2(m1 - n1);
     m0 = n0;
     m1 = n1;
-    float ls0 = 0.f, ls1 = 0.f;
-    uint32_t pb[TPS][2];
-#pragma unroll
-    for (int u = 0; u < TPS; ++u) {
-      const float p00 = ex2(s[u][0] - n0), p01 = ex2(s[u][1] - n1);
-      const float p10 = ex2(s[u][2] - n0), p11 = ex2(s[u][3] - n1);
-      ls0 += p00 + p10;
-      ls1 += p01 + p11;
-      pb[u][0] = movmatrix_t(MmaOp<T>::pack(p00, p01));
-      pb[u][1] = movmatrix_t(MmaOp<T>::pack(p10, p11));
-    }
-    l0 = l0 * al0 + ls0;
-    l1 = l1 * al1 + ls1;
+    const float p00 = ex2(s[0] - n0), p01 = ex2(s[1] - n1);
+    const float p10 = ex2(s[2] - n0), p11 = ex2(s[3] - n1);
+    l0 = l0 * al0 + (p00 + p10);
+    l1 = l1 * al1 + (p01 + p11);
+    const uint32_t pb0 = movmatrix_t(MmaOp<T>::pack(p00, p01)), pb1 = movmatrix_t(MmaOp<T>::pack(p10, p11));
 #pragma unroll
     for (int mt = 0; mt < KS; ++mt) {
       o[mt][0] *= al0;
       o[mt][2] *= al0;
       o[mt][1] *= al1;
       o[mt][3] *= al1;
-#pragma unroll
-      for (int u = 0; u < TPS; ++u) {
-        uint32_t af[4];
-        const int chunk = 2 * mt + v_chk;
-        ldsm_x4_t(af[0], af[1], af[2], af[3],
-                  src + (2 * u + 1) * TILE + v_tok * (D * 2) + ((chunk ^ (v_tok & 7)) << 4));
-        MmaOp<T>::run(o[mt], af, pb[u][0], pb[u][1]);
-      }
+      uint32_t af[4];
+      const int chunk = 2 * mt + v_chk;
+      ldsm_x4_t(af[0], af[1], af[2], af[3], src + TILE + v_tok * (D * 2) + ((chunk ^ (v_tok & 7)) << 4));
+      MmaOp<T>::run(o[mt], af, pb0, pb1);
     }
     __syncwarp();  // every lane has read the stage before its slot is filled again
   }
@@ -496,8 +602,7 @@ __global__ void __launch_bounds__(NW * 32) sparse_kernel(const SparseArgs a) {
   }
   // ---- merge of the warps' pieces (the ring is free once every warp is here)
   __syncthreads();
-  float* part = reinterpret_cast<float*>(ring);  // [NW][8][D + 4]
-  constexpr int PS = D + 4;
+  float* part = reinterpret_cast<float*>(ring);  // [NW][8][PS]
   {
     float* mp = part + size_t(warp) * 8 * PS;
 #pragma unroll
@@ -527,8 +632,36 @@ __global__ void __launch_bounds__(NW * 32) sparse_kernel(const SparseArgs a) {
       y0 += c * v.x;
       y1 += c * v.y;
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;  // nothing listed: zeros
-    reinterpret_cast<uint32_t*>(out)[i] = L > 0.f || L != L ? MmaOp<T>::pack(y0 * inv, y1 * inv) : 0u;
+    if (cs == 1) {
+      const float inv = L > 0.f ? 1.f / L : 0.f;  // nothing listed: zeros
+      reinterpret_cast<uint32_t*>(out)[i] = L > 0.f || L != L ? MmaOp<T>::pack(y0 * inv, y1 * inv) : 0u;
+    } else {  // this thread alone reads and writes these entries of warp 0's piece
+      *reinterpret_cast<float2*>(part + size_t(hh) * PS + e) = make_float2(y0, y1);
+      if (e == 0) ml_cta[hh] = make_float2(M, L);
+    }
+  }
+  if (cs > 1) {
+    // the CTAs' pieces, the output's elements shared among them
+    cluster_arrive();
+    cluster_wait();
+    for (int i = int(rank) * NW * 32 + threadIdx.x; i < G * D / 2; i += cs * NW * 32) {
+      const int hh = i / (D / 2), e = 2 * (i % (D / 2));
+      const uint32_t ml = smem_u32(ml_cta + hh), pc = smem_u32(part + size_t(hh) * PS + e);
+      float M = -1e30f;
+      for (int r = 0; r < cs; ++r) M = fmaxf(M, ld_cluster2(map_rank(ml, r)).x);
+      float L = 0.f, y0 = 0.f, y1 = 0.f;
+      for (int r = 0; r < cs; ++r) {
+        const float2 x = ld_cluster2(map_rank(ml, r)), v = ld_cluster2(map_rank(pc, r));
+        const float c = ex2(x.x - M);
+        L += c * x.y;
+        y0 += c * v.x;
+        y1 += c * v.y;
+      }
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      reinterpret_cast<uint32_t*>(out)[i] = L > 0.f || L != L ? MmaOp<T>::pack(y0 * inv, y1 * inv) : 0u;
+    }
+    cluster_arrive();
+    cluster_wait();  // no CTA leaves while another reads its pieces
   }
 }
 
@@ -550,13 +683,13 @@ __global__ void __launch_bounds__(256) sparse_generic_kernel(const SparseArgs a)
   const int t = int(blockIdx.x / unsigned(a.n_kv)), h = int(blockIdx.x % unsigned(a.n_kv));
   pdl_trigger();
   pdl_wait();
-  const Row row = find_row(a, t);
+  const int4 row4 = __ldg(reinterpret_cast<const int4*>(a.rows + t));
+  const struct { int64_t pa; int pos, mine; bool ok; } row{row4.x, row4.y, row4.y / a.page, row4.z != 0};
   const int64_t q0 = (int64_t(t) * a.n_heads + int64_t(h) * G) * D;
   const T* q = static_cast<const T*>(a.q) + q0;
   T* out = static_cast<T*>(a.out) + q0;
   int32_t* prow = a.pages + (int64_t(t) * a.n_kv + h) * a.budget;
   if (!row.ok) {
-    if (threadIdx.x == 0) flag(a.st, PKV_DEV_META_BAD);
     if (a.mode & PKV_SPARSE_SELECT)
       for (int i = threadIdx.x; i < a.budget; i += blockDim.x) prow[i] = -1;
     if (a.mode & PKV_SPARSE_ATTEND)
@@ -567,8 +700,11 @@ __global__ void __launch_bounds__(256) sparse_generic_kernel(const SparseArgs a)
   if (a.mode & PKV_SPARSE_SELECT) {
     const int n = row.mine + 1;
     if (n > a.budget) {
+      select_init(sel);
       quantise_query<T>(a, q, q8s, 2 * D, qs, warp, nw, lane);
       __syncthreads();
+      const int f0 = first_scored(a, n), f1 = end_scored(a, n);
+      uint32_t lo = 0xffffffffu, hi = 0u;
       for (int p = warp; p < n; p += nw) {
         const int64_t id = a.kv_indices[row.pa + p];
         uint32_t key = 0u;
@@ -586,11 +722,24 @@ __global__ void __launch_bounds__(256) sparse_generic_kernel(const SparseArgs a)
           }
           key = score_key(__fmul_rn(best, a.scales[id * a.n_kv + h]));
         }
-        if (lane == 0) keys[p] = forced_page(a, p, row.mine) ? KEY_FORCED : key;
+        if (lane == 0) keys[p] = key;
+        if (p >= f0 && p < f1) {
+          lo = min(lo, key);
+          hi = max(hi, key);
+        }
+      }
+      if (lane == 0 && lo <= hi) {
+        atomicMin(&sel.lo, lo);
+        atomicMax(&sel.hi, hi);
       }
       __syncthreads();
+      select_top(a, keys, n, sel, [&](int i, int p) { list[i] = p; });
+    } else {
+      for (int p = threadIdx.x; p < n; p += blockDim.x) list[p] = p;
     }
-    len = finish_list(a, keys, n, list, prow, sel);
+    len = min(n, a.budget);
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.budget; i += blockDim.x) prow[i] = i < len ? list[i] : -1;
   } else {
     for (int i = threadIdx.x; i < a.budget; i += blockDim.x) list[i] = prow[i];
   }
@@ -660,16 +809,52 @@ __global__ void __launch_bounds__(256) sparse_generic_kernel(const SparseArgs a)
 
 constexpr size_t SP_SMEM_MAX = 220 * 1024;  // dynamic part; the static part is below 7 KiB
 
-template <typename T, int D, int NW>
-int launch_sparse_t(const SparseArgs& a, cudaStream_t s) {
-  const size_t big = std::max(sp_ring_bytes<D, NW>(), (size_t(a.max_pages) * 4 + 15) & ~size_t(15));
-  const size_t smem = big + size_t(a.budget) * 4;
+// Raises a kernel's dynamic shared-memory limit once per device.
+struct SmemReady {
+  std::mutex mu;
+  std::vector<char> done;
+  int raise(const void* kern, int bytes) {
+    int dev = 0;
+    PKV_CUDA_RET(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if ((int)done.size() <= dev) done.resize(dev + 1, 0);
+    if (!done[dev]) {
+      PKV_CUDA_RET(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+      done[dev] = 1;
+    }
+    return PKV_OK;
+  }
+};
+
+template <typename T, int D, int NW, int NST, int SU, int MINB>
+int launch_sparse_t(const SparseArgs& a, int64_t rows, int cs, cudaStream_t s) {
+  const size_t big = std::max(sp_ring_bytes<D, NW, NST>(), (size_t(a.max_pages) * 4 + 15) & ~size_t(15));
+  const size_t smem = big + size_t(a.budget) * 8;
   if (smem > SP_SMEM_MAX)
     return fail(PKV_ERR_UNSUPPORTED, "page lists of " + std::to_string(a.max_pages) + " pages with a budget of " +
                                          std::to_string(a.budget) + " do not fit in shared memory");
-  auto kern = sparse_kernel<T, D, NW>;
-  PKV_CUDA_RET(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SP_SMEM_MAX)));
-  PKV_CUDA_RET(launch_kernel(kern, dim3(unsigned(int64_t(a.n_tokens) * a.n_kv)), dim3(NW * 32), smem, s, true, a));
+  auto kern = sparse_kernel<T, D, NW, NST, SU, MINB>;
+  static SmemReady ready;
+  if (int rc = ready.raise(reinterpret_cast<const void*>(kern), int(SP_SMEM_MAX))) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(rows * cs));
+  cfg.blockDim = dim3(NW * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cs > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim = {unsigned(cs), 1u, 1u};
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  PKV_CUDA_RET(cudaLaunchKernelEx(&cfg, kern, a, cs));
   return PKV_OK;
 }
 
@@ -680,7 +865,8 @@ int launch_sparse_generic(const SparseArgs& a, cudaStream_t s) {
     return fail(PKV_ERR_UNSUPPORTED, "page lists of " + std::to_string(a.max_pages) + " pages with a budget of " +
                                          std::to_string(a.budget) + " do not fit in shared memory");
   auto kern = sparse_generic_kernel<T>;
-  PKV_CUDA_RET(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SP_SMEM_MAX)));
+  static SmemReady ready;
+  if (int rc = ready.raise(reinterpret_cast<const void*>(kern), int(SP_SMEM_MAX))) return rc;
   PKV_CUDA_RET(launch_kernel(kern, dim3(unsigned(int64_t(a.n_tokens) * a.n_kv)), dim3(256), smem, s, true, a));
   return PKV_OK;
 }
@@ -688,7 +874,15 @@ int launch_sparse_generic(const SparseArgs& a, cudaStream_t s) {
 template <typename T>
 int launch_sparse(const SparseArgs& a, bool fast, cudaStream_t s) {
   if (!fast) return launch_sparse_generic<T>(a, s);
-  return a.d == 64 ? launch_sparse_t<T, 64, 4>(a, s) : launch_sparse_t<T, 128, 4>(a, s);
+  // rows are split over clusters of up to 8 CTAs while that leaves at most two per SM
+  const int64_t rows = int64_t(a.n_tokens) * a.n_kv;
+  const int sms = num_sms();
+  int cs = 1;
+  while (cs < 8 && rows * cs * 2 <= 2 * sms) cs *= 2;
+  if (a.d == 128) return launch_sparse_t<T, 128, 4, 3, 1, 2>(a, rows, cs, s);
+  // up to two CTAs per SM: 8 warps each; more: 4 warps and more CTAs resident
+  if (rows * cs <= 2 * sms) return launch_sparse_t<T, 64, 8, 2, 1, 2>(a, rows, cs, s);
+  return launch_sparse_t<T, 64, 4, 2, 1, 5>(a, rows, cs, s);
 }
 
 }  // namespace
@@ -699,9 +893,39 @@ int launch_sparse(const SparseArgs& a, bool fast, cudaStream_t s) {
 
 using namespace pkv;
 
+extern "C" int pkv_plan_sparse(const pkv_pool* pool, const pkv_batch* batch, const int32_t* batch_indices,
+                               int32_t max_pages, void* rows, void* stream) {
+  if (int rc = check_pool(pool)) return rc;
+  if (!batch) return fail(PKV_ERR_ARG, "batch descriptor is NULL");
+  if (batch->n_seqs <= 0) return fail(PKV_ERR_ARG, "batch has no sequences");
+  if (batch->n_tokens < 0 || batch->total_pages < 0 || batch->total_pages >= (int64_t(1) << 31))
+    return fail(PKV_ERR_ARG, "bad batch sizes");
+  if (max_pages <= 0) return fail(PKV_ERR_ARG, "max_pages must be positive");
+  if (batch->n_tokens == 0) return PKV_OK;
+  if (!rows || !batch_indices || !batch->cu_query_lens || !batch->kv_indptr || !batch->kv_last_page_len)
+    return fail(PKV_ERR_ARG, "rows, batch_indices and the batch CSR pointers must be non-NULL");
+  if (reinterpret_cast<uintptr_t>(rows) & 15) return fail(PKV_ERR_ARG, "rows must be 16-byte aligned");
+  RowArgs a;
+  a.cu_q = batch->cu_query_lens;
+  a.kv_lens = batch->kv_lens;
+  a.kv_indptr = batch->kv_indptr;
+  a.last_page_len = batch->kv_last_page_len;
+  a.batch_indices = batch_indices;
+  a.st = batch->dev_status;
+  a.rows = static_cast<Row*>(rows);
+  a.total_pages = batch->total_pages;
+  a.n_seqs = batch->n_seqs;
+  a.n_tokens = batch->n_tokens;
+  a.page = pool->block_size;
+  a.max_pages = max_pages;
+  sparse_plan_kernel<<<unsigned((batch->n_tokens + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  PKV_CUDA_RET(cudaGetLastError());
+  return PKV_OK;
+}
+
 extern "C" int pkv_attend_sparse(const pkv_pool* pool, const pkv_page_index* index, int32_t layer, int32_t n_heads,
                                  const void* q, void* out, int32_t* pages, float scale, int32_t budget, int32_t sink,
-                                 int32_t recent, const pkv_batch* batch, const int32_t* batch_indices,
+                                 int32_t recent, const pkv_batch* batch, const void* rows,
                                  int32_t max_pages, int32_t mode, void* stream) {
   if (int rc = check_pool(pool)) return rc;
   const pkv_pool& p = *pool;
@@ -726,11 +950,8 @@ extern "C" int pkv_attend_sparse(const pkv_pool* pool, const pkv_page_index* ind
   if (batch->n_tokens < 0 || batch->total_pages < 0 || batch->total_pages >= (int64_t(1) << 31))
     return fail(PKV_ERR_ARG, "bad batch sizes");
   if (batch->n_tokens == 0) return PKV_OK;
-  if (!q || !pages || !batch_indices || ((mode & PKV_SPARSE_ATTEND) && !out))
-    return fail(PKV_ERR_ARG, "q, out, pages and batch_indices must be non-NULL");
-  if (!batch->cu_query_lens || !batch->kv_indptr || !batch->kv_last_page_len ||
-      (batch->total_pages && !batch->kv_indices))
-    return fail(PKV_ERR_ARG, "batch CSR pointers must be non-NULL");
+  if (!q || !pages || !rows || !batch->kv_indices || ((mode & PKV_SPARSE_ATTEND) && !out))
+    return fail(PKV_ERR_ARG, "q, out, pages, rows and kv_indices must be non-NULL");
   if (max_pages <= 0) return fail(PKV_ERR_ARG, "max_pages must be positive");
   if (int64_t(batch->n_tokens) * p.n_kv_heads >= (int64_t(1) << 31))
     return fail(PKV_ERR_ARG, "too many tokens for one call");
@@ -747,16 +968,10 @@ extern "C" int pkv_attend_sparse(const pkv_pool* pool, const pkv_page_index* ind
   }
   a.k_slab = static_cast<const char*>(p.base) + int64_t(2) * layer * slab_bytes(p);
   a.v_slab = a.k_slab + slab_bytes(p);
-  a.cu_q = batch->cu_query_lens;
-  a.kv_lens = batch->kv_lens;
-  a.kv_indptr = batch->kv_indptr;
+  a.rows = static_cast<const Row*>(rows);
   a.kv_indices = batch->kv_indices;
-  a.last_page_len = batch->kv_last_page_len;
-  a.batch_indices = batch_indices;
   a.st = batch->dev_status;
   a.num_blocks = p.num_blocks;
-  a.total_pages = batch->total_pages;
-  a.n_seqs = batch->n_seqs;
   a.n_tokens = batch->n_tokens;
   a.n_heads = n_heads;
   a.n_kv = p.n_kv_heads;

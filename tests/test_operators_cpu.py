@@ -92,17 +92,25 @@ def batch(n=2, t=2, pages=4, cu=0x1000, ix=0x1000):
 
 def test_sparse_refusals(lib):
     def call(p=pool(), ix=index(), layer=0, hq=32, q=0x1000, out=0x1000, pages=0x1000, budget=8, sink=1, recent=1,
-             b=batch(), bi=0x1000, most=4, mode=3):
-        return lib.pkv_attend_sparse(p, ix, layer, hq, q, out, pages, 0.125, budget, sink, recent, b, bi, most, mode,
+             b=batch(), rows=0x1000, most=4, mode=3):
+        return lib.pkv_attend_sparse(p, ix, layer, hq, q, out, pages, 0.125, budget, sink, recent, b, rows, most, mode,
                                      None)
 
     for kw, rc in ((dict(layer=-1), 1), (dict(hq=30), 1), (dict(mode=0), 1), (dict(mode=4), 1), (dict(budget=0), 1),
                    (dict(sink=8), 1), (dict(recent=0), 1), (dict(ix=None), 1), (dict(b=None), 1),
-                   (dict(b=batch(n=0)), 1), (dict(b=batch(t=-1)), 1), (dict(b=batch(cu=None)), 1),
+                   (dict(b=batch(n=0)), 1), (dict(b=batch(t=-1)), 1),
                    (dict(b=batch(ix=None)), 1), (dict(q=None), 1), (dict(out=None), 1), (dict(pages=None), 1),
-                   (dict(bi=None), 1), (dict(most=0), 1), (dict(p=pool(dtype=3)), 2), (dict(p=pool(d=512)), 2)):
+                   (dict(rows=None), 1), (dict(most=0), 1), (dict(p=pool(dtype=3)), 2), (dict(p=pool(d=512)), 2)):
         assert call(**kw) == rc, kw
     assert call(b=batch(t=0)) == N.PKV_OK
+
+    def plan(p=pool(), b=batch(), bi=0x1000, most=4, rows=0x1000):
+        return lib.pkv_plan_sparse(p, b, bi, most, rows, None)
+
+    for kw in (dict(p=None), dict(b=None), dict(b=batch(n=0)), dict(b=batch(cu=None)), dict(bi=None), dict(most=0),
+               dict(rows=None), dict(rows=0x1008)):
+        assert plan(**kw) == N.PKV_ERR_ARG, kw
+    assert plan(b=batch(t=0)) == N.PKV_OK
 
 
 def test_shared_refusals(lib):
@@ -119,7 +127,7 @@ def test_shared_refusals(lib):
         assert plan(**kw) == rc, kw
 
     def attend(p=pool(), layer=0, q=0x1000, out=0x1000, b=batch(), ws=0x1000, n=size):
-        return lib.pkv_attend_shared_planned(p, layer, 32, q, out, 0.125, b, 1, ws, n, None)
+        return lib.pkv_attend_shared_planned(p, layer, 32, q, out, 0.125, b, ws, n, None)
 
     for kw, rc in ((dict(layer=2), 1), (dict(q=None), 1), (dict(q=0x1008), 1), (dict(out=None), 1), (dict(n=0), 1),
                    (dict(p=pool(d=128)), 2)):
