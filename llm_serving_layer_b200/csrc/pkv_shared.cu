@@ -43,15 +43,8 @@ constexpr int SH_MINB = 3;          // CTAs per SM
 constexpr int SH_NST = 2;           // slots of the K ring and of the V ring
 constexpr int SH_TMEM_COLS = 128;   // S in columns 0-63, O in 64-127
 constexpr int SH_PIECES = 16384;    // tile piece rows the workspace holds at most (x n_heads x 264 bytes)
-#ifndef SH_OVERHEAD
-#define SH_OVERHEAD 4
-#endif
-// SH_OVERHEAD: cost of an item besides its blocks, in blocks (set-up, piece written and read)
 constexpr int SH_WARPS = TC_THREADS / 32;
-#ifndef SH_SST_
-#define SH_SST_ 3
-#endif
-constexpr int SH_SST = SH_SST_;                         // ring stages of a streaming warp
+constexpr int SH_SST = 3;                         // ring stages of a streaming warp
 constexpr int SH_TILE = TC_P * TC_D * 2;          // one 16-token K or V tile of a head
 constexpr int SH_STAGE = 2 * SH_TILE;
 constexpr size_t SH_RING = size_t(SH_WARPS) * SH_SST * SH_STAGE;
@@ -215,7 +208,7 @@ __global__ void __launch_bounds__(128) shared_check_kernel(const PlanArgs a) {
 
 __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   __shared__ int warp_sum[32];
-  __shared__ int s_bad, s_maxblk, s_tot;
+  __shared__ int s_bad, s_maxblk, s_tot, s_listed;
   __shared__ unsigned long long s_best;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
@@ -234,13 +227,19 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   // fit the workspace, a second round (share = 0) computes every sequence by itself.
   int n_ents = 0, n_shared = 0, chunk = 1;
   for (int share = 1; share >= 0; --share) {
+    if (tid == 0) {
+      s_maxblk = 1;
+      s_listed = 0;
+    }
+    __syncthreads();
     for (int s = tid; s < a.n_seqs; s += blockDim.x) {
       const int g = group_of(a, s);
       const int f = a.group_indptr[g], e = a.group_indptr[g + 1];
       // a group of one sequence shares nothing
-      a.seq_np[s] = share && e - f >= 2 && !a.group_bad[g] ? a.prefix_pages[g] : 0;
+      const int np = share && e - f >= 2 && !a.group_bad[g] ? a.prefix_pages[g] : 0;
+      a.seq_np[s] = np;
+      if (a.cu_q[s + 1] - a.cu_q[s] == 1) atomicAdd(&s_listed, max(0, a.kv_indptr[s + 1] - a.kv_indptr[s] - np));
     }
-    if (tid == 0) s_maxblk = 1;
     __syncthreads();
     // ---- entities: the shared groups, then the several-token sequences
     n_ents = 0;
@@ -300,13 +299,18 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     }
     __threadfence_block();
     __syncthreads();
-    // ---- blocks per range: each thread weighs one length. A launch of items
-    // claimed by `slots` resident CTAs takes about the average load plus one
-    // item; ranges too short pay the items' overhead, too long the last item.
+    // ---- blocks per range: each thread weighs one length. The CTAs that start
+    // with tiles (all, or two thirds beside streaming ones) take an item after the
+    // other: rounds of a range's blocks and an item's set-up (two blocks' time);
+    // then the pieces, whose writing and reading is three blocks' work for a full
+    // tile, and the merge's rounds of eight. (256 sequences on a 4096-token prefix: ranges of 16 blocks, one
+    // round, 53 us; of 4 to 10 blocks 57 to 62 us.)
+    const int slots = int64_t(s_listed) * a.n_kv >= 8 * a.sms ? 2 * a.sms : SH_MINB * a.sms;
     const int maxblk = s_maxblk;
     const int step = (maxblk + int(blockDim.x) - 1) / int(blockDim.x);
     const int cand = min(maxblk, (tid + 1) * step);
-    float work = 0.f, n_it = 0.f;
+    float n_it = 0.f, rows = 0.f;
+    int most = 1;
     int64_t pieces = 0;
     bool fits = true;
     for (int i = 0; i < n_ents; ++i) {
@@ -314,12 +318,16 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
       const int nb = (x.pg1 - x.pg0 + TC_PPB - 1) / TC_PPB;
       const int sp = x.base < 0 ? 1 : (nb + cand - 1) / cand;
       fits &= sp <= a.splits_cap;
-      work += float(x.tiles) * nb;
       n_it += float(x.tiles) * sp;
-      if (x.base >= 0) pieces += int64_t(x.nt) * sp;
+      if (x.base >= 0) {
+        pieces += int64_t(x.nt) * sp;
+        rows += float(x.nt) * sp;
+        most = max(most, sp);
+      }
     }
     fits &= pieces <= a.pieces_cap;
-    const float est = (work + n_it * SH_OVERHEAD) * a.n_kv / (SH_MINB * a.sms) + cand + SH_OVERHEAD;
+    const float est = ceilf(n_it * a.n_kv / slots) * (cand + 2.f) + rows / a.tpt * a.n_kv * 3.f / a.sms +
+                      1.5f * ((most + 7) / 8);
     if (tid == 0) s_best = ~0ull;
     __syncthreads();
     if (fits && (tid == 0 || (tid + 1) * step < maxblk + step))
@@ -432,14 +440,12 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   // than there are: nothing is streamed
   const bool over = base_pg > a.total_pages;
   const int P = over ? 0 : base_pg;
-  // Streaming CTAs: all when there are no tiles, else one per SM, or two where
-  // the pages' time at the copy rate is the larger part (a page of one KV head:
-  // 4 KiB; a block of a tile: 820 cycles of its SM)
+  // CTAs that stream first: all when there are no tiles, else one per SM, or two
+  // where the pages' time at the copy rate is more than twice the tiles' (a page
+  // of one KV head: 4 KiB; a block of a tile: 820 cycles of its SM). 32 families
+  // of 8: two 53.4 us, one 63.6; the 4096-token prefix above: one 53, two 60.
   const float t_stream = float(P) * a.n_kv * 4096.f / 6.4e6f, t_tiles = float(blocks) * a.n_kv / a.sms * 0.43f;  // us
-  int n_stream = P == 0 ? 0 : n_items == 0 ? a.grid : min(a.grid, t_stream > 1.5f * t_tiles ? 2 * a.sms : a.sms);
-#ifdef SH_FORCE
-  if (P > 0 && n_items > 0) n_stream = SH_FORCE * a.sms;
-#endif
+  int n_stream = P == 0 ? 0 : n_items == 0 ? a.grid : t_stream > 2.f * t_tiles ? 2 * a.sms : a.sms;
   n_stream = min(n_stream, (P * a.n_kv + SH_WARPS - 1) / SH_WARPS);
   const int ranges = P == 0 ? 0 : max(1, min(P, n_stream * SH_WARPS / a.n_kv));
   __syncthreads();
@@ -494,7 +500,7 @@ struct ShArgs {
 // fp32 online softmax; keys past a page's tokens are neither read nor counted.
 template <typename T, int G>
 __device__ __forceinline__ void stream_range(const ShArgs& a, unsigned char* ring, int h, int r, int p0, int p1,
-                                             int lane) {
+                                             int2 cur, int2 nxt, int lane) {
   const int g = lane >> 2, c4 = lane & 3;
   const T* q = static_cast<const T*>(a.q);
   const int n = p1 - p0;
@@ -504,8 +510,6 @@ __device__ __forceinline__ void stream_range(const ShArgs& a, unsigned char* rin
   const int64_t lane_off = int64_t(r0) * row_b + int64_t(h) * TC_D * 2 + ch * 16;
   // descriptors: lane j holds pages wb + j (cur) and wb + 32 + j (nxt)
   int wb = 0;
-  int2 cur = lane < n ? __ldcg(a.desc + p0 + lane) : make_int2(-1, 0);
-  int2 nxt = 32 + lane < n ? __ldcg(a.desc + p0 + 32 + lane) : make_int2(-1, 0);
   auto desc_at = [&](int i) -> int2 {  // uniform i in [wb, wb + 64)
     const bool in_cur = i < wb + 32;
     return make_int2(__shfl_sync(0xffffffffu, in_cur ? cur.x : nxt.x, i & 31),
@@ -581,32 +585,40 @@ __device__ __forceinline__ void stream_range(const ShArgs& a, unsigned char* rin
       ldsm_x4(af[0], af[1], af[2], af[3], src + k_tok * 128 + ((chunk ^ (k_tok & 7)) << 4));
       MmaOp<T>::run(s, af, qb[ks][0], qb[ks][1]);
     }
-    const bool a0 = g < valid, a1 = g + 8 < valid;
-    s[0] = a0 ? s[0] * a.scale_log2 : -INFINITY;
-    s[1] = a0 ? s[1] * a.scale_log2 : -INFINITY;
-    s[2] = a1 ? s[2] * a.scale_log2 : -INFINITY;
-    s[3] = a1 ? s[3] * a.scale_log2 : -INFINITY;
-    float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
 #pragma unroll
-    for (int off = 4; off < 32; off <<= 1) {
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+    for (int e = 0; e < 4; ++e) s[e] *= a.scale_log2;
+    if (valid < TC_P) {
+      if (g >= valid) s[0] = s[1] = -INFINITY;
+      if (g + 8 >= valid) s[2] = s[3] = -INFINITY;
     }
-    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-    const float al0 = ex2(m0 - n0), al1 = ex2(m1 - n1);
-    m0 = n0;
-    m1 = n1;
-    const float p00 = ex2(s[0] - n0), p01 = ex2(s[1] - n1);
-    const float p10 = ex2(s[2] - n0), p11 = ex2(s[3] - n1);
-    l0 = l0 * al0 + (p00 + p10);
-    l1 = l1 * al1 + (p01 + p11);
+    float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+    if (__any_sync(0xffffffffu, x0 > m0 + TC_RESCALE || x1 > m1 + TC_RESCALE)) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+      }
+      const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+      const float al0 = ex2(m0 - n0), al1 = ex2(m1 - n1);
+      m0 = n0;
+      m1 = n1;
+      l0 *= al0;
+      l1 *= al1;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        o[mt][0] *= al0;
+        o[mt][2] *= al0;
+        o[mt][1] *= al1;
+        o[mt][3] *= al1;
+      }
+    }
+    const float p00 = ex2(s[0] - m0), p01 = ex2(s[1] - m1);
+    const float p10 = ex2(s[2] - m0), p11 = ex2(s[3] - m1);
+    l0 += p00 + p10;
+    l1 += p01 + p11;
     const uint32_t pb0 = movmatrix_t(MmaOp<T>::pack(p00, p01)), pb1 = movmatrix_t(MmaOp<T>::pack(p10, p11));
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
-      o[mt][0] *= al0;
-      o[mt][2] *= al0;
-      o[mt][1] *= al1;
-      o[mt][3] *= al1;
       uint32_t af[4];
       const int chunk = 2 * mt + v_chk;
       ldsm_x4_t(af[0], af[1], af[2], af[3], src + SH_TILE + v_tok * 128 + ((chunk ^ (v_tok & 7)) << 4));
@@ -668,8 +680,29 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
     const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap qmap, const ShArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ int s_first;
+  __shared__ uint32_t s_tmem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
+  // ---- tensor memory: 128 columns S | O, freed on every path below. Allocated
+  // first thing by every CTA, streaming ones too: the next CTA of the launch
+  // starts on an SM only once the one before has given up its allocation permit
+  // (measured: a CTA that kept it held the SM at two CTAs until it ended).
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                 "r"(SH_TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    pdl_trigger();  // after the allocation: the next kernel's may follow
+  }
+  // frees the tensor memory; all threads, after every role is done with it
+  auto leave = [&]() {
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(SH_TMEM_COLS) : "memory");
+    }
+    if (threadIdx.x == 0) tl_count_exit(a.claim);
+  };
   // the plan completed before this kernel could start and fenced its stores
   const int n_items = __ldcg(&a.ctl->n_items) * a.n_kv;
   const int n_stream = __ldcg(&a.ctl->n_stream);
@@ -677,24 +710,30 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
   const bool streams = int(blockIdx.x) >= n_tile;
   if (!streams && int(blockIdx.x) >= n_items) {  // nothing for this CTA (uniform over the CTA)
     pdl_wait();                                  // the counters belong to the previous launch until it completed
-    if (threadIdx.x == 0) tl_count_exit(a.claim);
+    leave();
     return;
   }
   if (streams) {
     const int ranges = __ldcg(&a.ctl->n_ranges), P = __ldcg(&a.ctl->listed);
-    pdl_wait();  // q and this layer's appended K/V rows are written by earlier kernels
     const int w = (int(blockIdx.x) - n_tile) * SH_WARPS + warp;
+    bool waited = false;
     for (int u = w; u < ranges * a.n_kv; u += n_stream * SH_WARPS) {
       const int h = u % a.n_kv, r = u / a.n_kv;
       const int p0 = int(int64_t(r) * P / ranges), p1 = int(int64_t(r + 1) * P / ranges);
-      if (p0 < p1) stream_range<T, G>(a, smem_raw + size_t(warp) * SH_SST * SH_STAGE, h, r, p0, p1, lane);
+      // the range's first page descriptors (the plan's: read ahead of the wait)
+      const int2 cur = lane < p1 - p0 ? __ldcg(a.desc + p0 + lane) : make_int2(-1, 0);
+      const int2 nxt = 32 + lane < p1 - p0 ? __ldcg(a.desc + p0 + 32 + lane) : make_int2(-1, 0);
+      if (!waited) pdl_wait();  // q and this layer's appended K/V rows are written by earlier kernels
+      waited = true;
+      stream_range<T, G>(a, smem_raw + size_t(warp) * SH_SST * SH_STAGE, h, r, p0, p1, cur, nxt, lane);
     }
+    if (!waited) pdl_wait();
     // the ring's generic-proxy accesses before the tiles' TMA writes
     fence_proxy_async_smem();
     if (threadIdx.x == 0) s_first = n_items > 0 ? n_tile + atomicAdd(a.claim, 1) : 0;
     __syncthreads();
     if (s_first >= n_items) {
-      if (threadIdx.x == 0) tl_count_exit(a.claim);
+      leave();
       return;
     }
   } else if (threadIdx.x == 0) {
@@ -720,7 +759,6 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
   uint64_t* item_full = o_free + 1;
   uint64_t* item_empty = item_full + 2;
   uint64_t* drain = item_empty + 2;
-  __shared__ uint32_t s_tmem;
   __shared__ ShItem s_item[2];
 
   if (threadIdx.x == 0) {
@@ -746,19 +784,11 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
     mbar_init(drain, 1);
     fence_mbar_init();
   }
-  // ---- tensor memory: 128 columns S | O, freed on every path below
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
-                 "r"(SH_TMEM_COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = s_tmem;
   const uint32_t tO = tbase + TC_KB;
-  pdl_wait();  // q and this layer's appended K/V rows are written by earlier kernels
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -782,6 +812,10 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
         pg_bad |= id < 0 || id >= a.num_blocks;
       }
       pg_bad = __any_sync(0xffffffffu, pg_bad);
+      // q, this layer's appended K/V rows and the pieces' last readers: the first
+      // item is the plan's and was read ahead of the wait; the other warps follow
+      // this one's copies
+      if (it == 0) pdl_wait();
       const int sl = it & 1;
       if (it >= 2 && !mbar_wait_bounded_sleepy(&item_empty[sl], ((it - 2) >> 1) & 1, a.st, 32)) dead = true;
       dead = __any_sync(0xffffffffu, dead);
@@ -1072,15 +1106,7 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
     }
   }
 
-  // ---- free tensor memory once every role is done with it
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(SH_TMEM_COLS)
-                 : "memory");
-  }
-  if (threadIdx.x == 0) tl_count_exit(a.claim);
+  leave();
 }
 
 // the tile role's buffers (1 KiB to align them), or the streaming warps' rings
@@ -1088,7 +1114,7 @@ size_t sh_smem() { return std::max(1024 + 2 * size_t(TC_QTILE) + size_t(2 * SH_N
 
 // ---------------------------------------------------------------- merge
 // One warp per (token, query head): its pieces over the shared keys and over its
-// own -> out. Two dims a lane, four pieces' loads in flight.
+// own -> out. Two dims a lane, eight pieces' loads in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) shared_merge_kernel(const int4* fold, const int4* rest, const float* part_o,
                                                            const float2* part_ml, void* out, int n_tokens,
@@ -1106,7 +1132,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const int4* fold, con
   pdl_wait();
   if (b.y <= 0) return;  // written straight to out, or its tables are inconsistent
   const int n = f.y + b.y;
-  constexpr int U = 4;
+  constexpr int U = 8;
   float M = -1e30f, L = 0.f, y0 = 0.f, y1 = 0.f;
   for (int i0 = 0; i0 < n; i0 += U) {
     float2 ml[U], v[U];
