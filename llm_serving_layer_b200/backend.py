@@ -347,20 +347,26 @@ class B200PagedBackend:
                              "tokens were supplied")
         if index is not None and index.backend is not self:
             raise ValueError("index belongs to another backend")
-        k, k_stride = self._rows(k, Hk * D)
-        v, v_stride = self._rows(v, Hk * D)
+        dt, row = self.dtype, Hk * D
+        ks, vs = k.stride(), v.stride()
+        if not (k.dtype is v.dtype is dt and k.get_device() == v.get_device() == dev and ks[1] == vs[1] == D
+                and ks[2] == vs[2] == 1 and ks[0] >= row and vs[0] >= row):
+            (k, ks), (v, vs) = self._rows(k, row), self._rows(v, row)
         q_ptr = qo_ptr = None
         q_stride = heads = 0
         if q is not None:
             heads = self.n_heads
             if q.shape != (tokens, heads, D):
                 raise ValueError(f"q has shape {tuple(q.shape)}, expected ({tokens}, {heads}, {D})")
-            q, q_stride = self._rows(q, heads * D)
+            qs = q.stride()
+            if not (q.dtype is dt and q.get_device() == dev and qs[1] == D and qs[2] == 1 and qs[0] >= heads * D):
+                q, qs = self._rows(q, heads * D)
+            q_stride = qs[0]
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            elif (q_out.shape != q.shape or q_out.dtype != self.dtype or q_out.get_device() != dev
+            elif (q_out.shape != q.shape or q_out.dtype != dt or q_out.get_device() != dev
                   or not q_out.is_contiguous()):
-                raise ValueError(f"q_out must be a contiguous {tuple(q.shape)} {self.dtype} tensor on {self.device}")
+                raise ValueError(f"q_out must be a contiguous {tuple(q.shape)} {dt} tensor on {self.device}")
             elif _overlap(q_out, q) and not (q_out.data_ptr() == q.data_ptr() and q.is_contiguous()):
                 raise ValueError("q_out overlaps q without being q")
             q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
@@ -368,9 +374,11 @@ class B200PagedBackend:
             raise ValueError("q_out given without q")
         if not tokens:
             return q_out
-        slots, pos = self._dev_vec(slots, torch.int32), self._dev_vec(pos, torch.int64)
+        if not (slots.dtype is torch.int32 and pos.dtype is torch.int64
+                and slots.get_device() == pos.get_device() == dev and slots.is_contiguous() and pos.is_contiguous()):
+            slots, pos = self._i32(slots), self._own(pos, torch.int64)
         rc = self._lib.pkv_rope_append(
-            self._pdesc, layer_idx, q_ptr, q_stride, qo_ptr, heads, k.data_ptr(), k_stride, v.data_ptr(), v_stride,
+            self._pdesc, layer_idx, q_ptr, q_stride, qo_ptr, heads, k.data_ptr(), ks[0], v.data_ptr(), vs[0],
             slots.data_ptr(), pos.data_ptr(), tokens, cos.data_ptr(), sin.data_ptr(), rows, 2 * half, interleaved,
             None if index is None else index._pdesc, self._status_ptr, N.raw_stream(self._dev_index))
         if rc:
@@ -385,20 +393,15 @@ class B200PagedBackend:
         raise ValueError(f"rope cos and sin must be contiguous float32 [max_pos, rotary_dim // 2] tensors of one shape "
                          f"on {self.device}")
 
-    def _rows(self, t: torch.Tensor, row: int) -> tuple[torch.Tensor, int]:
+    def _rows(self, t: torch.Tensor, row: int) -> tuple[torch.Tensor, tuple[int, ...]]:
         """t ``(T, heads, head_dim)`` on this device in the pool dtype with each
         token's ``row`` elements contiguous (no copy for slices of a fused
-        projection), and the elements from token to token."""
+        projection), and its strides."""
         st = t.stride()
         if t.dtype is self.dtype and t.get_device() == self._dev_index and st[2] == 1 and st[0] >= row \
                 and (st[1] == self.head_dim or row == self.head_dim):
-            return t, st[0]
-        return t.to(device=self.device, dtype=self.dtype).contiguous(), row
-
-    def _dev_vec(self, t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-        if t.dtype is dtype and t.get_device() == self._dev_index and t.is_contiguous():
-            return t
-        return t.to(device=self.device, dtype=dtype).contiguous()
+            return t, st
+        return t.to(device=self.device, dtype=self.dtype).contiguous(), (row,)
 
     def _rope_args(self, rope, meta):
         try:

@@ -59,14 +59,108 @@ __device__ __forceinline__ uint4 pack_vec(const float (&f)[16 / sizeof(T)]) {
     return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t min_word(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4) {
+    return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 m = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __nv_bfloat162 m =
+        __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __nv_bfloat162 m =
+        __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 min_words(const uint4& a, const uint4& b) {
+  return make_uint4(min_word<T>(a.x, b.x), min_word<T>(a.y, b.y), min_word<T>(a.z, b.z), min_word<T>(a.w, b.w));
+}
+template <typename T>
+__device__ __forceinline__ uint4 max_words(const uint4& a, const uint4& b) {
+  return make_uint4(max_word<T>(a.x, b.x), max_word<T>(a.y, b.y), max_word<T>(a.z, b.z), max_word<T>(a.w, b.w));
+}
+__device__ __forceinline__ uint4 shfl_xor4(const uint4& a, int off) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, a.x, off), __shfl_xor_sync(0xffffffffu, a.y, off),
+                    __shfl_xor_sync(0xffffffffu, a.z, off), __shfl_xor_sync(0xffffffffu, a.w, off));
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int w) {
+  return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w;
+}
+// largest magnitude of a word of bounds
+template <typename T>
+__device__ __forceinline__ float top_of_word(uint32_t lo, uint32_t hi) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fabsf(__uint_as_float(lo)), fabsf(__uint_as_float(hi)));
+  } else {
+    const float2 a = unpack2<T>(lo), b = unpack2<T>(hi);
+    return fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y)));
+  }
+}
+__device__ __forceinline__ int8_t code_of(float x, float scale, bool up) {
+  const float y = scale > 0.f ? (up ? ceilf(__fdiv_rn(x, scale)) : floorf(__fdiv_rn(x, scale))) : 0.f;
+  return int8_t(fminf(fmaxf(y, -127.f), 127.f));
+}
+// Codes of a word of bounds: floor(lo / scale) at c, ceil(hi / scale) at c + d,
+// clamped; 0 where the scale is 0.
+template <typename T>
+__device__ __forceinline__ void store_codes(int8_t* c, int d, uint32_t lo, uint32_t hi, float scale) {
+  if constexpr (sizeof(T) == 4) {
+    c[0] = code_of(__uint_as_float(lo), scale, false);
+    c[d] = code_of(__uint_as_float(hi), scale, true);
+  } else {
+    const float2 a = unpack2<T>(lo), b = unpack2<T>(hi);
+    *reinterpret_cast<char2*>(c) = make_char2(code_of(a.x, scale, false), code_of(a.y, scale, false));
+    *reinterpret_cast<char2*>(c + d) = make_char2(code_of(b.x, scale, true), code_of(b.y, scale, true));
+  }
+}
+
+template <typename T, int VE, bool INTER>
+__device__ __forceinline__ void turn_pair(float (&p)[VE], float (&r)[VE], const float (&c)[VE], const float (&s)[VE]) {
+  if constexpr (INTER) {
+#pragma unroll
+    for (int e = 0; e < VE; e += 2) {
+      rope_pair(p[e], p[e + 1], c[e / 2], s[e / 2]);
+      rope_pair(r[e], r[e + 1], c[VE / 2 + e / 2], s[VE / 2 + e / 2]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) rope_pair(p[e], r[e], c[e], s[e]);
+  }
+}
+template <int VE>
+__device__ __forceinline__ void load_angles(const float* p, float (&f)[VE]) {
+#pragma unroll
+  for (int e = 0; e < VE; e += 4) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p + e));
+    f[e] = v.x; f[e + 1] = v.y; f[e + 2] = v.z; f[e + 3] = v.w;
+  }
+}
+
 // One token's work, shared by wpt warps. VECTOR: 16-byte vectors of VE
 // elements; a lane owns one column of VE pairs (its cosines and sines stay in
 // registers) and steps over the heads, UB of them loaded before the first is
-// stored, so that a token's rows travel together. Otherwise single elements.
+// stored, so that a token's rows travel together (16384 tokens of 32 + 8 + 8
+// heads of 64: UB 5 36 us, 4 39.5, 2 43; at two CTAs per SM). Otherwise single
+// elements.
 template <typename T, bool VECTOR, bool INTER>
-__global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a) {
+__global__ void __launch_bounds__(256, 2) rope_append_kernel(const RopeAppendArgs a) {
   constexpr int VE = VECTOR ? 16 / int(sizeof(T)) : 1;
-  constexpr int UB = 4;
+  constexpr int UB = 5;
   using V = typename std::conditional<VECTOR, uint4, T>::type;
   pdl_trigger();
   pdl_wait();  // q, k, v, positions and slots may come from the kernels just before
@@ -108,12 +202,9 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a
     const int e0 = INTER ? 2 * i : i, e1 = INTER ? 2 * i + VE : half + i;
     const int h0 = i < cols * VE ? u0 / a.cols : heads;
     float c[VE], s[VE];
-#pragma unroll
-    for (int e = 0; e < VE; e += 4) {
-      const float4 cv = h0 < heads ? __ldg(reinterpret_cast<const float4*>(cs + i + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 sv = h0 < heads ? __ldg(reinterpret_cast<const float4*>(sn + i + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      c[e] = cv.x; c[e + 1] = cv.y; c[e + 2] = cv.z; c[e + 3] = cv.w;
-      s[e] = sv.x; s[e + 1] = sv.y; s[e + 2] = sv.z; s[e + 3] = sv.w;
+    if (h0 < heads) {
+      load_angles<VE>(cs + i, c);
+      load_angles<VE>(sn + i, s);
     }
     for (int hb = h0; hb < heads; hb += UB * step) {
       uint4 xa[UB], xb[UB];
@@ -130,18 +221,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a
         float p[VE], r[VE];
         unpack_vec<T>(xa[b], p);
         unpack_vec<T>(xb[b], r);
-        if (turn) {
-          if constexpr (INTER) {
-#pragma unroll
-            for (int e = 0; e < VE; e += 2) {
-              rope_pair(p[e], p[e + 1], c[e / 2], s[e / 2]);
-              rope_pair(r[e], r[e + 1], c[VE / 2 + e / 2], s[VE / 2 + e / 2]);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) rope_pair(p[e], r[e], c[e], s[e]);
-          }
-        }
+        if (turn) turn_pair<T, VE, INTER>(p, r, c, s);
         if (T* y = dst(hb + b * step)) {
           *reinterpret_cast<uint4*>(y + e0) = pack_vec<T>(p);
           *reinterpret_cast<uint4*>(y + e1) = pack_vec<T>(r);
@@ -227,69 +307,60 @@ __device__ __forceinline__ void index_entry(const IndexArgs& a, int layer, int64
   for (int i = 0; i < IX_MAX_EPL; ++i) {
     const int e = lane + 32 * i;
     if (e < d) {
-      // scale 0 (or not a number): the codes are 0
-      const float x = scale > 0.f ? floorf(__fdiv_rn(lo[i], scale)) : 0.f;
-      const float y = scale > 0.f ? ceilf(__fdiv_rn(hi[i], scale)) : 0.f;
-      c[e] = int8_t(fminf(fmaxf(x, -127.f), 127.f));
-      c[d + e] = int8_t(fminf(fmaxf(y, -127.f), 127.f));
+      c[e] = code_of(lo[i], scale, false);
+      c[d + e] = code_of(hi[i], scale, true);
     }
   }
   if (lane == 0) a.scales[entry] = scale;
 }
 
 // The same for heads of LPR 16-byte vectors (8, 16 or 32): LPR lanes on a key,
-// 32 / LPR keys at a time, up to 8 loads in flight; a lane keeps VE dims.
+// 32 / LPR keys at a time, four loads in flight; a lane keeps VE dims.
 template <typename T, int LPR>
 __device__ __forceinline__ void index_entry_vec(const IndexArgs& a, int layer, int64_t blk, int h, int lane) {
   constexpr int VE = 16 / int(sizeof(T)), D = LPR * VE, RPI = 32 / LPR;
   const T* k = reinterpret_cast<const T*>(a.k_base + int64_t(2) * layer * a.slab_bytes) +
                (blk * a.page * a.hkv + h) * D + (lane % LPR) * VE;
   const int64_t row = int64_t(a.hkv) * D;
-  float lo[VE], hi[VE];
+  // bounds as packed words: two 16-bit or one 32-bit value each
+  uint4 mn{}, mx{};
+  bool any = false;
+  for (int r0 = lane / LPR; r0 < a.page; r0 += 4 * RPI) {
+    uint4 x[4];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    lo[e] = INFINITY;
-    hi[e] = -INFINITY;
-  }
-#pragma unroll 8
-  for (int r = lane / LPR; r < a.page; r += RPI) {
-    float x[VE];
-    unpack_vec<T>(*reinterpret_cast<const uint4*>(k + r * row), x);
+    for (int b = 0; b < 4; ++b)
+      if (r0 + b * RPI < a.page) x[b] = *reinterpret_cast<const uint4*>(k + (r0 + b * RPI) * row);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      lo[e] = fminf(lo[e], x[e]);
-      hi[e] = fmaxf(hi[e], x[e]);
+    for (int b = 0; b < 4; ++b) {
+      if (r0 + b * RPI >= a.page) continue;
+      mn = any ? min_words<T>(mn, x[b]) : x[b];
+      mx = any ? max_words<T>(mx, x[b]) : x[b];
+      any = true;
     }
   }
+  // lanes without a key (fewer keys than lanes take) offer their neighbours nothing
+#pragma unroll
+  for (int off = LPR; off < 32; off <<= 1) {
+    const uint4 on = shfl_xor4(mn, off), ox = shfl_xor4(mx, off);
+    const bool there = __shfl_xor_sync(0xffffffffu, int(any), off) != 0;
+    mn = !there ? mn : any ? min_words<T>(mn, on) : on;
+    mx = !there ? mx : any ? max_words<T>(mx, ox) : ox;
+    any |= there;
+  }
+  // every lane of a column holds its bounds now: the RPI lanes share the vector's words
   float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-#pragma unroll
-    for (int off = LPR; off < 32; off <<= 1) {
-      lo[e] = fminf(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], off));
-      hi[e] = fmaxf(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], off));
-    }
-    top = fmaxf(top, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-  }
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, top_of_word<T>(word_of(mn, w), word_of(mx, w)));
 #pragma unroll
   for (int off = 1; off < LPR; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   const float scale = __fmul_rn(top, 1.0f / 127.0f);
   const int64_t entry = (int64_t(layer) * a.num_blocks + blk) * a.hkv + h;
-  if (lane < LPR) {
-    int8_t c[2][VE];
+  int8_t* out = a.codes + entry * 2 * D + (lane % LPR) * VE;
+  constexpr int WPL = 4 / RPI;  // words a lane encodes
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      const float x = scale > 0.f ? floorf(__fdiv_rn(lo[e], scale)) : 0.f;
-      const float y = scale > 0.f ? ceilf(__fdiv_rn(hi[e], scale)) : 0.f;
-      c[0][e] = int8_t(fminf(fmaxf(x, -127.f), 127.f));
-      c[1][e] = int8_t(fminf(fmaxf(y, -127.f), 127.f));
-    }
-    int8_t* out = a.codes + entry * 2 * D + lane * VE;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int w = 0; w < VE / 4; ++w)
-        reinterpret_cast<char4*>(out + b * D)[w] = make_char4(c[b][4 * w], c[b][4 * w + 1], c[b][4 * w + 2], c[b][4 * w + 3]);
+  for (int u = 0; u < WPL; ++u) {
+    const int w = lane / LPR * WPL + u;
+    store_codes<T>(out + w * (VE / 4), D, word_of(mn, w), word_of(mx, w), scale);
   }
   if (lane == 0) a.scales[entry] = scale;
 }
@@ -476,8 +547,9 @@ extern "C" int pkv_rope_append(const pkv_pool* pool, int32_t layer, const void* 
   a.cols = 1;
   while (a.cols < a.half / ve) a.cols *= 2;
   const bool vec = (al & 15) == 0 && a.half % ve == 0 && a.cols <= 32;
-  // one warp per token once that fills the SMs' warp slots, else up to 8
-  const int64_t want = int64_t(num_sms()) * 32;
+  // one warp per token from eight tokens per SM on, else up to 8 (512 tokens of
+  // 48 heads of 64: four warps 4.2 us, eight 6.5; 1700: one 8.4, four 10.3)
+  const int64_t want = int64_t(num_sms()) * 8;
   a.wpt = n_tokens >= want ? 1 : (2 * n_tokens >= want ? 2 : (4 * n_tokens >= want ? 4 : 8));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool inter = interleaved != 0;
