@@ -106,11 +106,30 @@ class RandomLlama:
         a, b = t[..., :half].float(), t[..., half:].float()
         return torch.cat([a * cos - b * sin, a * sin + b * cos], dim=-1).to(self.dtype)
 
+    def _after_attention(self, x: torch.Tensor, o: torch.Tensor, layer: int) -> torch.Tensor:
+        """The layer's output projection and FFN, each added to the residual."""
+        x = x + F.linear(o, self.w_o[layer])
+        gu = F.linear(self._norm(x, self.ln_ffn[layer]), self.w_gate_up[layer])
+        return x + F.linear(F.silu(gu[:, : self.cfg.ffn]) * gu[:, self.cfg.ffn:], self.w_down[layer])
+
     @torch.no_grad()
-    def forward_varlen(self, tokens: torch.Tensor, meta: Any, backend: Any) -> torch.Tensor:
+    def forward_varlen(self, tokens: torch.Tensor, meta: Any, backend: Any, *, shared: Any = None,
+                       sparse: Any = None, index: Any = None) -> torch.Tensor:
         """tokens: (T,) int token ids of every sequence's new tokens packed in
         sequence order; returns (n_seqs, vocab) logits (fp32) of each
-        sequence's last token."""
+        sequence's last token.
+
+        ``shared`` (``backend.plan_shared(meta, ...)``): attention reads the
+        pages that families of the batch share once. ``sparse``
+        (``backend.plan_sparse(meta, index, budget)``): each query attends over
+        the pages the index selects for it. At most one of them. With either, or
+        with ``index`` (a ``PageIndex`` to keep up to date, the sparse plan's by
+        default), q, k and v go to ``backend.rope_append`` as slices of the
+        projection."""
+        if shared is not None and sparse is not None:
+            raise ValueError("a step has a shared plan or a sparse plan, not both")
+        index = sparse.index if index is None and sparse is not None else index
+        planned = shared is not None or sparse is not None or index is not None
         cfg = self.cfg
         T = tokens.shape[0]
         Hq, Hkv, Dh = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
@@ -123,6 +142,17 @@ class RandomLlama:
         for layer in range(cfg.n_layers):
             h = self._norm(x, self.ln_attn[layer])
             qkv = F.linear(h, self.w_qkv[layer])
+            if planned:
+                q, k, v = (t.unflatten(1, (-1, Dh)) for t in qkv.split([Hq * Dh, Hkv * Dh, Hkv * Dh], 1))
+                q = backend.rope_append(layer, q, k, v, meta, (self.rope_cos, self.rope_sin), index=index)
+                if shared is not None:
+                    o = backend.attend_shared(q, layer, self.scale, shared)
+                elif sparse is not None:
+                    o, _ = backend.attend_sparse(q, layer, self.scale, sparse)
+                else:
+                    o = backend.attend(q, layer, self.scale, meta)
+                x = self._after_attention(x, o.reshape(T, Hq * Dh), layer)
+                continue
             v = qkv[:, (Hq + Hkv) * Dh:].reshape(T, Hkv, Dh)
             if fused:  # RoPE, KV-append and attention in the backend (one launch for a decode step)
                 q = qkv[:, : Hq * Dh].reshape(T, Hq, Dh)
@@ -136,10 +166,7 @@ class RandomLlama:
                 else:
                     backend.append_kv(layer, k, v, meta)
                     o = backend.attend(q, layer, self.scale, meta)
-            x = x + F.linear(o.reshape(T, Hq * Dh), self.w_o[layer])
-            h = self._norm(x, self.ln_ffn[layer])
-            gu = F.linear(h, self.w_gate_up[layer])
-            x = x + F.linear(F.silu(gu[:, : cfg.ffn]) * gu[:, cfg.ffn:], self.w_down[layer])
+            x = self._after_attention(x, o.reshape(T, Hq * Dh), layer)
         last = self._norm(x[meta.last_token_ix.to(self.device).long()], self.ln_final)
         if self.head32 is not None:
             return F.linear(last.float(), self.head32)
