@@ -730,7 +730,7 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
     if (!waited) pdl_wait();
     // the ring's generic-proxy accesses before the tiles' TMA writes
     fence_proxy_async_smem();
-    if (threadIdx.x == 0) s_first = n_items > 0 ? n_tile + atomicAdd(a.claim, 1) : 0;
+    if (threadIdx.x == 0) s_first = n_tile < n_items ? n_tile + atomicAdd(a.claim, 1) : n_items;
     __syncthreads();
     if (s_first >= n_items) {
       leave();
@@ -866,7 +866,8 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
       }
       dead = __shfl_sync(0xffffffffu, dead, 0);
       ++it;
-      if (lane == 0) w = n_tile + atomicAdd(a.claim, 1);
+      // no claim where the CTAs' own numbers cover the items: atomics on one address take turns
+      if (lane == 0) w = n_tile < n_items ? n_tile + atomicAdd(a.claim, 1) : n_items;
       w = __shfl_sync(0xffffffffu, w, 0);
     }
     if (dead && lane == 0) {

@@ -324,7 +324,9 @@ __global__ void __launch_bounds__(NW * 32, MINB) sparse_kernel(const SparseArgs 
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qb[ks][0] = qb[ks][1] = 0u;
   }
-  const struct { int64_t pa; int pos, mine; bool ok; } row{row4.x, row4.y, row4.y / a.page, row4.z != 0};
+  // (a plan made for longer lists than this call allows shared memory for is not followed)
+  const struct { int64_t pa; int pos, mine; bool ok; } row{row4.x, row4.y, row4.y / a.page,
+                                                           row4.z != 0 && row4.y / a.page < a.max_pages};
   T* out = static_cast<T*>(a.out) + q0;
   int32_t* prow = a.pages + (int64_t(t) * a.n_kv + h) * a.budget;
   if (!row.ok) {  // uniform over the cluster
@@ -684,7 +686,9 @@ __global__ void __launch_bounds__(256) sparse_generic_kernel(const SparseArgs a)
   pdl_trigger();
   pdl_wait();
   const int4 row4 = __ldg(reinterpret_cast<const int4*>(a.rows + t));
-  const struct { int64_t pa; int pos, mine; bool ok; } row{row4.x, row4.y, row4.y / a.page, row4.z != 0};
+  // (a plan made for longer lists than this call allows shared memory for is not followed)
+  const struct { int64_t pa; int pos, mine; bool ok; } row{row4.x, row4.y, row4.y / a.page,
+                                                           row4.z != 0 && row4.y / a.page < a.max_pages};
   const int64_t q0 = (int64_t(t) * a.n_heads + int64_t(h) * G) * D;
   const T* q = static_cast<const T*>(a.q) + q0;
   T* out = static_cast<T*>(a.out) + q0;

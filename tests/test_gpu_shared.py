@@ -104,6 +104,37 @@ def test_matches_unshared_attention(case, hq, hkv, dtype):
     assert torch.equal(again, out)
 
 
+def test_more_rows_than_the_workspace_holds_pieces_for():
+    """17000 sequences over one shared page: computed without sharing, same result."""
+    n = 17000
+    bk = B200PagedBackend(1, n + 1, 16, 1, 1, 64, device=DEV, validate="device")
+    g = torch.Generator(device=DEV).manual_seed(5)
+    for pool in (bk.k_pool[0], bk.v_pool[0]):
+        pool.copy_(torch.randn(pool.shape, generator=g, device=DEV))
+    tails = [1 + i % 16 for i in range(n)]
+    meta = build_meta([[0, i + 1] for i in range(n)], [16 + t for t in tails], [1] * n, 16, device=DEV)
+    q = torch.randn(n, 1, 64, generator=g, device=DEV).half()
+    out = bk.attend_shared(q, 0, 0.125, bk.plan_shared(meta, SharedPrefix([n], [1])))
+    bk.check_status()
+    k = torch.cat([bk.k_pool[0][0, :, 0].expand(n, 16, 64), bk.k_pool[0][1:, :, 0]], 1).double()
+    v = torch.cat([bk.v_pool[0][0, :, 0].expand(n, 16, 64), bk.v_pool[0][1:, :, 0]], 1).double()
+    w = torch.einsum("nd,nkd->nk", q[:, 0].double(), k) * 0.125
+    w = w.masked_fill(torch.arange(32, device=DEV) >= 16 + torch.tensor(tails, device=DEV)[:, None], -float("inf"))
+    close(out[:, 0], torch.einsum("nk,nkd->nd", torch.softmax(w, -1), v), bk)
+
+
+def test_many_sequences_in_families():
+    """More sequences and families than the plan has threads, mixed with chunks."""
+    fam = [(1 + i % 3, [(1 + (7 * i + j) % 40, 1) for j in range(1 + i % 4)]) for i in range(1100)]
+    fam[5] = (2, [(30, 30), (9, 1)])
+    bk, meta, q, shared, tables = build(fam, hq=4, hkv=2, validate="device")
+    out = bk.attend_shared(q, 0, 0.125, bk.plan_shared(meta, shared))
+    bk.check_status()
+    want = bk.attend(q, 0, 0.125, meta)  # the plain path, itself held to the oracle elsewhere
+    top = float(torch.nan_to_num(bk.v_pool[0].float()).abs().max())
+    assert float((out.double() - want.double()).abs().max()) <= (4 * UNIT[bk.dtype] + 2.0 ** -17) * top
+
+
 def test_layers_workspaces_and_streams():
     fam = CASES["chunks and decode rows"]
     bk, meta, q, shared, tables = build(fam, layers=3, validate="device")
