@@ -13,11 +13,19 @@
 // negative and positive parts, I_g is one int8 dot product of 2 D entries,
 // which the int8 tensor-core instruction takes 16 pages x 8 heads at a time.
 //
-// One CTA per (query, KV head) does all of it: scores into shared memory, a
-// radix selection over their order-preserving 32-bit keys, the listed pages
-// ascending, then attention (S^T = K q^T and O^T += V^T P^T on 16-token tiles,
-// fp32 online softmax) with the pages spread over its warps and merged at the
-// end.
+// One row (query, KV head) is one CTA's, or a cluster's where rows are few:
+// scores into shared memory, a selection over their order-preserving 32-bit keys,
+// the listed pages ascending, then attention (S^T = K q^T and O^T += V^T P^T on
+// 16-token tiles, fp32 online softmax) with the pages spread over its warps and
+// merged at the end. One launch, nothing passes through global memory but the list.
+//
+// Bound by HBM once rows are many: 256 sequences of 1.4 to 4.1 k tokens, 64 pages
+// each (2048 rows, fp16, 8 KV heads of 64): 537 MB of keys and values, 47 MB of
+// index; the attention alone 90 us = 6.0 TB/s (0.92 of the copy rate), with the
+// selection 105 us. Each row's chain (plan row, page ids, index entries,
+// selection, page reads: about 11000 cycles before the first page is asked for)
+// is hidden by the other CTAs of the SM there, and is the time itself where rows
+// are few: 2048 pages of one sequence 12.7 us, of which the chain is two thirds.
 #include <algorithm>
 #include <mutex>
 #include <string>
@@ -145,19 +153,38 @@ __device__ __forceinline__ int end_scored(const SparseArgs& a, int n) { return m
 // threshold's bin is listed whole or holds one value: one barrier a pass, since
 // every warp scans the bins itself. Then each warp counts and writes a
 // contiguous share of the pages. All threads call it.
-template <typename Put>
+// KPT > 0: n <= 32 KPT keys per warp, which every lane reads once into registers.
+template <int KPT, typename Put>
 __device__ __forceinline__ void select_top(const SparseArgs& a, const uint32_t* keys, int n, SelectSmem& sm, Put put) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
   const int f0 = first_scored(a, n), f1 = end_scored(a, n);
+  const int seg = (n + nw * 32 - 1) / (nw * 32) * 32;  // the warp's pages: [p0, p1)
+  const int p0 = min(n, warp * seg), p1 = min(n, p0 + seg);
   uint32_t lo = sm.lo, hi = sm.hi;
   uint32_t need = uint32_t(a.budget - f0 - (n - f1));  // scored pages to list (fewer than there are)
+  uint32_t held[KPT > 0 ? KPT : 1];
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const int p = p0 + 32 * i + lane;
+    held[i] = p < p1 ? keys[p] : 0u;
+  }
+  // f(page, key) over the lane's pages in order, 32 of the warp at a time (all lanes call it)
+  auto each = [&](auto f) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int i = 0; i < KPT; ++i)
+        if (p0 + 32 * i < p1) f(p0 + 32 * i + lane, held[i]);
+    } else {
+#pragma unroll 2
+      for (int q = p0; q < p1; q += 32) f(q + lane, q + lane < p1 ? keys[q + lane] : 0u);
+    }
+  };
   int buf = 0;
   while (need > 0 && lo < hi) {
     const int shift = max(0, 24 - __clz(hi - lo));  // (hi - lo) >> shift < 256
-    for (int p = f0 + tid; p < f1; p += nt) {
-      const uint32_t k = keys[p];
-      if (k >= lo && k <= hi) atomicAdd(&sm.hist[buf][255 - ((k - lo) >> shift)], 1u);
-    }
+    each([&](int p, uint32_t k) {
+      if (p >= f0 && p < min(f1, p1) && k >= lo && k <= hi) atomicAdd(&sm.hist[buf][255 - ((k - lo) >> shift)], 1u);
+    });
     // the next pass's bins, last read two passes ago: every warp has since met a barrier
     const int next = buf == 2 ? 0 : buf + 1;
     for (int i = tid; i < 256; i += nt) sm.hist[next][i] = 0;
@@ -195,23 +222,17 @@ __device__ __forceinline__ void select_top(const SparseArgs& a, const uint32_t* 
     buf = next;
   }
   // listed: keys above hi, then `need` of those in [lo, hi] in page order (all of them, or they are equal)
-  const int seg = (n + nw * 32 - 1) / (nw * 32) * 32;
-  const int p0 = min(n, warp * seg), p1 = min(n, p0 + seg);
-  auto judge = [&](int p, bool& gt, bool& eq) {
-    const uint32_t k = p < p1 ? keys[p] : 0u;
+  auto judge = [&](int p, uint32_t k, bool& gt, bool& eq) {
     gt = p < p1 && (p < f0 || p >= f1 || k > hi);
     eq = p < p1 && !gt && need > 0 && k >= lo;
   };
   uint32_t n_gt = 0, n_eq = 0;
-#pragma unroll 4
-  for (int q = p0; q < p1; q += 32) {
+  each([&](int p, uint32_t k) {
     bool gt, eq;
-    judge(q + lane, gt, eq);
-    n_gt += gt;
-    n_eq += eq;
-  }
-  n_gt = __reduce_add_sync(0xffffffffu, n_gt);
-  n_eq = __reduce_add_sync(0xffffffffu, n_eq);
+    judge(p, k, gt, eq);
+    n_gt += __popc(__ballot_sync(0xffffffffu, gt));
+    n_eq += __popc(__ballot_sync(0xffffffffu, eq));
+  });
   if (lane == 0) {
     sm.cnt[0][warp] = n_gt;
     sm.cnt[1][warp] = n_eq;
@@ -219,17 +240,16 @@ __device__ __forceinline__ void select_top(const SparseArgs& a, const uint32_t* 
   __syncthreads();
   uint32_t eq_before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.cnt[1][lane] : 0u);
   uint32_t at = __reduce_add_sync(0xffffffffu, lane < warp ? sm.cnt[0][lane] : 0u) + min(eq_before, need);
-#pragma unroll 2
-  for (int q = p0; q < p1; q += 32) {
+  each([&](int p, uint32_t k) {
     bool gt, eq;
-    judge(q + lane, gt, eq);
+    judge(p, k, gt, eq);
     const uint32_t beq = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1u;
     const bool sel = gt || (eq && eq_before + __popc(beq & below) < need);
     const uint32_t b = __ballot_sync(0xffffffffu, sel);
-    if (sel) put(int(at + __popc(b & below)), q + lane);
+    if (sel) put(int(at + __popc(b & below)), p);
     at += __popc(b);
     eq_before += __popc(beq);
-  }
+  });
 }
 
 __device__ __forceinline__ void imma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -271,6 +291,11 @@ __device__ __forceinline__ void red_cluster_min(uint32_t addr, uint32_t v) {
 }
 __device__ __forceinline__ void red_cluster_max(uint32_t addr, uint32_t v) {
   asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
   float2 v;
@@ -481,16 +506,22 @@ __global__ void __launch_bounds__(NW * 32, MINB) sparse_kernel(const SparseArgs 
   if (a.mode & PKV_SPARSE_SELECT) {
     len = min(n, a.budget);
     if (n > a.budget) {
-      if (rank == 0)
-        select_top(a, keys, n, sel, [&](int i, int p) {
+      if (rank == 0) {
+        auto put = [&](int i, int p) {
           prow[i] = p;
-          if (!attend) return;
-          list[i] = p;
-          for (int r = 1; r < cs; ++r) st_cluster(map_rank(smem_u32(list + i), r), uint32_t(p));
-        });
+          if (attend) list[i] = p;
+        };
+        if (n <= NW * 32 * 2) select_top<2>(a, keys, n, sel, put);
+        else if (n <= NW * 32 * 8) select_top<8>(a, keys, n, sel, put);
+        else select_top<0>(a, keys, n, sel, put);
+      }
       if (cs > 1) {
         cluster_arrive();
-        cluster_wait();  // rank 0's list is in every CTA
+        cluster_wait();  // rank 0's list is complete
+        if (attend && rank > 0) {
+          const uint32_t from = map_rank(smem_u32(list), 0);
+          for (int i = threadIdx.x; i < len; i += NW * 32) list[i] = int(ld_cluster(from + 4 * i));
+        }
       } else {
         __syncthreads();
       }
@@ -737,7 +768,7 @@ __global__ void __launch_bounds__(256) sparse_generic_kernel(const SparseArgs a)
         atomicMax(&sel.hi, hi);
       }
       __syncthreads();
-      select_top(a, keys, n, sel, [&](int i, int p) { list[i] = p; });
+      select_top<0>(a, keys, n, sel, [&](int i, int p) { list[i] = p; });
     } else {
       for (int p = threadIdx.x; p < n; p += blockDim.x) list[p] = p;
     }
@@ -878,13 +909,19 @@ int launch_sparse_generic(const SparseArgs& a, cudaStream_t s) {
 template <typename T>
 int launch_sparse(const SparseArgs& a, bool fast, cudaStream_t s) {
   if (!fast) return launch_sparse_generic<T>(a, s);
-  // rows are split over clusters of up to 8 CTAs while that leaves at most two per SM
+  // Rows are split over clusters of up to 8 CTAs while that leaves at most two CTAs
+  // per SM: 8 rows of 2048 pages 34 us without, 13.4 with clusters of 8; 256 rows
+  // of 350 pages 21 without, 27 in pairs.
   const int64_t rows = int64_t(a.n_tokens) * a.n_kv;
   const int sms = num_sms();
   int cs = 1;
   while (cs < 8 && rows * cs * 2 <= 2 * sms) cs *= 2;
+  // head_dim 128: 8 KiB a tile and 152 registers leave two CTAs of 4 warps; 3 ring
+  // stages 17.7 us on 140 rows of 250 pages, 2 stages 19.5, 4 stages 28.7
   if (a.d == 128) return launch_sparse_t<T, 128, 4, 3, 1, 2>(a, rows, cs, s);
-  // up to two CTAs per SM: 8 warps each; more: 4 warps and more CTAs resident
+  // Up to two CTAs per SM: 8 warps each (256 rows of 350 pages: 16.0 us, 4 warps
+  // 20.5); more rows: 4 warps, five CTAs resident (2048 rows of 170 pages: 107 us,
+  // four resident 116, 8 warps 127).
   if (rows * cs <= 2 * sms) return launch_sparse_t<T, 64, 8, 2, 1, 2>(a, rows, cs, s);
   return launch_sparse_t<T, 64, 4, 2, 1, 5>(a, rows, cs, s);
 }
