@@ -303,8 +303,8 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     // with tiles (all, or two thirds beside streaming ones) take an item after the
     // other: rounds of a range's blocks and an item's set-up (two blocks' time);
     // then the pieces, whose writing and reading is three blocks' work for a full
-    // tile, and the merge's rounds of eight. (256 sequences on a 4096-token prefix: ranges of 16 blocks, one
-    // round, 53 us; of 4 to 10 blocks 57 to 62 us.)
+    // tile, and the merge's rounds of eight. (256 sequences on a 4096-token
+    // prefix: ranges of 16 blocks, 256 items, 44 us; 22 blocks 49, 32 blocks 57.)
     const int slots = int64_t(s_listed) * a.n_kv >= 8 * a.sms ? 2 * a.sms : SH_MINB * a.sms;
     const int maxblk = s_maxblk;
     const int step = (maxblk + int(blockDim.x) - 1) / int(blockDim.x);
@@ -440,12 +440,19 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   // than there are: nothing is streamed
   const bool over = base_pg > a.total_pages;
   const int P = over ? 0 : base_pg;
-  // CTAs that stream first: all when there are no tiles, else one per SM, or two
-  // where the pages' time at the copy rate is more than twice the tiles' (a page
-  // of one KV head: 4 KiB; a block of a tile: 820 cycles of its SM). 32 families
-  // of 8: two 53.4 us, one 63.6; the 4096-token prefix above: one 53, two 60.
+  // CTAs that stream first: all when there are no tiles; 7/4 an SM where the
+  // pages' time at the copy rate is more than four times the tiles' (a page of one
+  // KV head: 4 KiB; a block of a tile: 820 cycles of its SM); else those that the
+  // tiles' one round leaves, 1 to 7/4 an SM. 32 groups of 8 sequences (ratio 9):
+  // 1, 5/4, 3/2, 7/4, 2 an SM 58.0, 54.0, 50.8, 49.4, 50.5 us; 256 sequences on a
+  // 4096-token prefix (ratio 2, 256 items): 48.5, 44.5, 58.1, 59.0, 58.5, as left
+  // by the round (188 of 444 CTAs) 43.9.
   const float t_stream = float(P) * a.n_kv * 4096.f / 6.4e6f, t_tiles = float(blocks) * a.n_kv / a.sms * 0.43f;  // us
-  int n_stream = P == 0 ? 0 : n_items == 0 ? a.grid : t_stream > 2.f * t_tiles ? 2 * a.sms : a.sms;
+  const int most_stream = a.sms * 7 / 4;
+  int n_stream = P == 0                     ? 0
+                 : n_items == 0             ? a.grid
+                 : t_stream > 4.f * t_tiles ? most_stream
+                                            : int(max(int64_t(a.sms), min(int64_t(most_stream), a.grid - int64_t(n_items) * a.n_kv)));
   n_stream = min(n_stream, (P * a.n_kv + SH_WARPS - 1) / SH_WARPS);
   const int ranges = P == 0 ? 0 : max(1, min(P, n_stream * SH_WARPS / a.n_kv));
   __syncthreads();
