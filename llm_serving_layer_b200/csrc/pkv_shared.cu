@@ -40,7 +40,10 @@ namespace pkv {
 namespace {
 
 constexpr int SH_MINB = 3;          // CTAs per SM
-constexpr int SH_NST = 2;           // slots of the K ring and of the V ring
+// Slots of the K and of the V ring. A K slot is free when its S is computed, a
+// period before the next S is; a V slot when its P V is, a period later: with
+// three K slots and K loaded two blocks ahead of V both have two periods' time.
+constexpr int SH_KST = 3, SH_VST = 2;
 constexpr int SH_TMEM_COLS = 128;   // S in columns 0-63, O in 64-127
 constexpr int SH_PIECES = 16384;    // tile piece rows the workspace holds at most (x n_heads x 264 bytes)
 constexpr int SH_WARPS = TC_THREADS / 32;
@@ -759,14 +762,14 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
   // 1024-byte aligned by its declaration: every address below is a constant
   unsigned char* smem = smem_raw;
   unsigned char* qbuf = smem;                             // [128 rows][128 B], 128B swizzle
-  unsigned char* kst = smem + TC_QTILE;                   // SH_NST x K [64 keys][128 B]
-  unsigned char* vst = kst + size_t(SH_NST) * TC_KTILE;   // SH_NST x V [64 keys][128 B]
-  unsigned char* pbuf = vst + size_t(SH_NST) * TC_KTILE;  // P [128 rows][128 B], 128B swizzle
+  unsigned char* kst = smem + TC_QTILE;                   // SH_KST x K [64 keys][128 B]
+  unsigned char* vst = kst + size_t(SH_KST) * TC_KTILE;   // SH_VST x V [64 keys][128 B]
+  unsigned char* pbuf = vst + size_t(SH_VST) * TC_KTILE;  // P [128 rows][128 B], 128B swizzle
   uint64_t* kfull = reinterpret_cast<uint64_t*>(pbuf + TC_QTILE);
-  uint64_t* kempty = kfull + SH_NST;
-  uint64_t* vfull = kempty + SH_NST;
-  uint64_t* vempty = vfull + SH_NST;
-  uint64_t* s_full = vempty + SH_NST;
+  uint64_t* kempty = kfull + SH_KST;
+  uint64_t* vfull = kempty + SH_KST;
+  uint64_t* vempty = vfull + SH_VST;
+  uint64_t* s_full = vempty + SH_VST;
   uint64_t* s_free = s_full + 1;
   uint64_t* p_full = s_free + 1;
   uint64_t* pv_done = p_full + 1;
@@ -781,22 +784,24 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
   if (threadIdx.x == 0) {
     prefetch_tmap(&tmap);
     prefetch_tmap(&qmap);
-    for (int i = 0; i < SH_NST; ++i) {
+    for (int i = 0; i < SH_KST; ++i) {
       mbar_init(&kfull[i], 1);
       mbar_init(&kempty[i], 1);
+    }
+    for (int i = 0; i < SH_VST; ++i) {
       mbar_init(&vfull[i], 1);
       mbar_init(&vempty[i], 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, 128);
-    mbar_init(p_full, 128);
+    mbar_init(s_free, 4);
+    mbar_init(p_full, 4);
     mbar_init(pv_done, 1);
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    mbar_init(o_free, 128);
+    mbar_init(o_free, 4);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 129);
+      mbar_init(&item_empty[i], 5);
     }
     mbar_init(drain, 1);
     fence_mbar_init();
@@ -810,7 +815,7 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     const int kvc = 2 * a.layer;
-    uint32_t kiss = 0, viss = 0;  // K / V slots filled so far
+    uint32_t kiss = 0, viss = 0, qiss = 0;  // K / V slots and query tiles filled so far
     int it = 0;                   // items published
     bool dead = false;
     int w = s_first;
@@ -847,53 +852,63 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
       __syncwarp();
       if (end) break;
       if (lane == 0) {
-        if (it >= 1 && !mbar_wait_bounded_sleepy(q_empty, (it - 1) & 1, a.st, 64)) dead = true;
-        if (!dead) {
-          mbar_arrive_expect_tx(q_full, TC_QTILE);
-          tma_load_3d(qbuf, &qmap, q_full, 0, I.h * G, I.t0);
-        }
-        for (int j = 0; j < I.nblk && !dead; ++j) {
-          int rows[TC_PPB];
+        // four pages' rows of block j; a page past the range reads the zero fill of a negative coordinate
+        auto load = [&](unsigned char* dst, uint64_t* full, int j, int kv) {
+          mbar_arrive_expect_tx(full, TC_KTILE);
 #pragma unroll
           for (int u = 0; u < TC_PPB; ++u) {
             const int pg = j * TC_PPB + u;
-            // a page past the range reads the zero fill of a negative coordinate
-            rows[u] = pg < I.n_pg && !pg_bad ? a.kv_indices[pg_at + pg] * TC_P : -TC_P;
+            const int row = pg < I.n_pg && !pg_bad ? a.kv_indices[pg_at + pg] * TC_P : -TC_P;
+            tma_load_4d(dst + u * TC_PAGE, &tmap, full, 0, row, I.h, kv);
           }
-          const int st = int(kiss % SH_NST);
-          if (kiss >= SH_NST && !mbar_wait_bounded_sleepy(&kempty[st], ((kiss / SH_NST) - 1) & 1, a.st, 32)) {
+        };
+        auto load_k = [&](int j) {
+          const int st = int(kiss % SH_KST);
+          if (kiss >= SH_KST && !mbar_wait_bounded_sleepy(&kempty[st], ((kiss / SH_KST) - 1) & 1, a.st, 32)) {
             dead = true;
-            break;
+            return;
           }
-          mbar_arrive_expect_tx(&kfull[st], TC_KTILE);
-#pragma unroll
-          for (int u = 0; u < TC_PPB; ++u)
-            tma_load_4d(kst + size_t(st) * TC_KTILE + u * TC_PAGE, &tmap, &kfull[st], 0, rows[u], I.h, kvc);
+          load(kst + size_t(st) * TC_KTILE, &kfull[st], j, kvc);
           ++kiss;
-          if (viss >= SH_NST && !mbar_wait_bounded_sleepy(&vempty[st], ((viss / SH_NST) - 1) & 1, a.st, 32)) {
+        };
+        // the query tile: first thing, or once the item before has read its own
+        if (it >= 1) {
+          for (int j = 0; j < SH_KST - 1 && j < I.nblk && !dead; ++j) load_k(j);
+          if (!dead && !mbar_wait_bounded_sleepy(q_empty, (it - 1) & 1, a.st, 64)) dead = true;
+        }
+        if (!dead) {
+          mbar_arrive_expect_tx(q_full, TC_QTILE);
+          tma_load_3d(qbuf, &qmap, q_full, 0, I.h * G, I.t0);
+          ++qiss;
+        }
+        if (it == 0)
+          for (int j = 0; j < SH_KST - 1 && j < I.nblk && !dead; ++j) load_k(j);
+        for (int j = 0; j < I.nblk && !dead; ++j) {
+          if (j + SH_KST - 1 < I.nblk) load_k(j + SH_KST - 1);
+          if (dead) break;
+          // the next item, two blocks before it is needed. No claim where the CTAs' own
+          // numbers cover the items: atomics on one address take turns
+          if (j == I.nblk - 1) w = n_tile < n_items ? n_tile + atomicAdd(a.claim, 1) : n_items;
+          const int st = int(viss % SH_VST);
+          if (viss >= SH_VST && !mbar_wait_bounded_sleepy(&vempty[st], ((viss / SH_VST) - 1) & 1, a.st, 32)) {
             dead = true;
             break;
           }
-          mbar_arrive_expect_tx(&vfull[st], TC_KTILE);
-#pragma unroll
-          for (int u = 0; u < TC_PPB; ++u)
-            tma_load_4d(vst + size_t(st) * TC_KTILE + u * TC_PAGE, &tmap, &vfull[st], 0, rows[u], I.h, kvc + 1);
+          load(vst + size_t(st) * TC_KTILE, &vfull[st], j, kvc + 1);
           ++viss;
         }
       }
       dead = __shfl_sync(0xffffffffu, dead, 0);
       ++it;
-      // no claim where the CTAs' own numbers cover the items: atomics on one address take turns
-      if (lane == 0) w = n_tile < n_items ? n_tile + atomicAdd(a.claim, 1) : n_items;
       w = __shfl_sync(0xffffffffu, w, 0);
     }
     if (dead && lane == 0) {
       // let this CTA's own copies land before its shared memory can be released
-      for (uint32_t i = kiss > SH_NST ? kiss - SH_NST : 0; i < kiss; ++i)
-        mbar_wait_bounded(&kfull[i % SH_NST], (i / SH_NST) & 1, nullptr);
-      for (uint32_t i = viss > SH_NST ? viss - SH_NST : 0; i < viss; ++i)
-        mbar_wait_bounded(&vfull[i % SH_NST], (i / SH_NST) & 1, nullptr);
-      if (it >= 1) mbar_wait_bounded(q_full, (it - 1) & 1, nullptr);
+      for (uint32_t i = kiss > SH_KST ? kiss - SH_KST : 0; i < kiss; ++i)
+        mbar_wait_bounded(&kfull[i % SH_KST], (i / SH_KST) & 1, nullptr);
+      for (uint32_t i = viss > SH_VST ? viss - SH_VST : 0; i < viss; ++i)
+        mbar_wait_bounded(&vfull[i % SH_VST], (i / SH_VST) & 1, nullptr);
+      if (qiss >= 1) mbar_wait_bounded(q_full, (qiss - 1) & 1, nullptr);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
@@ -905,10 +920,10 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
     int it = 0;
     bool dead = false;
     auto pv = [&](uint32_t gp, int jp, const ShItem& I) -> bool {
-      const int stp = int(gp % SH_NST);
+      const int stp = int(gp % SH_VST);
       bool bad = !mbar_wait_bounded(p_full, gp & 1, a.st);
       if (!bad && jp == 0 && it >= 1 && !mbar_wait_bounded(o_free, (it - 1) & 1, a.st)) bad = true;
-      if (!bad && !mbar_wait_bounded(&vfull[stp], (gp / SH_NST) & 1, a.st)) bad = true;
+      if (!bad && !mbar_wait_bounded(&vfull[stp], (gp / SH_VST) & 1, a.st)) bad = true;
       bad = __any_sync(0xffffffffu, bad);
       if (bad) return false;
       if (I.tail_pg >= 0 && jp == I.tail_pg / TC_PPB) {
@@ -943,10 +958,10 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
       if (dead) break;
       for (int j = 0; j < I.nblk; ++j) {
         const uint32_t gj = g + j;
-        const int st = int(gj % SH_NST);
+        const int st = int(gj % SH_KST);
         // S_j overwrites S_{j-1}: after the softmax threads loaded it
         if (gj >= 1 && !mbar_wait_bounded(s_free, (gj - 1) & 1, a.st)) dead = true;
-        if (!dead && !mbar_wait_bounded(&kfull[st], (gj / SH_NST) & 1, a.st)) dead = true;
+        if (!dead && !mbar_wait_bounded(&kfull[st], (gj / SH_KST) & 1, a.st)) dead = true;
         dead = __any_sync(0xffffffffu, dead);
         if (dead) break;
         if (lane == 0) {
@@ -999,8 +1014,12 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
       const int nblk = s_item[sl].nblk;
       if (nblk == 0) break;
       const int nt = s_item[sl].nt;
-      // last key of the range this row sees (a row past the tile's tokens: none)
-      const int lim = r / G < nt ? s_item[sl].lim0 + s_item[sl].causal * (r / G) : -1;
+      // last key of the range this row sees. A row past the tile's tokens is not
+      // masked (the mask costs its warp 550 of 2400 cycles a block): nothing reads it
+      const int lim = r / G < nt ? s_item[sl].lim0 + s_item[sl].causal * (r / G) : 0x7fffffff;
+      // no token in this warp's 32 rows: only the barriers. Its rows of P hold
+      // anything: they reach its own rows of O alone, which nothing reads
+      const bool idle = q4 * 32 / G >= nt;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nblk; ++j) {
         const uint32_t gj = g + j;
@@ -1008,10 +1027,19 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
         dead = __any_sync(0xffffffffu, dead);
         if (dead) break;
         tc_fence_after();
+        if (idle) {
+          if (lane == 0) mbar_arrive(s_free);
+          if (gj >= 1 && !mbar_wait_bounded(pv_done, (gj - 1) & 1, a.st)) dead = true;
+          dead = __any_sync(0xffffffffu, dead);
+          if (dead) break;
+          if (lane == 0) mbar_arrive(p_full);
+          continue;
+        }
         uint32_t sr[64];
         tmem_ld64(tbase + lane_off, sr);
         tc_fence_before();
-        mbar_arrive(s_free);  // S_{j+1} may overwrite S now
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);  // S_{j+1} may overwrite S now
         const int kb0 = j * TC_KB;
         if (sl2 <= 0.f) {  // a non-positive scale: scale first so the masked -inf stays the minimum
 #pragma unroll
@@ -1052,7 +1080,8 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
           sh_rescale_o(tO + lane_off, alpha);
         }
         tc_fence_before();
-        mbar_arrive(p_full);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
       }
       if (dead) break;
       // ---- epilogue: O / l of the item -> its piece rows in fp32 (or out in the
@@ -1076,8 +1105,11 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
         tmem_ld32(tO + lane_off + half * 32, o);
         tc_fence_before();
         if (half == 1) {
-          mbar_arrive(o_free);           // O read: the next item's first P.V may overwrite it
-          mbar_arrive(&item_empty[sl]);  // and the item's fields
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(o_free);           // O read: the next item's first P.V may overwrite it
+            mbar_arrive(&item_empty[sl]);  // and the item's fields
+          }
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(inv == 0.f ? 0.f : __uint_as_float(o[i]) * inv);
@@ -1126,7 +1158,7 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
 }
 
 // the tile role's buffers, or the streaming warps' rings
-size_t sh_smem() { return std::max(2 * size_t(TC_QTILE) + size_t(2 * SH_NST) * TC_KTILE + 256, SH_RING); }
+size_t sh_smem() { return std::max(2 * size_t(TC_QTILE) + size_t(SH_KST + SH_VST) * TC_KTILE + 256, SH_RING); }
 
 // ---------------------------------------------------------------- merge
 // One warp per (token, query head): its pieces over the shared keys and over its
