@@ -185,6 +185,17 @@ __device__ __forceinline__ int group_of(const PlanArgs& a, int s) {
   return lo;
 }
 
+// CTAs that stream first at the least, from the streaming's and the tiles' time on
+// the whole GPU (a page of one KV head is 4 KiB at the copy rate; a block of a
+// tile keeps its SM for 860 cycles): 7/4 an SM from four times the tiles' time on,
+// below that the streaming's share, one an SM at most (256 sequences of 2 tokens
+// on an 8192-token prefix: 7 CTAs, 46 us; one an SM 54).
+__device__ __forceinline__ int stream_least(const PlanArgs& a, int listed, float blocks) {
+  const float t_stream = float(listed) * a.n_kv * 4096.f / 6.4e6f, t_tiles = blocks * a.n_kv / a.sms * 0.45f;  // us
+  if (t_stream >= 4.f * t_tiles) return a.sms * 7 / 4;
+  return min(a.sms, int(a.grid * t_stream / (t_stream + t_tiles)) + 1);
+}
+
 // One CTA per sequence: do its leading pages agree with its group's first
 // sequence's, and do its new tokens lie after them? If not the group is marked
 // (and flagged) and computed without sharing.
@@ -228,7 +239,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   }
   // share = 1: as the groups say. Should even one piece per row and range not
   // fit the workspace, a second round (share = 0) computes every sequence by itself.
-  int n_ents = 0, n_shared = 0, chunk = 1;
+  int n_ents = 0, n_shared = 0, chunk = 1, n_lo = 0;
   for (int share = 1; share >= 0; --share) {
     if (tid == 0) {
       s_maxblk = 1;
@@ -303,16 +314,16 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     __threadfence_block();
     __syncthreads();
     // ---- blocks per range: each thread weighs one length. The CTAs that start
-    // with tiles (all, or two thirds beside streaming ones) take an item after the
-    // other: rounds of a range's blocks and an item's set-up (two blocks' time);
-    // then the pieces, whose writing and reading is three blocks' work for a full
-    // tile, and the merge's rounds of eight. (256 sequences on a 4096-token
-    // prefix: ranges of 16 blocks, 256 items, 44 us; 22 blocks 49, 32 blocks 57.)
-    const int slots = int64_t(s_listed) * a.n_kv >= 8 * a.sms ? 2 * a.sms : SH_MINB * a.sms;
+    // with tiles take an item after the other: rounds of a range's blocks and an
+    // item's set-up and epilogue (four blocks' time); then the pieces, whose writing
+    // and reading is three blocks' work for a full tile, and the merge's rounds of
+    // eight. (256 sequences on a 4096-token prefix, 512-token rest: ranges of 16
+    // blocks, 256 items, 44 us; 22 blocks 49, 32 blocks 57. 24 groups of 2 on
+    // prefixes of up to 4000 tokens: 39 us, with a set-up of two blocks 53.)
     const int maxblk = s_maxblk;
     const int step = (maxblk + int(blockDim.x) - 1) / int(blockDim.x);
     const int cand = min(maxblk, (tid + 1) * step);
-    float n_it = 0.f, rows = 0.f;
+    float n_it = 0.f, rows = 0.f, n_blk = 0.f;
     int most = 1;
     int64_t pieces = 0;
     bool fits = true;
@@ -322,6 +333,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
       const int sp = x.base < 0 ? 1 : (nb + cand - 1) / cand;
       fits &= sp <= a.splits_cap;
       n_it += float(x.tiles) * sp;
+      n_blk += float(x.tiles) * nb;
       if (x.base >= 0) {
         pieces += int64_t(x.nt) * sp;
         rows += float(x.nt) * sp;
@@ -329,8 +341,9 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
       }
     }
     fits &= pieces <= a.pieces_cap;
-    const float est = ceilf(n_it * a.n_kv / slots) * (cand + 2.f) + rows / a.tpt * a.n_kv * 3.f / a.sms +
-                      1.5f * ((most + 7) / 8);
+    n_lo = stream_least(a, s_listed, n_blk);
+    const float slots = float(a.grid - n_lo), items = n_it * a.n_kv;
+    const float est = ceilf(items / slots) * (cand + 4.f) + rows / a.tpt * a.n_kv * 3.f / a.sms + 1.5f * ((most + 7) / 8);
     if (tid == 0) s_best = ~0ull;
     __syncthreads();
     if (fits && (tid == 0 || (tid + 1) * step < maxblk + step))
@@ -443,19 +456,15 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   // than there are: nothing is streamed
   const bool over = base_pg > a.total_pages;
   const int P = over ? 0 : base_pg;
-  // CTAs that stream first: all when there are no tiles; 7/4 an SM where the
-  // pages' time at the copy rate is more than four times the tiles' (a page of one
-  // KV head: 4 KiB; a block of a tile: 820 cycles of its SM); else those that the
-  // tiles' one round leaves, 1 to 7/4 an SM. 32 groups of 8 sequences (ratio 9):
-  // 1, 5/4, 3/2, 7/4, 2 an SM 58.0, 54.0, 50.8, 49.4, 50.5 us; 256 sequences on a
-  // 4096-token prefix (ratio 2, 256 items): 48.5, 44.5, 58.1, 59.0, 58.5, as left
-  // by the round (188 of 444 CTAs) 43.9.
-  const float t_stream = float(P) * a.n_kv * 4096.f / 6.4e6f, t_tiles = float(blocks) * a.n_kv / a.sms * 0.43f;  // us
+  // CTAs that stream first: all when there are no tiles, else those that the tiles'
+  // one round leaves, stream_least to 7/4 an SM. 32 groups of 8 sequences (the
+  // streaming's time is 9 of the tiles'): 1, 5/4, 3/2, 7/4, 2 an SM 58.0, 54.0,
+  // 50.8, 49.4, 50.5 us; 256 sequences on a 4096-token prefix (2 of the tiles', 256
+  // items): 48.5, 44.5, 58.1, 59.0, 58.5, as left by the round (188 of 444 CTAs) 43.9.
   const int most_stream = a.sms * 7 / 4;
-  int n_stream = P == 0                     ? 0
-                 : n_items == 0             ? a.grid
-                 : t_stream > 4.f * t_tiles ? most_stream
-                                            : int(max(int64_t(a.sms), min(int64_t(most_stream), a.grid - int64_t(n_items) * a.n_kv)));
+  int n_stream = P == 0       ? 0
+                 : n_items == 0 ? a.grid
+                                : int(max(int64_t(n_lo), min(int64_t(most_stream), a.grid - int64_t(n_items) * a.n_kv)));
   n_stream = min(n_stream, (P * a.n_kv + SH_WARPS - 1) / SH_WARPS);
   const int ranges = P == 0 ? 0 : max(1, min(P, n_stream * SH_WARPS / a.n_kv));
   __syncthreads();
@@ -1084,6 +1093,15 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
         if (lane == 0) mbar_arrive(p_full);
       }
       if (dead) break;
+      if (idle) {
+        if (lane == 0) {
+          mbar_arrive(o_free);
+          mbar_arrive(&item_empty[sl]);
+        }
+        g += nblk;
+        ++it;
+        continue;
+      }
       // ---- epilogue: O / l of the item -> its piece rows in fp32 (or out in the
       // pool dtype), staged through this warp's own rows of the P tile (the
       // item's last P.V completed) 32 columns at a time, so that the stores are
