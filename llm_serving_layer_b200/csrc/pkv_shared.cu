@@ -387,8 +387,6 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   if (tid == 0) s_tot = item0 <= a.items_cap ? 1 : 0;
   __syncthreads();
   const bool room = s_tot != 0;  // the capacity covers every case: kept as a check
-  if (tid == 0) s_maxblk = 0;
-  __syncthreads();
   for (int i = warp; room && i < n_ents; i += 32) {
     const ShEnt x = a.ents[i];
     for (int k = lane; k < x.tiles * x.splits; k += 32) {
@@ -408,7 +406,6 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
       I.lpl = x.lpl;
       I.piece = x.base < 0 ? -1 : x.base + sp * x.nt + i0;
       a.items[x.item0 + k] = I;
-      atomicAdd(&s_maxblk, I.nblk);
     }
     if (x.base >= 0) {
       int4* to = x.causal ? a.rest : a.fold;
@@ -416,7 +413,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     }
   }
   __syncthreads();
-  const int n_items = room ? item0 : 0, blocks = s_maxblk;
+  const int n_items = room ? item0 : 0;
   // ---- the one-token sequences' list: their pages after the shared ones
   int base_seq = 0, base_pg = 0;
   for (int c0 = 0; c0 < a.n_seqs; c0 += blockDim.x) {

@@ -222,14 +222,14 @@ __device__ __forceinline__ void select_top(const SparseArgs& a, const uint32_t* 
     buf = next;
   }
   // listed: keys above hi, then `need` of those in [lo, hi] in page order (all of them, or they are equal)
-  auto judge = [&](int p, uint32_t k, bool& gt, bool& eq) {
+  auto compare = [&](int p, uint32_t k, bool& gt, bool& eq) {
     gt = p < p1 && (p < f0 || p >= f1 || k > hi);
     eq = p < p1 && !gt && need > 0 && k >= lo;
   };
   uint32_t n_gt = 0, n_eq = 0;
   each([&](int p, uint32_t k) {
     bool gt, eq;
-    judge(p, k, gt, eq);
+    compare(p, k, gt, eq);
     n_gt += __popc(__ballot_sync(0xffffffffu, gt));
     n_eq += __popc(__ballot_sync(0xffffffffu, eq));
   });
@@ -242,7 +242,7 @@ __device__ __forceinline__ void select_top(const SparseArgs& a, const uint32_t* 
   uint32_t at = __reduce_add_sync(0xffffffffu, lane < warp ? sm.cnt[0][lane] : 0u) + min(eq_before, need);
   each([&](int p, uint32_t k) {
     bool gt, eq;
-    judge(p, k, gt, eq);
+    compare(p, k, gt, eq);
     const uint32_t beq = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1u;
     const bool sel = gt || (eq && eq_before + __popc(beq & below) < need);
     const uint32_t b = __ballot_sync(0xffffffffu, sel);
