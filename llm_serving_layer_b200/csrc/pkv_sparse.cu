@@ -127,10 +127,12 @@ __device__ __forceinline__ void quantise_query(const SparseArgs& a, const T* q, 
 }
 
 struct SelectSmem {
-  uint32_t hist[3][256];  // reversed bins: entry 255 - b counts bin b
-  uint32_t cnt[2][32];    // per warp: keys above the threshold, keys equal to it
-  uint32_t lo, hi;        // range of the scored keys
+  alignas(16) uint32_t hist[3][256];  // reversed bins: entry 255 - b counts bin b
+  uint32_t cnt[2][32];                // per warp: keys above the threshold, keys equal to it
+  uint32_t lo, hi;                    // range of the scored keys
 };
+static_assert(alignof(SelectSmem) >= alignof(uint4) && sizeof(SelectSmem::hist[0]) % sizeof(uint4) == 0,
+              "select_top reads the bins four at a time");
 
 // Before the scores: an empty range and histogram (a barrier follows).
 __device__ __forceinline__ void select_init(SelectSmem& sm) {
