@@ -828,6 +828,10 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
   tc_fence_after();
   const uint32_t tbase = s_tmem;
   const uint32_t tO = tbase + TC_KB;
+  // The kernels before this one may run for as long as they need: the bounded
+  // waits below count from their completion (warp 0 waits once it has read the
+  // plan's part of its first item).
+  if (warp != 0) pdl_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -852,8 +856,7 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
       }
       pg_bad = __any_sync(0xffffffffu, pg_bad);
       // q, this layer's appended K/V rows and the pieces' last readers: the first
-      // item is the plan's and was read ahead of the wait; the other warps follow
-      // this one's copies
+      // item is the plan's and was read ahead of the wait
       if (it == 0) pdl_wait();
       const int sl = it & 1;
       if (it >= 2 && !mbar_wait_bounded_sleepy(&item_empty[sl], ((it - 2) >> 1) & 1, a.st, 32)) dead = true;
