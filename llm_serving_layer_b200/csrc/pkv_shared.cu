@@ -557,7 +557,9 @@ __device__ __forceinline__ void stream_range(const ShArgs& a, unsigned char* rin
       cp_async16(dst + SH_TILE + sw, a.v_slab + off, ok);
     }
   };
-  auto load_q = [&](int sq, uint32_t (&qb)[4][2]) {  // B operand of list entry sq's queries of this KV head
+  // B operand of list entry sq's queries of this KV head (plain loads: the
+  // kernel that writes them may still run when this one starts)
+  auto load_q = [&](int sq, uint32_t (&qb)[4][2]) {
     const int row = sq < a.n_seqs ? __ldcg(a.rows + sq) : -1;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) qb[ks][0] = qb[ks][1] = 0u;
@@ -565,8 +567,8 @@ __device__ __forceinline__ void stream_range(const ShArgs& a, unsigned char* rin
       const T* qr = q + (int64_t(row) * a.n_heads + h * G + g) * TC_D + 2 * c4;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        qb[ks][0] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16));
-        qb[ks][1] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8));
+        qb[ks][0] = *reinterpret_cast<const uint32_t*>(qr + ks * 16);
+        qb[ks][1] = *reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8);
       }
     }
   };

@@ -338,14 +338,16 @@ __global__ void __launch_bounds__(NW * 32, MINB) sparse_kernel(const SparseArgs 
   const int64_t q0 = (int64_t(t) * a.n_heads + int64_t(h) * G) * D;
   const T* q = static_cast<const T*>(a.q) + q0;
   // this lane's part of the queries as the score products' B operand, loaded
-  // while the row travels
+  // while the row travels. Plain loads here and for the index: the kernel that writes
+  // them may still run when this one starts, and the read-only path is for what
+  // stays as it is from launch to end
   uint32_t qb[KS][2];
   if (g < G) {
     const T* qr = q + g * D + 2 * c4;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      qb[ks][0] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16));
-      qb[ks][1] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8));
+      qb[ks][0] = *reinterpret_cast<const uint32_t*>(qr + ks * 16);
+      qb[ks][1] = *reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8);
     }
   } else {
 #pragma unroll
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(NW * 32, MINB) sparse_kernel(const SparseArgs 
           const int64_t idr = __shfl_sync(0xffffffffu, id[u], g + 8 * r);
           const uint4* src = reinterpret_cast<const uint4*>(a.codes + (idr * a.n_kv + h) * (2 * D)) + c4;
 #pragma unroll
-          for (int j = 0; j < J; ++j) w[u][r][j] = __ldg(src + 4 * j);
+          for (int j = 0; j < J; ++j) w[u][r][j] = src[4 * j];
         }
       }
 #pragma unroll

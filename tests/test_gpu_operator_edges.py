@@ -56,3 +56,52 @@ def test_a_long_kernel_before_is_waited_for():
     bk.check_status()
     slow.check_status()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("attention", ["shared", "sparse", "attend"])
+def test_a_chain_of_launches_reads_what_was_just_written(attention):
+    """Steps into the same buffers without a pause, each kernel launched while the one before still runs: every q,
+    key and index entry that a step reads is the one just written."""
+    P, n, hq, hkv, d, steps = 16, 64, 8, 2, 64, 48
+    g = torch.Generator(device=DEV).manual_seed(8)
+    lead = list(range(8))
+    tables = [lead + [8 + 4 * i + j for j in range(4)] for i in range(n)]
+    qkv = torch.randn(steps, n, (hq + 2 * hkv) * d, generator=g, device=DEV).half()
+    ang = torch.rand(256, d // 2, generator=g, device=DEV) * 6
+    rope = (torch.cos(ang), torch.sin(ang))
+    kv = [len(lead) * P + 1] * n
+
+    def run(pause):
+        bk = B200PagedBackend(1, 8 + 4 * n, P, hkv, hq, d, device=DEV, validate="device")
+        bk.k_pool[0].copy_(torch.randn(bk.k_pool[0].shape, generator=g.manual_seed(9), device=DEV))
+        bk.v_pool[0].copy_(torch.randn(bk.v_pool[0].shape, generator=g, device=DEV))
+        index = PageIndex(bk)
+        index.rebuild(range(bk.num_blocks))
+        q_out = torch.empty(n, hq, d, dtype=torch.float16, device=DEV)
+        outs = torch.empty(steps, n, hq, d, dtype=torch.float16, device=DEV)
+        metas = [build_meta(tables, [x + t for x in kv], [1] * n, P, device=DEV) for t in range(steps)]
+        plan = {"shared": lambda m: bk.plan_shared(m, SharedPrefix([n], [8])),
+                "sparse": lambda m: bk.plan_sparse(m, index, 5), "attend": lambda m: m}[attention]
+        plans = [plan(m) for m in metas]
+        slices = [[x.unflatten(1, (-1, d)) for x in s.split([hq * d, hkv * d, hkv * d], 1)] for s in qkv]
+        torch.cuda.synchronize()
+        for t in range(steps):
+            if attention == "attend":
+                bk.plan(metas[t])
+            bk.rope_append(0, *slices[t], metas[t], rope, index=index, q_out=q_out)
+            if pause:
+                torch.cuda.synchronize()
+            if attention == "shared":
+                bk.attend_shared(q_out, 0, 0.125, plans[t], out=outs[t])
+            elif attention == "sparse":
+                bk.attend_sparse(q_out, 0, 0.125, plans[t], out=outs[t])
+            else:
+                bk.attend(q_out, 0, 0.125, metas[t], out=outs[t])
+            if pause:
+                torch.cuda.synchronize()
+        bk.check_status()
+        return outs
+
+    want = run(True)
+    for _ in range(3):
+        assert torch.equal(run(False), want)
