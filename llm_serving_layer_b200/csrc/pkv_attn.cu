@@ -182,15 +182,17 @@ __device__ __forceinline__ int cta_of(int64_t p, int64_t P, int G) {
   return int(((p + 1) * G + P - 1) / P) - 1;
 }
 
+// Plain loads: the kernel that writes q may still run when this one starts (the
+// read-only path is for what stays as it is from launch to end).
 template <typename T, int GROUPS>
-__device__ __forceinline__ void load_q_frag(const T* __restrict__ q, int row, int n_heads, int h,
+__device__ __forceinline__ void load_q_frag(const T* q, int row, int n_heads, int h,
                                             int g, int c4, uint32_t (&qb)[4][2]) {
   if (g < GROUPS) {
     const T* qr = q + (int64_t(row) * n_heads + h * GROUPS + g) * DK_D + 2 * c4;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      qb[ks][0] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16));
-      qb[ks][1] = __ldg(reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8));
+      qb[ks][0] = *reinterpret_cast<const uint32_t*>(qr + ks * 16);
+      qb[ks][1] = *reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8);
     }
   } else {
 #pragma unroll
@@ -625,12 +627,19 @@ __global__ void __maxnreg__(DK_MAXNREG) decode_kernel(const __grid_constant__ CU
                   flag(a.st, PKV_DEV_META_BAD);  // the row is stored unrotated
                 }
               }
+              // the row's vectors, at most two a lane (8 heads of 128 bytes), loaded
+              // before the first store
+              const int n_vec = int(rb / 16);
+              uint4 vx[2];
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                if (lane + 32 * u < n_vec) vx[u] = vs[lane + 32 * u];
               if (cs) {
                 // lane = (head, chunk j): dims 8j .. 8j + 7 (uint4 j of the head's
                 // row) pair with dims 32 + 8j .. (uint4 j + 4)
                 const int hh = lane >> 2, j = lane & 3;
                 if (hh < n_cons) {
-                  const uint4 lo = __ldg(ks + hh * 8 + j), hi = __ldg(ks + hh * 8 + j + 4);
+                  const uint4 lo = ks[hh * 8 + j], hi = ks[hh * 8 + j + 4];
                   const float4 c0 = __ldg(reinterpret_cast<const float4*>(cs + 8 * j));
                   const float4 c1 = __ldg(reinterpret_cast<const float4*>(cs + 8 * j + 4));
                   const float4 s0 = __ldg(reinterpret_cast<const float4*>(sn + 8 * j));
@@ -650,13 +659,18 @@ __global__ void __maxnreg__(DK_MAXNREG) decode_kernel(const __grid_constant__ CU
                   kd[hh * 8 + j] = make_uint4(ol[0], ol[1], ol[2], ol[3]);
                   kd[hh * 8 + j + 4] = make_uint4(oh[0], oh[1], oh[2], oh[3]);
                 }
-                for (int e = lane; e < int(rb / 16); e += 32) vd[e] = __ldg(vs + e);
               } else {
-                for (int e = lane; e < int(rb / 16); e += 32) {
-                  kd[e] = __ldg(ks + e);
-                  vd[e] = __ldg(vs + e);
-                }
+                uint4 kx[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                  if (lane + 32 * u < n_vec) kx[u] = ks[lane + 32 * u];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                  if (lane + 32 * u < n_vec) kd[lane + 32 * u] = kx[u];
               }
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                if (lane + 32 * u < n_vec) vd[lane + 32 * u] = vx[u];
               asm volatile("fence.proxy.async.global;" ::: "memory");
             }
           }

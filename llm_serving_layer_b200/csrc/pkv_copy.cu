@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256) append_kernel(char* __restrict__ k_slab,
     T buf[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i0 + 32 * u < n) buf[u] = __ldg(src + i0 + 32 * u);
+      if (i0 + 32 * u < n) buf[u] = __ldcg(src + i0 + 32 * u);  // not read-only: the launch before may write k
     if (slot < 0 || slot >= n_slots) {
       if (lane == 0 && kv == 0) flag(st, PKV_DEV_SLOT_OOB);
       return;

@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(512, 1) prefill_kernel(const __grid_constant__
       const int j = tw0 + r % TPW;
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (j < ql)
-        v = __ldg(reinterpret_cast<const uint4*>(qg + ((int64_t(q0) + j) * a.n_heads + kvh * G + r / TPW) * PF_D) + c);
+        v = reinterpret_cast<const uint4*>(qg + ((int64_t(q0) + j) * a.n_heads + kvh * G + r / TPW) * PF_D)[c];
       *reinterpret_cast<uint4*>(qs + r * 128 + ((c ^ (r & 7)) << 4)) = v;
     }
     __syncwarp();

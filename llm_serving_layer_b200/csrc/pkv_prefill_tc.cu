@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(NG == 1 ? TC_THREADS : 384, NG == 1 ? 2 : 1)
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
                                                        ((int64_t(q0) + (qok ? jq_sm : 0)) * a.n_heads + h * G + r_sm / TPT) * TC_D);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) qv[c] = qok ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+    for (int c = 0; c < 8; ++c) qv[c] = qok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
   }
   if (!early) check_pages();
   if (threadIdx.x == 0) {
