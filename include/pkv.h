@@ -214,11 +214,12 @@ typedef struct pkv_page_index {
  * and v[t]. q [n_tokens][n_heads][head_dim], k and v [n_tokens][n_kv_heads]
  * [head_dim] in the pool dtype (PKV_F16, PKV_BF16 or PKV_F32), each token's
  * row contiguous and token t's row at t * stride elements (so slices of a fused
- * projection are taken as they are); q_out contiguous. n_heads may be 0 (k and v
- * only). The first rotary_dim dims of each head are rotated, the rest copied:
- * pair (i, i + rotary_dim / 2), or (2i, 2i + 1) when `interleaved`, by the
- * angle whose cosine / sine are rope_cos / rope_sin[positions[t]][i] (fp32
- * [rope_max_pos][rotary_dim / 2]); rounding as pkv_rope, so the bits are those
+ * projection are taken as they are); q_out contiguous: q itself, or memory that
+ * meets none of q, k and v. n_heads may be 0 (k and v only). The first rotary_dim
+ * dims of each head are rotated, the rest copied: pair (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) when `interleaved`, by the angle whose cosine / sine are
+ * rope_cos / rope_sin[positions[t]][i] (fp32 [rope_max_pos][rotary_dim / 2]);
+ * rounding as pkv_rope, so the bits are those
  * of pkv_rope followed by pkv_append_kv. With `index` non-NULL the pages whose
  * last slot the step fills are indexed (a second launch). A position outside
  * the tables leaves its token unrotated (PKV_DEV_META_BAD), a slot outside the

@@ -308,7 +308,8 @@ class B200PagedBackend:
         """Rotates q ``(T, n_heads, head_dim)`` and k ``(T, n_kv_heads, head_dim)``
         at ``meta.positions`` and appends the rotated k and v at
         ``meta.slot_mapping``, in one launch for any step; returns the rotated q
-        (``q_out`` or a new tensor; None when q is None). q, k and v may be
+        (``q_out``, which may be q itself but not overlap k or v, or a new
+        tensor; None when q is None). q, k and v may be
         slices of the fused projection: any stride between tokens, each token's
         heads contiguous (other layouts are copied first).
 
@@ -369,6 +370,8 @@ class B200PagedBackend:
                 raise ValueError(f"q_out must be a contiguous {tuple(q.shape)} {dt} tensor on {self.device}")
             elif _overlap(q_out, q) and not (q_out.data_ptr() == q.data_ptr() and q.is_contiguous()):
                 raise ValueError("q_out overlaps q without being q")
+            elif _overlap(q_out, k) or _overlap(q_out, v):
+                raise ValueError("q_out overlaps k or v (a row may be read after q_out has been written)")
             q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out given without q")

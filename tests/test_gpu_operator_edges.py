@@ -105,3 +105,26 @@ def test_a_chain_of_launches_reads_what_was_just_written(attention):
     want = run(True)
     for _ in range(3):
         assert torch.equal(run(False), want)
+
+
+# ---------------------------------------------------------------- rope_append
+def test_q_out_over_k_or_v_is_refused():
+    """k or v may be read after a row of q_out has been written."""
+    bk = B200PagedBackend(1, 8, 16, 2, 2, 64, device=DEV)
+    meta = build_meta([[0, 1]], [20], [20], 16, device=DEV)
+    rope = (torch.ones(32, 32, device=DEV), torch.zeros(32, 32, device=DEV))
+    q, k, v = (torch.randn(20, 2, 64, device=DEV).half() for _ in range(3))
+    for kw in (dict(k=k, v=v, q_out=k), dict(k=k, v=v, q_out=v)):
+        with pytest.raises(ValueError, match="overlaps"):
+            bk.rope_append(0, q, kw["k"], kw["v"], meta, rope, q_out=kw["q_out"])
+    flat = torch.zeros(2 * q.numel() - 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):  # k's last head is q_out's first
+        bk.rope_append(0, q, flat[:q.numel()].view(q.shape), v, meta, rope, q_out=flat[-q.numel():].view(q.shape))
+    qkv = torch.cat([q.flatten(1), k.flatten(1), v.flatten(1)], 1)
+    qs, ks, vs = (x.unflatten(1, (-1, 64)) for x in qkv.split([128, 128, 128], 1))
+    fits = torch.zeros(3 * q.numel(), dtype=torch.float16, device=DEV)  # neighbours that do not meet
+    for args, out in (((qs, ks, vs), fits[:q.numel()].view(q.shape)), ((q, k, v), q)):
+        got = bk.rope_append(0, *args, meta, rope, q_out=out)
+        assert got is out
+        slots = meta.slot_mapping.long()
+        assert torch.equal(bk.k_pool[0].flatten(0, 1)[slots], k) and torch.equal(bk.v_pool[0].flatten(0, 1)[slots], v)
