@@ -157,7 +157,7 @@ struct PlanArgs {
   ShItem* items;
   int2* desc;      // listed page {block, index of its sequence in the list << 7 | first << 6 | last << 5 | tokens}
   int4* fold;      // a row's pieces over the shared keys {first piece row, pieces, stride}
-  int4* rest;      // ... over its own
+  int4* rest;      // ... over its own; {0, 0, 0, 1}: the tiles write the row; {0, 0, 0, 0}: nobody does
 };
 
 struct SeqInfo {
@@ -410,6 +410,8 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     if (x.base >= 0) {
       int4* to = x.causal ? a.rest : a.fold;
       for (int k = lane; k < x.nt; k += 32) to[x.t0 + k] = make_int4(x.base + k, x.splits, x.nt, 0);
+    } else {  // no pieces: the tiles write these rows
+      for (int k = lane; k < x.nt; k += 32) a.rest[x.t0 + k] = make_int4(0, 0, 0, 1);
     }
   }
   __syncthreads();
@@ -1209,7 +1211,11 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const int4* fold, con
   const int4 b = __ldcg(rest + t);  // the plan's: complete before any kernel of the step started
   const int4 f = __ldcg(fold + t);
   pdl_wait();
-  if (b.y <= 0) return;  // written straight to out, or its tables are inconsistent
+  uint32_t* row = reinterpret_cast<uint32_t*>(static_cast<T*>(out) + (int64_t(t) * n_heads + hh) * TC_D) + lane;
+  if (b.y <= 0) {
+    if (b.w == 0) *row = 0u;  // its sequence's tables are inconsistent: zeros
+    return;
+  }
   const int n = f.y + b.y;
   constexpr int U = 8;
   float M = -1e30f, L = 0.f, y0 = 0.f, y1 = 0.f;
@@ -1234,8 +1240,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const int4* fold, con
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  reinterpret_cast<uint32_t*>(static_cast<T*>(out) + (int64_t(t) * n_heads + hh) * TC_D)[lane] =
-      MmaOp<T>::pack(y0 * inv, y1 * inv);
+  *row = MmaOp<T>::pack(y0 * inv, y1 * inv);
 }
 
 // ---------------------------------------------------------------- host

@@ -128,3 +128,30 @@ def test_q_out_over_k_or_v_is_refused():
         assert got is out
         slots = meta.slot_mapping.long()
         assert torch.equal(bk.k_pool[0].flatten(0, 1)[slots], k) and torch.equal(bk.v_pool[0].flatten(0, 1)[slots], v)
+
+
+# ---------------------------------------------------------------- shared-prefix attention
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (4, 4)])
+def test_rows_of_inconsistent_tables_are_zeros(hq, hkv):
+    """Every row of out is written: zeros where the sequence's tables are refused, the others' results as ever."""
+    fam = [(4, [(20, 1), (9, 3)]), (0, [(40, 5), (8, 1)]), (0, [(30, 2)]), (3, [(7, 1), (1, 1)])]
+    bk, meta, q, shared, tables = sh.build(fam, hq, hkv, validate="device")
+    want = sh.attend64(bk, meta, q, tables, 0.125)
+    row_of = meta.batch_indices
+    for bad in ([0], [1], [2, 3], [4], [5, 6], list(range(7))):
+        kl = meta.kv_lens.clone()
+        kl[bad] += 16
+        out = torch.full_like(q, float("nan"))
+        bk.attend_shared(q, 0, 0.125, bk.plan_shared(dataclasses.replace(meta, kv_lens=kl), shared), out=out)
+        with pytest.raises(PkvError, match="inconsistent"):
+            bk.check_status()
+        refused = torch.isin(row_of, torch.tensor(bad, dtype=row_of.dtype, device=DEV))
+        assert not out[refused].any()
+        sh.close(out, torch.where(refused[:, None, None], 0.0, want), bk)
+    # the step's own sums disagree: nothing is computed
+    out = torch.full_like(q, float("nan"))
+    bk.attend_shared(q, 0, 0.125, bk.plan_shared(dataclasses.replace(meta, cu_query_lens=meta.cu_query_lens + 1), shared),
+                     out=out)
+    with pytest.raises(PkvError, match="inconsistent"):
+        bk.check_status()
+    assert not out.any()
