@@ -280,12 +280,16 @@ PKV_API int pkv_attend_sparse(const pkv_pool* pool, const pkv_page_index* index,
  * are zeros. The plan is made once per step and reused by every layer with the
  * same batch and workspace (device, 256-byte aligned, of
  * pkv_shared_workspace_size bytes). Two launches per layer. Geometry of the
- * decode kernel only (PKV_ERR_UNSUPPORTED otherwise: use pkv_attend). */
+ * decode kernel only (PKV_ERR_UNSUPPORTED, and a workspace size of 0, otherwise:
+ * use pkv_attend). pkv_check_shared makes the plan's check of the groups alone,
+ * for any geometry: PKV_DEV_META_BAD where page lists disagree. */
 PKV_API size_t pkv_shared_workspace_size(const pkv_pool* pool, int32_t n_heads, int32_t n_seqs, int32_t n_tokens,
                                          int64_t total_pages);
 PKV_API int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* batch, int32_t n_groups,
                             const int32_t* group_indptr, const int32_t* prefix_pages, void* workspace,
                             size_t workspace_bytes, void* stream);
+PKV_API int pkv_check_shared(const pkv_pool* pool, const pkv_batch* batch, int32_t n_groups,
+                             const int32_t* group_indptr, const int32_t* prefix_pages, void* stream);
 PKV_API int pkv_attend_shared_planned(const pkv_pool* pool, int32_t layer, int32_t n_heads, const void* q, void* out,
                                       float scale, const pkv_batch* batch, void* workspace, size_t workspace_bytes,
                                       void* stream);

@@ -87,6 +87,7 @@ SIGNATURES = {
                                   P_BATCH, c_vp, c_i32, c_i32, c_vp]),
     "pkv_shared_workspace_size": (c_size, [P_POOL, c_i32, c_i32, c_i32, c_i64]),
     "pkv_plan_shared": (c_i32, [P_POOL, c_i32, P_BATCH, c_i32, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "pkv_check_shared": (c_i32, [P_POOL, P_BATCH, c_i32, c_vp, c_vp, c_vp]),
     "pkv_attend_shared_planned": (c_i32, [P_POOL, c_i32, c_i32, c_vp, c_vp, c_float, P_BATCH, c_vp, c_size, c_vp]),
     "pkv_attend_decode_noalloc": (c_i32, [P_POOL, c_i32, c_i32, c_vp, c_vp, c_float, P_BATCH, c_vp]),
     "pkv_wait_probe": (c_i32, [c_vp, c_vp, c_vp, c_vp]),

@@ -20,6 +20,7 @@ torch or CPU fallback, and construction fails on a non-CUDA device.
 from __future__ import annotations
 
 import ctypes
+from types import SimpleNamespace
 from typing import Any, Sequence
 
 import torch
@@ -505,8 +506,9 @@ class B200PagedBackend:
         plan = SharedPlan()
         self._plan_batch(plan, meta)
         plan.meta = None
+        seen = None
         if self.validate == "host":
-            self._host_validate(meta, n, int(meta.kv_indices.shape[0]))
+            seen = self._host_validate(meta, n, int(meta.kv_indices.shape[0]))
             self._validate_shared(meta, shared)
         bounds = [0]
         for size in shared.group_sizes:
@@ -515,17 +517,40 @@ class B200PagedBackend:
         plan.tensors["groups"] = groups
         b = plan.batch
         need = int(self._lib.pkv_shared_workspace_size(self._pdesc, self.n_heads, n, plan.n_tokens, b.total_pages))
+        if need == 0:  # other geometries: every sequence by itself, in attend
+            if self.validate == "device":
+                N.check(self._lib.pkv_check_shared(
+                    self._pdesc, plan.batch_ref, len(shared.group_sizes), groups.data_ptr(),
+                    groups.data_ptr() + 4 * len(bounds), N.stream_ptr(self.device)), "plan_shared")
+            plan.meta = self._plan_meta(plan, meta, seen)
+            plan.workspace, plan.ws_ptr, plan.ws_bytes = None, None, 0
+            return plan
         if workspace is None or workspace.numel() < need or workspace.device != self.device:
             workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
         plan.workspace, plan.ws_ptr, plan.ws_bytes = workspace, workspace.data_ptr(), workspace.numel()
-        rc = self._lib.pkv_plan_shared(
+        N.check(self._lib.pkv_plan_shared(
             self._pdesc, self.n_heads, plan.batch_ref, len(shared.group_sizes), groups.data_ptr(),
-            groups.data_ptr() + 4 * len(bounds), plan.ws_ptr, plan.ws_bytes, N.stream_ptr(self.device))
-        if rc == N.PKV_ERR_UNSUPPORTED:  # other geometries: every sequence by itself, in attend
-            plan.meta, plan.workspace, plan.ws_ptr, plan.ws_bytes = meta, None, None, 0
-            return plan
-        N.check(rc, "plan_shared")
+            groups.data_ptr() + 4 * len(bounds), plan.ws_ptr, plan.ws_bytes, N.stream_ptr(self.device)), "plan_shared")
         return plan
+
+    def _plan_meta(self, plan: SharedPlan, meta: Any, seen: tuple[bool, int] | None) -> SimpleNamespace:
+        """What ``attend`` reads of a step, made of the plan's own tables: an
+        object that no other step has (``attend`` knows its steps by identity).
+        ``seen``: the result of the host validation that was made, if any."""
+        t = plan.tensors
+        own = SimpleNamespace(
+            query_lens=t["cu"][1:] - t["cu"][:-1], cu_query_lens=t["cu"], kv_lens=t["kl"], kv_indptr=t["ip"],
+            kv_indices=t["ix"], kv_last_page_len=t["lp"], slot_mapping=None,
+            positions=torch.empty(plan.n_tokens, dtype=torch.int64, device="meta"))  # counted, not read
+        if seen is not None:
+            decode, hint = seen
+            own.is_prefill, own.max_query_len, own.min_query_len = not decode, 1 if decode else 2, 2 if hint == 2 else 1
+            own.checked_blocks = self.num_blocks
+            return own
+        for name in ("is_prefill", "max_query_len", "min_query_len"):
+            if hasattr(meta, name):
+                setattr(own, name, getattr(meta, name))
+        return own
 
     def attend_shared(self, q: torch.Tensor, layer_idx: int, scale: float, plan: SharedPlan, *,
                       out: torch.Tensor | None = None) -> torch.Tensor:

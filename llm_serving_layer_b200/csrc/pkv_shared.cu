@@ -146,7 +146,7 @@ struct PlanArgs {
   const int32_t* prefix_pages;  // [n_groups]
   int32_t* st;
   int64_t num_blocks, total_pages;
-  int n_seqs, n_tokens, n_groups, n_kv, tpt, sms, splits_cap, grid;
+  int n_seqs, n_tokens, n_groups, page, n_kv, tpt, sms, splits_cap, grid;  // page: TC_P but for the check alone
   int64_t pieces_cap, items_cap;
   ShCtl* ctl;
   int32_t* rows;   // row of each listed one-token sequence
@@ -173,9 +173,9 @@ __device__ __forceinline__ SeqInfo seq_info(const PlanArgs& a, int s) {
   r.lpl = a.last_page_len[s];
   r.pa = int(pa);
   r.pages = int(pb - pa);
-  r.kv = (pb - pa - 1) * TC_P + r.lpl;
+  r.kv = (pb - pa - 1) * a.page + r.lpl;
   r.ok = r.q0 >= 0 && r.ql >= 1 && int64_t(r.q0) + r.ql <= a.n_tokens && pa >= 0 && pb > pa && pb <= a.total_pages &&
-         r.lpl >= 1 && r.lpl <= TC_P && r.kv >= r.ql && r.kv < 0x7fffffff && (!a.kv_lens || a.kv_lens[s] == r.kv);
+         r.lpl >= 1 && r.lpl <= a.page && r.kv >= r.ql && r.kv < 0x7fffffff && (!a.kv_lens || a.kv_lens[s] == r.kv);
   return r;
 }
 // group of sequence s: the last g with group_indptr[g] <= s
@@ -202,7 +202,7 @@ __device__ __forceinline__ int stream_least(const PlanArgs& a, int listed, float
 
 // One CTA per sequence: do its leading pages agree with its group's first
 // sequence's, and do its new tokens lie after them? If not the group is marked
-// (and flagged) and computed without sharing.
+// (where there are marks) and flagged, and computed without sharing.
 __global__ void __launch_bounds__(128) shared_check_kernel(const PlanArgs a) {
   const int s = blockIdx.x;
   const int g = group_of(a, s);
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(128) shared_check_kernel(const PlanArgs a) {
   bool bad = f < 0 || s < f || s >= e || e > a.n_seqs || np < 0;
   if (!bad && np > 0) {
     const SeqInfo x = seq_info(a, s), y = seq_info(a, f);
-    bad = !x.ok || !y.ok || int64_t(np) * TC_P > x.kv - x.ql || np > y.pages;
+    bad = !x.ok || !y.ok || int64_t(np) * a.page > x.kv - x.ql || np > y.pages;
     if (!bad)
       for (int i = threadIdx.x; i < np; i += blockDim.x) {
         const int id = a.kv_indices[x.pa + i];
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(128) shared_check_kernel(const PlanArgs a) {
   }
   if (bad) {
     flag(a.st, PKV_DEV_META_BAD);
-    if (g >= 0 && g < a.n_groups) a.group_bad[g] = 1;
+    if (a.group_bad && g >= 0 && g < a.n_groups) a.group_bad[g] = 1;
   }
 }
 
@@ -1244,22 +1244,59 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const int4* fold, con
 }
 
 // ---------------------------------------------------------------- host
-int check_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* b) {
-  if (int rc = check_pool(pool)) return rc;
+bool shared_geometry(const pkv_pool& p, int n_heads) {
+  const int g = n_heads / p.n_kv_heads;
+  return (p.dtype == PKV_F16 || p.dtype == PKV_BF16) && p.head_dim == TC_D && p.block_size == TC_P &&
+         p.n_kv_heads <= 8 && (g == 1 || g == 2 || g == 4 || g == 8);
+}
+
+int check_batch(const pkv_batch* b) {
   if (!b) return fail(PKV_ERR_ARG, "batch descriptor is NULL");
-  if (n_heads <= 0 || n_heads % pool->n_kv_heads)
-    return fail(PKV_ERR_ARG, "n_heads must be a positive multiple of n_kv_heads");
-  const int g = n_heads / pool->n_kv_heads;
-  if ((pool->dtype != PKV_F16 && pool->dtype != PKV_BF16) || pool->head_dim != TC_D || pool->block_size != TC_P ||
-      pool->n_kv_heads > 8 || (g != 1 && g != 2 && g != 4 && g != 8))
-    return fail(PKV_ERR_UNSUPPORTED, "shared-prefix attention takes fp16 / bf16 pools, head_dim 64, 16-token pages, "
-                                     "up to 8 KV heads and 1, 2, 4 or 8 query heads per KV head");
   if (b->n_seqs <= 0) return fail(PKV_ERR_ARG, "batch has no sequences");
   if (b->n_tokens < 0 || b->total_pages < 0 || b->total_pages >= (int64_t(1) << 31) || b->n_seqs >= (1 << 24))
     return fail(PKV_ERR_ARG, "bad batch sizes");
   if (!b->cu_query_lens || !b->kv_indptr || !b->kv_last_page_len || (b->total_pages && !b->kv_indices))
     return fail(PKV_ERR_ARG, "batch CSR pointers must be non-NULL");
   return PKV_OK;
+}
+
+int check_shared(const pkv_pool* pool, int32_t n_heads, const pkv_batch* b) {
+  if (int rc = check_pool(pool)) return rc;
+  if (!b) return fail(PKV_ERR_ARG, "batch descriptor is NULL");
+  if (n_heads <= 0 || n_heads % pool->n_kv_heads)
+    return fail(PKV_ERR_ARG, "n_heads must be a positive multiple of n_kv_heads");
+  if (!shared_geometry(*pool, n_heads))
+    return fail(PKV_ERR_UNSUPPORTED, "shared-prefix attention takes fp16 / bf16 pools, head_dim 64, 16-token pages, "
+                                     "up to 8 KV heads and 1, 2, 4 or 8 query heads per KV head");
+  return check_batch(b);
+}
+
+int check_groups(const pkv_batch& b, int32_t n_groups, const int32_t* group_indptr, const int32_t* prefix_pages) {
+  if (n_groups <= 0 || n_groups > b.n_seqs)
+    return fail(PKV_ERR_ARG, "n_groups must be between 1 and the number of sequences");
+  if (!group_indptr || !prefix_pages) return fail(PKV_ERR_ARG, "group_indptr and prefix_pages must be non-NULL");
+  return PKV_OK;
+}
+
+// The step's part of the plan's arguments: what shared_check_kernel reads.
+PlanArgs step_args(const pkv_pool& p, const pkv_batch& b, int32_t n_groups, const int32_t* group_indptr,
+                   const int32_t* prefix_pages) {
+  PlanArgs a{};
+  a.cu_q = b.cu_query_lens;
+  a.kv_lens = b.kv_lens;
+  a.kv_indptr = b.kv_indptr;
+  a.kv_indices = b.kv_indices;
+  a.last_page_len = b.kv_last_page_len;
+  a.group_indptr = group_indptr;
+  a.prefix_pages = prefix_pages;
+  a.st = b.dev_status;
+  a.num_blocks = p.num_blocks;
+  a.total_pages = b.total_pages;
+  a.n_seqs = b.n_seqs;
+  a.n_tokens = b.n_tokens;
+  a.n_groups = n_groups;
+  a.page = p.block_size;
+  return a;
 }
 
 template <typename T, int G>
@@ -1303,7 +1340,8 @@ using namespace pkv;
 
 extern "C" size_t pkv_shared_workspace_size(const pkv_pool* pool, int32_t n_heads, int32_t n_seqs, int32_t n_tokens,
                                             int64_t total_pages) {
-  if (!pool || pool->n_kv_heads <= 0 || n_heads < pool->n_kv_heads || n_seqs <= 0 || n_tokens < 0 || total_pages < 0)
+  if (!pool || pool->n_kv_heads <= 0 || n_heads < pool->n_kv_heads || n_seqs <= 0 || n_tokens < 0 || total_pages < 0 ||
+      !shared_geometry(*pool, n_heads))
     return 0;
   return sh_layout(n_heads, pool->n_kv_heads, n_seqs, n_tokens, total_pages).total;
 }
@@ -1312,29 +1350,14 @@ extern "C" int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_
                                const int32_t* group_indptr, const int32_t* prefix_pages, void* workspace,
                                size_t workspace_bytes, void* stream) {
   if (int rc = check_shared(pool, n_heads, batch)) return rc;
-  if (n_groups <= 0 || n_groups > batch->n_seqs)
-    return fail(PKV_ERR_ARG, "n_groups must be between 1 and the number of sequences");
-  if (!group_indptr || !prefix_pages) return fail(PKV_ERR_ARG, "group_indptr and prefix_pages must be non-NULL");
+  if (int rc = check_groups(*batch, n_groups, group_indptr, prefix_pages)) return rc;
   const int groups = n_heads / pool->n_kv_heads;
   const ShLayout w = sh_layout(n_heads, pool->n_kv_heads, batch->n_seqs, batch->n_tokens, batch->total_pages);
   if (!workspace || workspace_bytes < w.total)
     return fail(PKV_ERR_ARG, "workspace too small: need " + std::to_string(w.total) + " bytes");
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(PKV_ERR_ARG, "workspace must be 256-byte aligned");
   char* ws = static_cast<char*>(workspace);
-  PlanArgs a;
-  a.cu_q = batch->cu_query_lens;
-  a.kv_lens = batch->kv_lens;
-  a.kv_indptr = batch->kv_indptr;
-  a.kv_indices = batch->kv_indices;
-  a.last_page_len = batch->kv_last_page_len;
-  a.group_indptr = group_indptr;
-  a.prefix_pages = prefix_pages;
-  a.st = batch->dev_status;
-  a.num_blocks = pool->num_blocks;
-  a.total_pages = batch->total_pages;
-  a.n_seqs = batch->n_seqs;
-  a.n_tokens = batch->n_tokens;
-  a.n_groups = n_groups;
+  PlanArgs a = step_args(*pool, *batch, n_groups, group_indptr, prefix_pages);
   a.n_kv = pool->n_kv_heads;
   a.tpt = TC_ROWS / groups;
   a.sms = num_sms();
@@ -1357,6 +1380,17 @@ extern "C" int pkv_plan_shared(const pkv_pool* pool, int32_t n_heads, const pkv_
   shared_check_kernel<<<unsigned(batch->n_seqs), 128, 0, s>>>(a);
   PKV_CUDA_RET(cudaGetLastError());
   shared_plan_kernel<<<1, 1024, 0, s>>>(a);
+  PKV_CUDA_RET(cudaGetLastError());
+  return PKV_OK;
+}
+
+extern "C" int pkv_check_shared(const pkv_pool* pool, const pkv_batch* batch, int32_t n_groups,
+                                const int32_t* group_indptr, const int32_t* prefix_pages, void* stream) {
+  if (int rc = check_pool(pool)) return rc;
+  if (int rc = check_batch(batch)) return rc;
+  if (int rc = check_groups(*batch, n_groups, group_indptr, prefix_pages)) return rc;
+  shared_check_kernel<<<unsigned(batch->n_seqs), 128, 0, static_cast<cudaStream_t>(stream)>>>(
+      step_args(*pool, *batch, n_groups, group_indptr, prefix_pages));
   PKV_CUDA_RET(cudaGetLastError());
   return PKV_OK;
 }

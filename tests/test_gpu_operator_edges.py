@@ -155,3 +155,37 @@ def test_rows_of_inconsistent_tables_are_zeros(hq, hkv):
     with pytest.raises(PkvError, match="inconsistent"):
         bk.check_status()
     assert not out.any()
+
+
+@pytest.mark.parametrize("where", [DEV, "cpu"])
+@pytest.mark.parametrize("validate", ["host", "device"])
+def test_plans_without_the_kernel_hold_their_tables(validate, where):
+    """head_dim 32: a plan keeps its step when ``meta`` is overwritten in place, and the next plan sees the new one."""
+    bk, meta, q, shared, tables = sh.build([(0, [(100, 1), (70, 5), (33, 1)])], 6, 2, validate=validate, d=32)
+    meta = build_meta(tables, [100, 70, 33], [1, 5, 1], 16, device=where)
+    first = bk.plan_shared(meta, shared)
+    want = sh.attend64(bk, meta, q, tables, 0.2)
+    sh.close(bk.attend_shared(q, 0, 0.2, first), want, bk)
+    assert first.workspace is None
+    other = [tables[0], tables[1], tables[0][:3]]  # the third sequence takes over pages of the first
+    changed = build_meta(other, [99, 70, 48], [1, 5, 1], 16, device=where)
+    for f in ("kv_lens", "positions", "kv_indptr", "kv_indices", "kv_last_page_len"):
+        getattr(meta, f).copy_(getattr(changed, f))
+    second = bk.plan_shared(meta, shared)
+    sh.close(bk.attend_shared(q, 0, 0.2, second), sh.attend64(bk, meta, q, other, 0.2), bk)
+    sh.close(bk.attend_shared(q, 0, 0.2, first), want, bk)
+    bk.check_status()
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(32, 6, 2), (64, 6, 2), (128, 4, 4)])
+@pytest.mark.parametrize("claim", ["other pages", "past the new tokens", "more pages than there are"])
+def test_wrong_claims_without_the_kernel(claim, d, hq, hkv):
+    fam = [(4, [(20, 1), (9, 1)]), (3, [(40, 5), (8, 1)])]
+    pages = {"other pages": [5, 3], "past the new tokens": [4, 5], "more pages than there are": [4, 50]}[claim]
+    bk, meta, q, shared, tables = sh.build(fam, hq, hkv, validate="device", d=d)
+    out = bk.attend_shared(q, 0, 0.2, bk.plan_shared(meta, SharedPrefix([2, 2], pages)))
+    with pytest.raises(PkvError, match="inconsistent"):
+        bk.check_status()
+    sh.close(out, sh.attend64(bk, meta, q, tables, 0.2), bk)
+    bk.plan_shared(meta, shared)
+    bk.check_status()

@@ -133,3 +133,14 @@ def test_shared_refusals(lib):
                    (dict(p=pool(d=128)), 2)):
         assert attend(**kw) == rc, kw
     assert attend(b=batch(t=0)) == N.PKV_OK
+
+
+def test_shared_check_refusals(lib):
+    def check(p=pool(d=128), b=batch(), groups=1, gi=0x1000, pp=0x1000):
+        return lib.pkv_check_shared(p, b, groups, gi, pp, None)
+
+    for kw in (dict(p=None), dict(b=None), dict(b=batch(n=0)), dict(b=batch(t=-1)), dict(b=batch(cu=None)),
+               dict(b=batch(ix=None)), dict(groups=0), dict(groups=3), dict(gi=None), dict(pp=None)):
+        assert check(**kw) == N.PKV_ERR_ARG, kw
+    for p, hq in ((pool(d=128), 32), (pool(page=32), 32), (pool(dtype=2), 32), (pool(), 24), (pool(n_kv=9), 36)):
+        assert lib.pkv_shared_workspace_size(p, hq, 2, 2, 4) == 0  # geometries that attend serves
