@@ -1128,7 +1128,7 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
       tc_fence_after();
       const int h = s_item[sl].h, t0 = s_item[sl].t0, piece = s_item[sl].piece;
       const bool zero = s_item[sl].zero != 0;
-      const float inv = (l > 0.f && !zero) ? 1.f / l : 0.f;  // rows that saw nothing, or a bad page: zeros
+      const float inv = (l == 0.f || zero) ? 0.f : 1.f / l;  // rows that saw nothing, or a bad page: zeros (not a NaN sum)
       if (piece >= 0 && r / G < nt)
         __stcg(a.part_ml + int64_t(piece + r / G) * a.n_heads + h * G + r % G,
                make_float2(m == -INFINITY || zero ? -1e30f : m, zero ? 0.f : l));

@@ -189,3 +189,16 @@ def test_wrong_claims_without_the_kernel(claim, d, hq, hkv):
     sh.close(out, sh.attend64(bk, meta, q, tables, 0.2), bk)
     bk.plan_shared(meta, shared)
     bk.check_status()
+
+
+@pytest.mark.parametrize("pages", [0, 2])
+def test_queries_that_are_not_numbers_give_no_numbers(pages):
+    """A NaN in one query row reaches that row of out, and no other, shared or not."""
+    bk, meta, q, shared, tables = sh.build([(pages, [(40, 5), (30, 1), (9, 2)])], 8, 2)
+    q[1, 3, 7] = q[5, 0, 0] = q[6, 7, 63] = float("nan")
+    out = bk.attend_shared(q, 0, 0.125, bk.plan_shared(meta, shared))
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device=DEV)
+    bad[1, 3] = bad[5, 0] = bad[6, 7] = True
+    assert bool(torch.isnan(out[bad]).all())
+    want = sh.attend64(bk, meta, torch.where(bad[..., None], 0, q), tables, 0.125)
+    sh.close(torch.where(bad[..., None], want.to(q.dtype), out), want, bk)
