@@ -202,8 +202,10 @@ PKV_API int pkv_append_attend_rope_planned(const pkv_pool* pool, int32_t layer, 
  * block_size keys and scale = max(|lo|, |hi|) * (1/127) (fp32 product),
  *   codes[layer][block][kv head][0][d] = floor(lo / scale)
  *   codes[layer][block][kv head][1][d] = ceil(hi / scale)
- * clamped to [-127, 127] (0 where scale is 0). Only entries of completed pages
- * are meaningful. */
+ * clamped to [-127, 127] (0 where scale is 0). A key that is no number makes
+ * scale NaN and the codes 0; an infinite one makes scale infinite, the codes of
+ * infinite bounds +-127 and the others 0. Only entries of completed pages are
+ * meaningful. */
 typedef struct pkv_page_index {
   int8_t* codes;  /* device [num_layers][num_blocks][n_kv_heads][2][head_dim], 16-byte aligned */
   float* scales;  /* device [num_layers][num_blocks][n_kv_heads] */
@@ -245,7 +247,8 @@ PKV_API int pkv_page_index_rebuild(const pkv_pool* pool, const pkv_page_index* i
  * PKV_SPARSE_SELECT the pages are chosen and written to pages[n_tokens]
  * [n_kv_heads][budget] (page numbers within the sequence, ascending, -1 past
  * the end): the first `sink` pages, the last `recent` (the query's own page and
- * those before it), then the pages of highest score, ties to the lower page:
+ * those before it), then the pages of highest score, ties to the lower page, a
+ * score that is no number above every number:
  *   qs_g = max_d |q_gd| * (1/127), q8_g = round-half-even(q_g / qs_g)
  *   I_g = sum_d max(q8_gd * codes[0][d], q8_gd * codes[1][d])
  *   score = (max over the KV head's query heads g of fl(I_g * qs_g)) * scale

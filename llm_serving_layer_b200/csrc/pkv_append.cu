@@ -13,6 +13,10 @@
 //   page_index_kernel    bounds of whole pages: lo / hi = elementwise min / max
 //                        of the page's keys, scale = max(|lo|, |hi|) / 127,
 //                        codes floor(lo / scale), ceil(hi / scale).
+//                        A NaN key makes the scale NaN (and the codes 0), so that
+//                        its page scores no number, above every number; an
+//                        infinite one makes it infinite: +-127 for infinite
+//                        bounds, 0 for the others.
 //
 // Both move each byte once and do a few operations on it: HBM bound. 16384 tokens
 // of 32 + 8 + 8 heads of 64 (fp16, 203 MB): 36 us = 5.6 TB/s (0.87 of the copy
@@ -67,26 +71,26 @@ __device__ __forceinline__ uint4 pack_vec(const float (&f)[16 / sizeof(T)]) {
 template <typename T>
 __device__ __forceinline__ uint32_t min_word(uint32_t a, uint32_t b) {
   if constexpr (sizeof(T) == 4) {
-    return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b)));
+    return __float_as_uint(fmin_nan(__uint_as_float(a), __uint_as_float(b)));
   } else if constexpr (std::is_same<T, __half>::value) {
-    const __half2 m = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    const __half2 m = __hmin2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&m);
   } else {
     const __nv_bfloat162 m =
-        __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&m);
   }
 }
 template <typename T>
 __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
   if constexpr (sizeof(T) == 4) {
-    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    return __float_as_uint(fmax_nan(__uint_as_float(a), __uint_as_float(b)));
   } else if constexpr (std::is_same<T, __half>::value) {
-    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&m);
   } else {
     const __nv_bfloat162 m =
-        __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&m);
   }
 }
@@ -110,14 +114,17 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int w) {
 template <typename T>
 __device__ __forceinline__ float top_of_word(uint32_t lo, uint32_t hi) {
   if constexpr (sizeof(T) == 4) {
-    return fmaxf(fabsf(__uint_as_float(lo)), fabsf(__uint_as_float(hi)));
+    return fmax_nan(fabsf(__uint_as_float(lo)), fabsf(__uint_as_float(hi)));
   } else {
     const float2 a = unpack2<T>(lo), b = unpack2<T>(hi);
-    return fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y)));
+    return fmax_nan(fmax_nan(fabsf(a.x), fabsf(a.y)), fmax_nan(fabsf(b.x), fabsf(b.y)));
   }
 }
+// An infinite bound (its scale is infinite too: the finite ones' codes are 0) is
+// the extreme code of its sign; a scale of 0 or NaN gives 0.
 __device__ __forceinline__ int8_t code_of(float x, float scale, bool up) {
-  const float y = scale > 0.f ? (up ? ceilf(__fdiv_rn(x, scale)) : floorf(__fdiv_rn(x, scale))) : 0.f;
+  float y = scale > 0.f ? (up ? ceilf(__fdiv_rn(x, scale)) : floorf(__fdiv_rn(x, scale))) : 0.f;
+  if (fabsf(x) == INFINITY && scale > 0.f) y = x;
   return int8_t(fminf(fmaxf(y, -127.f), 127.f));
 }
 // Codes of a word of bounds: floor(lo / scale) at c, ceil(hi / scale) at c + d,
@@ -294,17 +301,17 @@ __device__ __forceinline__ void index_entry(const IndexArgs& a, int layer, int64
       const int e = lane + 32 * i;
       if (e < d) {
         const float x = to_f<T>(k[r * row + e]);
-        lo[i] = fminf(lo[i], x);
-        hi[i] = fmaxf(hi[i], x);
+        lo[i] = fmin_nan(lo[i], x);
+        hi[i] = fmax_nan(hi[i], x);
       }
     }
   }
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < IX_MAX_EPL; ++i)
-    if (lane + 32 * i < d) top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+    if (lane + 32 * i < d) top = fmax_nan(top, fmax_nan(fabsf(lo[i]), fabsf(hi[i])));
 #pragma unroll
-  for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  for (int off = 16; off; off >>= 1) top = fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
   const float scale = __fmul_rn(top, 1.0f / 127.0f);
   const int64_t entry = (int64_t(layer) * a.num_blocks + blk) * a.hkv + h;
   int8_t* c = a.codes + entry * 2 * d;
@@ -355,9 +362,9 @@ __device__ __forceinline__ void index_entry_vec(const IndexArgs& a, int layer, i
   // every lane of a column holds its bounds now: the RPI lanes share the vector's words
   float top = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, top_of_word<T>(word_of(mn, w), word_of(mx, w)));
+  for (int w = 0; w < 4; ++w) top = fmax_nan(top, top_of_word<T>(word_of(mn, w), word_of(mx, w)));
 #pragma unroll
-  for (int off = 1; off < LPR; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  for (int off = 1; off < LPR; off <<= 1) top = fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
   const float scale = __fmul_rn(top, 1.0f / 127.0f);
   const int64_t entry = (int64_t(layer) * a.num_blocks + blk) * a.hkv + h;
   int8_t* out = a.codes + entry * 2 * D + (lane % LPR) * VE;

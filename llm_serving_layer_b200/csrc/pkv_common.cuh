@@ -302,6 +302,18 @@ struct MmaOp<__nv_bfloat16> {
   }
 };
 
+// minimum / maximum of which a NaN operand is the result (fminf and fmaxf drop it)
+__device__ __forceinline__ float fmin_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // scalar conversions for the generic kernels
 template <typename T>
 __device__ __forceinline__ float to_f(T x);

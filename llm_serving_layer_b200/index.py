@@ -4,7 +4,9 @@ which page-sparse attention scores pages with (``B200PagedBackend.plan_sparse``)
 
 For a page whose keys have elementwise minimum ``lo`` and maximum ``hi``,
 ``scale = max(|lo|, |hi|) * (1/127)``, ``codes[0] = floor(lo / scale)`` and
-``codes[1] = ceil(hi / scale)``. An entry belongs to the physical block, so
+``codes[1] = ceil(hi / scale)``. A page with a key that is no number has a NaN
+scale and scores above every number; infinite bounds have an infinite scale and
+the codes -127 / 127. An entry belongs to the physical block, so
 sequences that share a page (radix prefix sharing) share its entry. Only entries
 of completed pages are read (a query's own page is always attended), so nothing
 is kept up to date token by token: ``rope_append(..., index=)`` or ``update``

@@ -202,3 +202,61 @@ def test_queries_that_are_not_numbers_give_no_numbers(pages):
     assert bool(torch.isnan(out[bad]).all())
     want = sh.attend64(bk, meta, torch.where(bad[..., None], 0, q), tables, 0.125)
     sh.close(torch.where(bad[..., None], want.to(q.dtype), out), want, bk)
+
+
+# ---------------------------------------------------------------- page index
+GEOMETRIES = [(torch.float16, 16, 64), (torch.bfloat16, 16, 64), (torch.float32, 16, 64), (torch.float16, 16, 128),
+              (torch.bfloat16, 32, 256), (torch.float32, 16, 128), (torch.float16, 5, 40), (torch.float32, 3, 33)]
+
+
+@pytest.mark.parametrize("dtype,page,d", GEOMETRIES)
+def test_index_of_keys_that_are_not_finite(dtype, page, d):
+    """An infinite key: an infinite scale, 127 with its sign where a bound is infinite, 0 elsewhere. A key that is
+    no number: neither is the scale, codes 0."""
+    bk = B200PagedBackend(1, 9, page, 2, 2, d, device=DEV, dtype=dtype)
+    k = bk.k_pool[0]
+    k.copy_(torch.randn(k.shape, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV))
+    inf, nan = float("inf"), float("nan")
+    k[1, 2, 0, 5] = inf
+    k[2, 0, 1, d - 1] = -inf
+    k[3, :, 0, 7], k[3, page - 1, 0, 0] = inf, -inf
+    k[4, :, 1, 9] = -inf
+    k[5, 1, 0, 3] = nan
+    k[6, page - 1, 1, d - 1], k[6, 0, 1, 0] = nan, inf
+    k[7, :, :, :] = nan
+    index = PageIndex(bk)
+    index.rebuild(range(9))
+    x = k.float().cpu().numpy()
+    lo, hi = x.min(1), x.max(1)  # a NaN is the minimum and the maximum
+    with np.errstate(invalid="ignore", divide="ignore"):
+        scale = np.maximum(abs(lo), abs(hi)).max(-1) * np.float32(1 / 127)
+        def code(b, up):
+            y = np.clip((np.ceil if up else np.floor)(b / scale[..., None]), -127, 127)
+            y = np.where(np.isinf(b), np.copysign(127, b), np.where(np.isinf(scale)[..., None], 0, y))
+            return np.where(scale[..., None] > 0, y, 0)
+        want = np.stack([code(lo, False), code(hi, True)], -2).astype(np.int8)
+    assert np.array_equal(index.scales[0].cpu().numpy(), scale, equal_nan=True)
+    assert np.array_equal(index.codes[0].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype,page,d", [(torch.float16, 16, 64), (torch.bfloat16, 16, 128), (torch.float32, 16, 64),
+                                          (torch.float16, 8, 64)])
+def test_pages_of_keys_that_are_not_finite(dtype, page, d):
+    """Order of the scores: no number, then the infinite bound that the query reaches, then finite ones, then the
+    bound of minus infinity; equal ones to the lower page."""
+    bk, index, seqs, meta, q = sp.build([(page * 40, 1)], page, 2, 1, d, dtype)
+    ids = seqs[0].block_ids
+    q.copy_(torch.randn(q.shape, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).abs() + 0.1)
+    k = bk.k_pool[0]
+    k[ids[30], 1, 0, 4] = float("inf")   # positive query: +inf
+    k[ids[10], 2, 0, 3] = float("inf")
+    k[ids[20], 0, 0, 8] = float("nan")
+    k[ids[25], 0, 0, 8] = float("-inf")  # 0 from that dim, 0 from the others: 0 * inf, no number
+    k[ids[5], :, 0, 2] = float("-inf")   # whatever the key: -inf
+    index.rebuild(ids)
+    def chosen(budget):
+        plan = bk.plan_sparse(meta, index, budget, sink=0, recent=1)
+        return bk.select_pages(q, 0, plan)[0, 0].tolist()
+    assert chosen(3) == [20, 25, 39]
+    assert chosen(5) == [10, 20, 25, 30, 39]
+    assert chosen(39) == [p for p in range(40) if p != 5]
