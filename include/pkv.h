@@ -248,7 +248,8 @@ PKV_API int pkv_page_index_rebuild(const pkv_pool* pool, const pkv_page_index* i
  * [n_kv_heads][budget] (page numbers within the sequence, ascending, -1 past
  * the end): the first `sink` pages, the last `recent` (the query's own page and
  * those before it), then the pages of highest score, ties to the lower page, a
- * score that is no number above every number:
+ * score that is no number above every number (every page's for a KV head with a
+ * query that is not finite):
  *   qs_g = max_d |q_gd| * (1/127), q8_g = round-half-even(q_g / qs_g)
  *   I_g = sum_d max(q8_gd * codes[0][d], q8_gd * codes[1][d])
  *   score = (max over the KV head's query heads g of fl(I_g * qs_g)) * scale

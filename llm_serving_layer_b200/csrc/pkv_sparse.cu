@@ -57,6 +57,12 @@ struct SparseArgs {
   float scale_log2;
 };
 
+// Scale of a query's codes from its largest magnitude: a query that is not finite
+// has a NaN scale and codes 0, so that its scores are no numbers, all equal.
+__device__ __forceinline__ float query_scale(float top) {
+  return top < INFINITY ? __fmul_rn(top, 1.0f / 127.0f) : __int_as_float(0x7fffffff);
+}
+
 // unsigned order = order of the scores; not a number above every number
 __device__ __forceinline__ uint32_t score_key(float x) {
   if (x != x) return 0xffffffffu;
@@ -112,10 +118,10 @@ __device__ __forceinline__ void quantise_query(const SparseArgs& a, const T* q, 
   for (int g = warp; g < a.groups; g += nw) {
     const T* x = q + int64_t(g) * a.d;
     float top = 0.f;
-    for (int e = lane; e < a.d; e += 32) top = fmaxf(top, fabsf(to_f<T>(x[e])));
+    for (int e = lane; e < a.d; e += 32) top = fmax_nan(top, fabsf(to_f<T>(x[e])));
 #pragma unroll
-    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float s = __fmul_rn(top, 1.0f / 127.0f);
+    for (int off = 16; off; off >>= 1) top = fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float s = query_scale(top);
     for (int e = lane; e < a.d; e += 32) {
       float y = s > 0.f ? rintf(__fdiv_rn(to_f<T>(x[e]), s)) : 0.f;
       y = fminf(fmaxf(y, -127.f), 127.f);
@@ -383,11 +389,11 @@ __global__ void __launch_bounds__(NW * 32, MINB) sparse_kernel(const SparseArgs 
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float2 x = unpack2<T>(qb[ks][e]);
-        top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+        top = fmax_nan(top, fmax_nan(fabsf(x.x), fabsf(x.y)));
       }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float q_scale = __fmul_rn(top, 1.0f / 127.0f);
+    top = fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float q_scale = query_scale(top);
     select_init(sel);
     if (cs > 1) cluster_arrive();  // waited for before the first remote store
 #pragma unroll
@@ -461,9 +467,9 @@ __global__ void __launch_bounds__(NW * 32, MINB) sparse_kernel(const SparseArgs 
           for (int r = 0; r < 2; ++r) {
             float m = -INFINITY;
             if (v0) m = __fmul_rn(float(acc[2 * r]), s0);
-            if (v1) m = fmaxf(m, __fmul_rn(float(acc[2 * r + 1]), s1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            if (v1) m = fmax_nan(m, __fmul_rn(float(acc[2 * r + 1]), s1));
+            m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
             // row g of (half, r) = page 16 half + 8 r + g: hand it to that lane
             const float mm = __shfl_sync(0xffffffffu, m, (lane & 7) * 4);
             if ((lane >> 3) == 2 * half + r) mykey = score_key(__fmul_rn(mm, bs[u]));
@@ -757,7 +763,7 @@ __global__ void __launch_bounds__(256) sparse_generic_kernel(const SparseArgs a)
             for (int e = lane; e < 2 * D; e += 32) dot += int(c[e]) * int(q8s[g * 2 * D + e]);
 #pragma unroll
             for (int off = 16; off; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-            best = fmaxf(best, __fmul_rn(float(dot), qs[g]));
+            best = fmax_nan(best, __fmul_rn(float(dot), qs[g]));
           }
           key = score_key(__fmul_rn(best, a.scales[id * a.n_kv + h]));
         }

@@ -260,3 +260,17 @@ def test_pages_of_keys_that_are_not_finite(dtype, page, d):
     assert chosen(3) == [20, 25, 39]
     assert chosen(5) == [10, 20, 25, 30, 39]
     assert chosen(39) == [p for p in range(40) if p != 5]
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype,page,hq,d", [(torch.float16, 16, 8, 64), (torch.bfloat16, 16, 2, 128),
+                                             (torch.float32, 16, 4, 64), (torch.float16, 16, 9, 64)])
+def test_queries_that_are_not_finite_choose_the_lowest_pages(dtype, page, hq, d, value):
+    """The scores of a KV head with such a query are no numbers: all equal. Other KV heads keep theirs."""
+    bk, index, seqs, meta, q = sp.build([(page * 60, 1), (page * 50, 1)], page, 2 * hq, 2, d, dtype)
+    plan = bk.plan_sparse(meta, index, 7, sink=1, recent=2)
+    before = bk.select_pages(q, 0, plan)
+    q[0, hq - 1, 5] = value
+    after = bk.select_pages(q, 0, plan)
+    assert after[0, 0].tolist() == [0, 1, 2, 3, 4, 58, 59]
+    assert torch.equal(after[0, 1], before[0, 1]) and torch.equal(after[1], before[1])
