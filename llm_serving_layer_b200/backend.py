@@ -124,6 +124,7 @@ class B200PagedBackend:
         self._pos_meta: Any = None  # the meta whose int64 device positions are cached in _pos
         self._pos: torch.Tensor | None = None
         self._ws: torch.Tensor | None = None
+        self._indexes: list[Any] = []  # weak references to the PageIndex objects of this pool
         # per-step state, keyed by BatchMeta identity (a strong reference keeps
         # the id from being recycled while it is cached)
         self._meta: Any = None
@@ -170,6 +171,8 @@ class B200PagedBackend:
             return
         N.check(self._lib.pkv_copy_block(self._pdesc, src, dst, N.stream_ptr(self.device)),
                 "copy_block", IndexError)
+        if self._indexes:
+            self._reindex_blocks(torch.full((1,), dst, dtype=torch.int32, device=self.device))
 
     def copy_blocks(self, src: Sequence[int] | torch.Tensor, dst: Sequence[int] | torch.Tensor) -> None:
         """Batched ``copy_block``: all pairs, all layers, one launch. The
@@ -195,6 +198,8 @@ class B200PagedBackend:
         N.check(self._lib.pkv_copy_blocks(self._pdesc, s.data_ptr(), d.data_ptr(), s.numel(),
                                           self._status.data_ptr(), N.stream_ptr(self.device)),
                 "copy_blocks")
+        if self._indexes:
+            self._reindex_blocks(d)
 
     def append_kv(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, meta: Any) -> None:
         """Scatter this step's K/V into the pool at ``meta.slot_mapping``
@@ -205,6 +210,8 @@ class B200PagedBackend:
         N.check(self._lib.pkv_append_kv(self._pdesc, layer_idx, k.data_ptr(), v.data_ptr(),
                                         slots.data_ptr(), tokens, self._status_ptr,
                                         N.raw_stream(self._dev_index)), "append_kv")
+        if self._indexes:
+            self._reindex_step(layer_idx, slots)
 
     def append_attend(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor,
                       scale: float, meta: Any, *, out: torch.Tensor | None = None,
@@ -241,6 +248,8 @@ class B200PagedBackend:
             self._pdesc, layer_idx, self.n_heads, k.data_ptr(), v.data_ptr(), slots.data_ptr(), q.data_ptr(),
             out.data_ptr(), float(scale), st["batch_ref"], st["hint"], st["ws_ptr"], st["ws_bytes"],
             N.raw_stream(self._dev_index)), "append_attend")
+        if self._indexes:
+            self._reindex_step(layer_idx, slots)
         return out
 
     def _append_attend_rope(self, layer_idx, k, v, q, scale, meta, out, rope) -> torch.Tensor:
@@ -269,6 +278,8 @@ class B200PagedBackend:
         N.check(rc, "append_attend")
         self.n_runs += 1
         self.last_kernel = st["kernel"]
+        if self._indexes:
+            self._reindex_step(layer_idx, slots)
         return out
 
     def rope(self, q: torch.Tensor | None, k: torch.Tensor | None, meta: Any,
@@ -318,8 +329,9 @@ class B200PagedBackend:
         device, ``rotary_dim <= head_dim``; the dims after rotary_dim pass
         through. Pair (i, i + rotary_dim // 2) is turned, or (2i, 2i + 1) when
         ``interleaved``. Same bits as ``rope`` followed by ``append_kv``.
-        ``index`` (a ``PageIndex`` of this backend): the entries of the pages
-        this step completes are written too. fp16, bf16 or fp32 pools."""
+        The entries of the pages this step completes are written too, in
+        ``index`` (a ``PageIndex`` of this backend) by the same call and in the
+        backend's other indexes after it. fp16, bf16 or fp32 pools."""
         # the checks of every call in their cheapest form; the tables' refusal is worded by a helper
         dev, D, Hk = self._dev_index, self.head_dim, self.n_kv_heads
         try:
@@ -387,7 +399,24 @@ class B200PagedBackend:
             None if index is None else index._pdesc, self._status_ptr, N.raw_stream(self._dev_index))
         if rc:
             N.check(rc, "rope_append")
+        if self._indexes:
+            self._reindex_step(layer_idx, slots, index)
         return q_out
+
+    def _reindex_step(self, layer_idx: int, slots: torch.Tensor, done: Any = None) -> None:
+        """The pages whose last slot is among ``slots`` (int32, on this device),
+        in every index of this pool but ``done``."""
+        for ref in self._indexes:
+            index = ref()
+            if index is not None and index is not done:
+                index._write(layer_idx, slots)
+
+    def _reindex_blocks(self, ids: torch.Tensor) -> None:
+        """Whole blocks (ids int32, on this device), every layer, in every index of this pool."""
+        for ref in self._indexes:
+            index = ref()
+            if index is not None:
+                index._write(-1, ids)
 
     def _refuse_rope_tables(self, rope):
         try:
@@ -873,8 +902,12 @@ class B200PagedBackend:
             raise ValueError(f"layer_idx {layer_idx} out of range [0, {self.num_layers})")
 
     def reset(self) -> None:
-        """Zero every pool and drop the cached step state. Tests only."""
+        """Zero every pool and its indexes and drop the cached step state. Tests only."""
         self._pool.zero_()
+        for ref in self._indexes:
+            if (index := ref()) is not None:
+                index.codes.zero_()
+                index.scales.zero_()
         self.invalidate_plan()
 
     def __repr__(self) -> str:

@@ -9,8 +9,12 @@ scale and scores above every number; infinite bounds have an infinite scale and
 the codes -127 / 127. An entry belongs to the physical block, so
 sequences that share a page (radix prefix sharing) share its entry. Only entries
 of completed pages are read (a query's own page is always attended), so nothing
-is kept up to date token by token: ``rope_append(..., index=)`` or ``update``
-write the entries of the pages a step completes.
+is kept up to date token by token: the backend writes the entries of the pages
+that a step completes, or of the blocks that it fills, after every ``append_kv``,
+``append_attend``, ``rope_append``, ``copy_block(s)`` and swap-in while the index
+lives. ``update`` and ``rebuild`` are for what is written past the backend (into
+``k_pool`` itself, by the C entry points, by a CUDA graph captured before the
+index was made) or before it existed.
 
 The reference has no counterpart (its attention reads every page).
 """
@@ -18,6 +22,7 @@ The reference has no counterpart (its attention reads every page).
 from __future__ import annotations
 
 import ctypes
+import weakref
 from typing import Any, Iterable
 
 import torch
@@ -44,27 +49,39 @@ class PageIndex:
         self.scales = torch.zeros(shape, dtype=torch.float32, device=backend.device)
         self._desc = N.PageIndexDesc(self.codes.data_ptr(), self.scales.data_ptr())
         self._pdesc = ctypes.byref(self._desc)
+        # the backend's writers keep this index current until it is dropped
+        backend._indexes.append(weakref.ref(self, backend._indexes.remove))
 
     def nbytes(self) -> int:
         return self.codes.numel() + 4 * self.scales.numel()
 
     def update(self, layer_idx: int, meta: Any) -> None:
-        """Entries of the pages completed by the step ``meta`` describes, after
-        its append to layer ``layer_idx`` (``rope_append(..., index=)`` does this
-        itself)."""
+        """Entries of the pages completed by the step ``meta`` describes, once
+        layer ``layer_idx`` holds its keys (the backend's writers do this
+        themselves)."""
         bk = self.backend
         bk._check_layer(layer_idx)
         if getattr(meta, "slot_mapping", None) is None:
             raise ValueError("PageIndex.update requires meta.slot_mapping")
-        slots = bk._i32(meta.slot_mapping)
+        self._write(layer_idx, bk._i32(meta.slot_mapping))
+
+    def _write(self, layer_idx: int, ids: torch.Tensor) -> None:
+        """int32 ids on the device: the slots of a step in one layer, or blocks
+        in every layer (``layer_idx`` -1)."""
+        bk = self.backend
         with torch.cuda.device(bk.device):
-            N.check(bk._lib.pkv_page_index_update(bk._pdesc, self._pdesc, layer_idx, slots.data_ptr(), slots.numel(),
-                                                  bk._status_ptr, N.raw_stream(bk._dev_index)), "PageIndex.update")
+            if layer_idx >= 0:
+                N.check(bk._lib.pkv_page_index_update(bk._pdesc, self._pdesc, layer_idx, ids.data_ptr(), ids.numel(),
+                                                      bk._status_ptr, N.raw_stream(bk._dev_index)), "PageIndex.update")
+            else:
+                N.check(bk._lib.pkv_page_index_rebuild(bk._pdesc, self._pdesc, ids.data_ptr(), ids.numel(),
+                                                       bk._status_ptr, N.raw_stream(bk._dev_index)),
+                        "PageIndex.rebuild")
 
     def rebuild(self, block_ids: Iterable[int] | torch.Tensor) -> None:
-        """Entries of these blocks in every layer, from the pool: after
-        ``copy_block``, a swap-in, or for a pool filled before the index was
-        made. ``IndexError`` for ids outside the pool."""
+        """Entries of these blocks in every layer, from the pool: for blocks
+        filled before the index was made, or past the backend. ``IndexError``
+        for ids outside the pool."""
         bk = self.backend
         ids = torch.as_tensor(list(block_ids) if not isinstance(block_ids, torch.Tensor) else block_ids,
                               dtype=torch.int32).flatten()
@@ -73,7 +90,4 @@ class PageIndex:
         lo, hi = int(ids.min()), int(ids.max())
         if lo < 0 or hi >= bk.num_blocks:
             raise IndexError(f"rebuild: block ids outside [0, {bk.num_blocks})")
-        ids = ids.to(bk.device)
-        with torch.cuda.device(bk.device):
-            N.check(bk._lib.pkv_page_index_rebuild(bk._pdesc, self._pdesc, ids.data_ptr(), ids.numel(),
-                                                   bk._status_ptr, N.raw_stream(bk._dev_index)), "PageIndex.rebuild")
+        self._write(-1, ids.to(bk.device))

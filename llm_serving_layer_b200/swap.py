@@ -198,6 +198,8 @@ class B200SwapSpace:
                 self._sw, self.backend._pdesc, idx.data_ptr(), handle.num_blocks, handle.k.data_ptr(),
                 handle.v.data_ptr(), N.stream_ptr(self.device), self.backend._status.data_ptr(),
                 ctypes.byref(ticket)), "swap_in")
+            if self.backend._indexes:  # the blocks have other keys now; this stream waits for them
+                self.backend._reindex_blocks(idx)
         # the host buffers and ids must outlive the transfer
         self._pending.append((ticket.value, [idx, handle.k, handle.v]))
         if self.synchronous:

@@ -274,3 +274,85 @@ def test_queries_that_are_not_finite_choose_the_lowest_pages(dtype, page, hq, d,
     after = bk.select_pages(q, 0, plan)
     assert after[0, 0].tolist() == [0, 1, 2, 3, 4, 58, 59]
     assert torch.equal(after[0, 1], before[0, 1]) and torch.equal(after[1], before[1])
+
+
+class _Blocks:
+    is_freed, seq_id = False, 0
+
+    def __init__(self, ids, tokens):
+        self.block_ids, self.num_tokens = ids, tokens
+
+
+def _index_is_the_pools(bk, index, blocks):
+    fresh = PageIndex(bk)
+    fresh.rebuild(blocks)
+    assert torch.equal(fresh.codes[:, blocks], index.codes[:, blocks])
+    assert torch.equal(fresh.scales[:, blocks], index.scales[:, blocks])
+
+
+@pytest.mark.parametrize("writer", ["append_kv", "append_attend decode", "append_attend prompt", "append_attend rope",
+                                    "rope_append", "rope_append with another index", "copy_block", "copy_blocks",
+                                    "swap_in", "reset"])
+def test_every_writer_keeps_the_index(writer):
+    """Blocks taken over from a former owner: their entries are the new keys', whoever wrote them."""
+    from llm_serving_layer_b200 import B200SwapSpace
+    P, hkv, hq, d, layers = 16, 2, 8, 64, 2
+    bk = B200PagedBackend(layers, 12, P, hkv, hq, d, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(11)
+    def fill():
+        for pool in bk.k_pool + bk.v_pool:
+            pool.copy_(torch.randn(pool.shape, generator=g, device=DEV))
+    fill()
+    index = PageIndex(bk)
+    index.rebuild(range(12))
+    old = index.codes.clone()
+    tables, done = [[7, 2, 9], [4, 11]], [7, 2, 4, 11]
+    def step(kv, new):
+        m = build_meta(tables, kv, new, P, device=DEV)
+        x = [torch.randn(sum(new), h, d, generator=g, device=DEV).half() for h in (hq, hkv, hkv)]
+        return m, *x
+    rope = (torch.randn(64, d // 2, device=DEV, generator=g), torch.randn(64, d // 2, device=DEV, generator=g))
+    if writer.startswith("copy") or writer in ("swap_in", "reset"):
+        if writer == "copy_block":
+            for a, b in ((0, 7), (1, 2), (3, 4), (5, 11)):
+                bk.copy_block(a, b)
+        elif writer == "copy_blocks":
+            bk.copy_blocks([0, 1, 3, 5], done)
+        elif writer == "swap_in":
+            space = B200SwapSpace(bk, synchronous=False)
+            handle = space.swap_out("r", _Blocks([0, 1, 3, 5], 64))
+            space.swap_in(handle, _Blocks(done, 64))
+            space.wait()
+        else:
+            bk.reset()
+            done = list(range(12))
+    elif writer == "append_attend decode":
+        m, q, k, v = step([35, 31], [35, 31])
+        bk.append_kv(0, k, v, m)
+        bk.append_kv(1, k, v, m)
+        m, q, k, v = step([36, 32], [1, 1])
+        for l in range(layers):
+            bk.append_attend(l, k, v, q, 0.125, m)
+    else:
+        m, q, k, v = step([40, 32], [40, 32])
+        other = PageIndex(bk) if writer == "rope_append with another index" else None
+        for l in range(layers):
+            if writer == "append_kv":
+                bk.append_kv(l, k, v, m)
+            elif writer == "append_attend prompt":
+                bk.append_attend(l, k, v, q, 0.125, m)
+            elif writer == "append_attend rope":
+                bk.append_attend(l, k, v, q, 0.125, m, rope=rope)
+            else:
+                bk.rope_append(l, q, k, v, m, rope, index=other)
+    bk.check_status()
+    assert not torch.equal(index.codes[:, done], old[:, done])
+    _index_is_the_pools(bk, index, done)
+
+
+def test_an_index_that_is_gone_costs_nothing():
+    bk = B200PagedBackend(1, 4, 16, 2, 2, 64, device=DEV)
+    index = PageIndex(bk)
+    assert len(bk._indexes) == 1
+    del index
+    assert not bk._indexes
