@@ -356,3 +356,67 @@ def test_an_index_that_is_gone_costs_nothing():
     assert len(bk._indexes) == 1
     del index
     assert not bk._indexes
+
+
+# ---------------------------------------------------------------- pools beyond 4 GiB
+def test_offsets_past_32_bits():
+    """A K slab of more than 2^32 bytes: append, index and page-sparse attention at its end."""
+    import test_gpu_rope_append as ra
+    hkv, hq, d, P = 8, 8, 128, 16
+    blocks = (1 << 32) // (P * hkv * d * 2) + 24
+    bk = B200PagedBackend(1, blocks, P, hkv, hq, d, device=DEV, validate="device")
+    ids = [blocks - 1 - i for i in range(20)]
+    kv = P * 20 - 3
+    meta = build_meta([ids], [kv], [kv], P, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, v = (torch.randn(kv, h, d, generator=g, device=DEV).half() for h in (hq, hkv, hkv))
+    index, rope = PageIndex(bk), ra.tables(512, d)
+    q = bk.rope_append(0, q, k, v, meta, rope, index=index)
+    slots = meta.slot_mapping.long()
+    kp, vp = bk.k_pool[0].flatten(0, 1), bk.v_pool[0].flatten(0, 1)
+    ra.check_rotation(kp[slots], k, meta.positions, rope, False)
+    assert torch.equal(vp[slots], v)
+    assert not bk.k_pool[0][:1000].any() and not bk.v_pool[0][:1000].any()
+    codes, scales = ra.entries(bk.k_pool[0][ids[:19]])
+    assert np.array_equal(index.codes[0, ids[:19]].cpu().numpy(), codes)
+    assert np.array_equal(index.scales[0, ids[:19]].cpu().numpy(), scales)
+
+    class S:
+        block_ids = ids
+    last, step = q[-1:].contiguous(), build_meta([ids], [kv], [1], P, device=DEV)
+    out, pages = bk.attend_sparse(last, 0, d ** -0.5, bk.plan_sparse(step, index, 6))
+    bk.check_status()
+    assert pages[0].tolist() == sp.choose(bk, index, [S], step, last, 6, 1, 1)[0]
+    sp.close(out, sp.attend64(bk, [S], step, last, pages.tolist(), d ** -0.5), bk)
+
+
+def test_shared_pages_past_32_bits():
+    """... and shared pages, rests and chunks at its end."""
+    hkv, hq, d, P = 8, 16, 64, 16
+    blocks = (1 << 32) // (P * hkv * d * 2) + 40
+    bk = B200PagedBackend(1, blocks, P, hkv, hq, d, device=DEV, validate="device")
+    ids = [blocks - 1 - i for i in range(30)]
+    tables = [ids[:9] + ids[9:12], ids[:9] + ids[12:20], ids[20:28]]
+    kv, ql = [9 * P + 40, 9 * P + 120, 100], [1, 7, 1]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for pool in (bk.k_pool[0], bk.v_pool[0]):
+        pool[ids] = torch.randn(30, P, hkv, d, generator=g, device=DEV).half()
+    meta = build_meta(tables, kv, ql, P, device=DEV)
+    q = torch.randn(9, hq, d, generator=g, device=DEV).half()
+    out = bk.attend_shared(q, 0, 0.125, bk.plan_shared(meta, SharedPrefix([2, 1], [9, 0])))
+    bk.check_status()
+    want = sh.attend64(bk, meta, q, tables, 0.125)
+    top = float(bk.v_pool[0][ids].abs().max())
+    assert float((out.double() - want).abs().max()) <= (2 * 2.0 ** -11 + 2.0 ** -18) * top
+
+
+@pytest.mark.parametrize("new", [300, 700])
+def test_prompt_chunks_over_listed_pages(new):
+    """Page-sparse attention of hundreds of new tokens of one sequence beside a decode row."""
+    bk, index, seqs, meta, q = sp.build([(900, new), (400, 1)], 16, 4, 2, 64)
+    plan = bk.plan_sparse(meta, index, 9, sink=1, recent=3)
+    out, pages = bk.attend_sparse(q, 0, 0.125, plan)
+    bk.check_status()
+    want = sp.choose(bk, index, seqs, meta, q, 9, 1, 3)
+    assert np.array_equal(pages.cpu().numpy(), np.array([[r + [-1] * (9 - len(r)) for r in row] for row in want]))
+    sp.close(out, sp.attend64(bk, seqs, meta, q, want, 0.125), bk)
