@@ -122,7 +122,6 @@ __global__ void __launch_bounds__(NG == 1 ? TC_THREADS : 384, NG == 1 ? 2 : 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile_idx = int(blockIdx.x) / a.n_kv, h = int(blockIdx.x) % a.n_kv;
-  pdl_trigger();
   // A CTA of the first wave may start while the kernel before it (this
   // layer's append, the previous layer's attention) still runs: up to
   // pdl_wait() it reads only the plan's tile list and the step's BatchMeta,
@@ -236,6 +235,9 @@ __global__ void __launch_bounds__(NG == 1 ? TC_THREADS : 384, NG == 1 ? 2 : 1)
                  "r"(TC_TMEM_COLS * NG)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // after the allocation: the next kernel may allocate ahead of its wait for this
+    // one, and columns that it held would be waited for here for good
+    pdl_trigger();
   }
   tc_fence_before();
   __syncthreads();
@@ -599,7 +601,6 @@ __global__ void __launch_bounds__(TC_THREADS, 2) prefill_tc_persistent_kernel(
   __shared__ int s_pg_bad[2];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
   // The plan kernel (tile list) completed before this kernel could start and
   // fenced its stores: the item count may be read before griddepcontrol.wait.
   const int n_items = __ldcg(a.n_tiles) * a.n_kv;
@@ -643,6 +644,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) prefill_tc_persistent_kernel(
                  "r"(TC_TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    pdl_trigger();  // after the allocation, as above
   }
   tc_fence_before();
   __syncthreads();
@@ -997,11 +999,11 @@ __global__ void __launch_bounds__(TC_THREADS, TL_MINB) prefill_tc_lean_kernel(
   __shared__ TlItem s_item[2];        // the items, in the order every role walks them
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
   // The plan kernel (tile list) completed before this kernel could start and
   // fenced its stores: the item count may be read before griddepcontrol.wait.
   const int n_items = __ldcg(a.n_tiles) * a.n_kv;
   if (int(blockIdx.x) >= n_items) {  // no item for this CTA (uniform over the CTA)
+    pdl_trigger();
     pdl_wait();                      // the counters belong to the previous launch until it completed
     if (threadIdx.x == 0) tl_count_exit(a.claim);
     return;
@@ -1048,6 +1050,7 @@ __global__ void __launch_bounds__(TC_THREADS, TL_MINB) prefill_tc_lean_kernel(
                  "r"(TL_TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    pdl_trigger();  // after the allocation, as above
   }
   tc_fence_before();
   __syncthreads();

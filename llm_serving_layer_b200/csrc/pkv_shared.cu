@@ -726,7 +726,9 @@ __global__ void __launch_bounds__(TC_THREADS, SH_MINB) shared_kernel(
   // ---- tensor memory: 128 columns S | O, freed on every path below. Allocated
   // first thing by every CTA, streaming ones too: the next CTA of the launch
   // starts on an SM only once the one before has given up its allocation permit
-  // (measured: a CTA that kept it held the SM at two CTAs until it ended).
+  // (measured: a CTA that kept it held the SM at two CTAs until it ended). It is
+  // held while the kernels before this one end, and they need none of it: each
+  // kernel that allocates lets its successor start only after it has.
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(SH_TMEM_COLS)

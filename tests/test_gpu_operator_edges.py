@@ -420,3 +420,26 @@ def test_prompt_chunks_over_listed_pages(new):
     want = sp.choose(bk, index, seqs, meta, q, 9, 1, 3)
     assert np.array_equal(pages.cpu().numpy(), np.array([[r + [-1] * (9 - len(r)) for r in row] for row in want]))
     sp.close(out, sp.attend64(bk, seqs, meta, q, want, 0.125), bk)
+
+
+@pytest.mark.parametrize("new", [40, 700])
+def test_tensor_memory_through_a_chain_of_launches(new):
+    """Prompt attention and shared-prefix attention one after the other behind a kernel of some milliseconds, none
+    of them with a pause: each holds tensor memory of its own."""
+    bk, meta, q, shared, tables = sh.build([(21, [(4 + i % 37, 1 + i % 3) for i in range(40)]), (0, [(new, new)] * 6)],
+                                           validate="device")
+    plan = bk.plan_shared(meta, shared)
+    slow = B200PagedBackend(1, 1, 1024, 1, 1, 64, device=DEV, dtype=torch.float32, validate="device")
+    one = build_meta([[0]], [1024], [1], 1024, device=DEV)
+    splan = slow.plan_sparse(one, PageIndex(slow), 100, max_pages=1)
+    x, pages = torch.ones(1, 1, 64, device=DEV), torch.zeros((1, 1, 100), dtype=torch.int32, device=DEV)
+    bk.plan(meta)
+    want_a, want_s = bk.attend(q, 0, 0.125, meta), bk.attend_shared(q, 0, 0.125, plan)
+    outs = [torch.empty_like(q) for _ in range(6)]
+    torch.cuda.synchronize()
+    slow.attend_pages(x, 0, 0.1, splan, pages)
+    for i in range(0, 6, 2):
+        bk.attend(q, 0, 0.125, meta, out=outs[i])
+        bk.attend_shared(q, 0, 0.125, plan, out=outs[i + 1])
+    bk.check_status()
+    assert all(torch.equal(o, want_a) for o in outs[0::2]) and all(torch.equal(o, want_s) for o in outs[1::2])
