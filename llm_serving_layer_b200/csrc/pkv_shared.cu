@@ -88,8 +88,6 @@ struct ShCtl {
   int n_stream;    // CTAs that stream first
   int n_ranges;    // ranges the listed pages are cut into (one warp per range and KV head)
   int listed;      // pages listed
-  int chunk;       // blocks per range of a tile item
-  int n_ents, n_shared;
 };
 
 struct ShLayout {
@@ -243,7 +241,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   }
   // share = 1: as the groups say. Should even one piece per row and range not
   // fit the workspace, a second round (share = 0) computes every sequence by itself.
-  int n_ents = 0, n_shared = 0, chunk = 1, n_lo = 0;
+  int n_ents = 0, chunk = 1, n_lo = 0;
   for (int share = 1; share >= 0; --share) {
     if (tid == 0) {
       s_maxblk = 1;
@@ -286,7 +284,6 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
       if (is) a.ents[i] = x;
       n_ents += tot;
     }
-    n_shared = n_ents;
     for (int c0 = 0; c0 < a.n_seqs; c0 += blockDim.x) {
       const int s = c0 + tid;
       ShEnt x{};
@@ -482,9 +479,6 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     if (!room) flag(a.st, PKV_DEV_WORKSPACE);
     if (over) flag(a.st, PKV_DEV_META_BAD);
     a.ctl->n_items = n_items;
-    a.ctl->chunk = chunk;
-    a.ctl->n_ents = n_ents;
-    a.ctl->n_shared = n_shared;
     a.ctl->n_stream = n_stream;
     a.ctl->n_ranges = ranges;
     a.ctl->listed = P;
@@ -639,6 +633,7 @@ __device__ __forceinline__ void stream_range(const ShArgs& a, unsigned char* rin
     const float p10 = ex2(s[2] - m0), p11 = ex2(s[3] - m1);
     l0 += p00 + p10;
     l1 += p01 + p11;
+    // P in the pool dtype, the product's operand type (see tl_exp64_smem)
     const uint32_t pb0 = movmatrix_t(MmaOp<T>::pack(p00, p01)), pb1 = movmatrix_t(MmaOp<T>::pack(p10, p11));
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {

@@ -623,6 +623,9 @@ __global__ void __launch_bounds__(NW * 32, MINB) sparse_kernel(const SparseArgs 
     const float p10 = ex2(s[2] - n0), p11 = ex2(s[3] - n1);
     l0 = l0 * al0 + (p00 + p10);
     l1 = l1 * al1 + (p01 + p11);
+    // P in the pool dtype, the product's operand type: relative 2^-11 (fp16) or 2^-8
+    // (bf16) of weights that sum to 1 is that part of max |v| at most, as the
+    // output's own rounding is; l sums them unrounded
     const uint32_t pb0 = movmatrix_t(MmaOp<T>::pack(p00, p01)), pb1 = movmatrix_t(MmaOp<T>::pack(p10, p11));
 #pragma unroll
     for (int mt = 0; mt < KS; ++mt) {

@@ -167,7 +167,10 @@ static __device__ __noinline__ void tl_rescale_o(uint32_t tO, float alpha) {
 // exp2(s * sc - mu) of a row's 64 scores, packed to pairs of the pool dtype
 // and stored as the row of P in shared memory (16-byte chunk c of row r at
 // r * 128 + ((c ^ (r & 7)) << 4): the 128B swizzle of a K-major operand); the
-// sum of the exponentials is added to `l`.
+// sum of the exponentials, as they were before that rounding, is added to `l`.
+// The rounding is the tensor cores' operand type: relative 2^-11 (fp16) or 2^-8
+// (bf16) of weights that sum to 1 moves an output by that part of max |v| at most,
+// as its own rounding does; a 32-bit P would be a tf32 product at half the rate.
 template <typename T>
 __device__ __forceinline__ void tl_exp64_smem(const uint32_t (&s)[64], unsigned long long sc2,
                                               unsigned long long nmu2, float& l, unsigned char* prow, int r) {
