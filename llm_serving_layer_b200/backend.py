@@ -35,15 +35,15 @@ class SharedPlan:
     used by every layer of the step. Holds the step's tables and a workspace of
     its own (``workspace`` may be passed on to the next step's plan)."""
 
-    __slots__ = ("meta", "n_tokens", "batch", "batch_ref", "tensors", "workspace", "ws_ptr", "ws_bytes")
+    __slots__ = ("backend", "meta", "n_tokens", "batch", "batch_ref", "tensors", "workspace", "ws_ptr", "ws_bytes")
 
 
 class SparsePlan:
     """One step of ``attend_sparse``: made by ``B200PagedBackend.plan_sparse``,
     used by every layer of the step."""
 
-    __slots__ = ("index", "budget", "sink", "recent", "max_pages", "n_tokens", "batch", "batch_ref", "tensors",
-                 "rows_ptr")
+    __slots__ = ("backend", "index", "budget", "sink", "recent", "max_pages", "n_tokens", "batch", "batch_ref",
+                 "tensors", "rows_ptr")
 
 
 class B200PagedBackend:
@@ -588,6 +588,8 @@ class B200PagedBackend:
         Geometries outside the tensor-core kernels' (fp16 / bf16, head_dim 64,
         16-token pages, up to 8 KV heads, 1/2/4/8 query heads per KV head) run
         ``attend`` itself."""
+        if plan.backend is not self:  # its page ids were checked against that pool
+            raise ValueError("the plan belongs to another backend")
         if plan.meta is not None:
             return self.attend(q, layer_idx, scale, plan.meta, out=out)
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
@@ -678,6 +680,8 @@ class B200PagedBackend:
         return self._sparse(q, layer_idx, scale, plan, out, pages, N.SPARSE_ATTEND)[0]
 
     def _sparse(self, q, layer_idx, scale, plan, out, pages, mode):
+        if plan.backend is not self:
+            raise ValueError("the plan belongs to another backend")
         if layer_idx is None or not 0 <= layer_idx < self.num_layers:
             self._check_layer(layer_idx)
         q = self._query(q, plan.n_tokens)
@@ -706,6 +710,7 @@ class B200PagedBackend:
 
     def _plan_batch(self, plan: Any, meta: Any) -> None:
         """The step's device tables and batch descriptor of a plan object."""
+        plan.backend = self
         n = int(meta.query_lens.shape[0])
         if n <= 0:
             raise ValueError("BatchMeta has no sequences")

@@ -443,3 +443,42 @@ def test_tensor_memory_through_a_chain_of_launches(new):
         bk.attend_shared(q, 0, 0.125, plan, out=outs[i + 1])
     bk.check_status()
     assert all(torch.equal(o, want_a) for o in outs[0::2]) and all(torch.equal(o, want_s) for o in outs[1::2])
+
+
+# ---------------------------------------------------------------- plans
+def test_plans_of_another_backend_are_refused():
+    """A plan's page ids were checked against its own backend's pool, which may be larger."""
+    bk, meta, q, shared, _ = sh.build(sh.CASES["one family"], 8, 2)
+    index = PageIndex(bk)
+    plans = bk.plan_shared(meta, shared), bk.plan_sparse(meta, index, 4)
+    other = B200PagedBackend(1, 2, 16, 2, 8, 64, device=DEV)
+    pages = torch.zeros(4, 2, 4, dtype=torch.int32, device=DEV)
+    for call in (lambda: other.attend_shared(q, 0, 0.125, plans[0]), lambda: other.attend_sparse(q, 0, 0.125, plans[1]),
+                 lambda: other.select_pages(q, 0, plans[1]), lambda: other.attend_pages(q, 0, 0.125, plans[1], pages)):
+        with pytest.raises(ValueError, match="another backend"):
+            call()
+    small, meta, q, shared, _ = sh.build([(0, [(100, 1), (70, 5)])], 6, 2, d=32)  # attend's geometry
+    plan = small.plan_shared(meta, shared)
+    with pytest.raises(ValueError, match="another backend"):
+        other.attend_shared(q, 0, 0.125, plan)
+
+
+def test_plans_of_device_built_steps():
+    """Steps assembled on the device into buffers that are used again: a plan holds its own copies."""
+    from llm_serving_layer_b200 import DeviceBlockTables
+    bk, meta, q, shared, tables = sh.build([(4, [(20, 1), (9, 3)]), (0, [(40, 5)])], 8, 2)
+    bt = DeviceBlockTables(8, 16, 16, num_blocks=bk.num_blocks, device=DEV, ring=1)
+    for i, t in enumerate(tables):
+        bt.bind(i, t)
+    index = PageIndex(bk)
+    index.rebuild(sorted({p for t in tables for p in t[:2]}))
+    want = bk.attend_shared(q, 0, 0.125, bk.plan_shared(meta, shared))
+    want_s = bk.attend_sparse(q, 0, 0.125, bk.plan_sparse(meta, index, 3))
+    step = bt.build_batch_meta([0, 1, 2], [1, 3, 5], [84, 73, 40])
+    plan, sparse = bk.plan_shared(step, shared), bk.plan_sparse(step, index, 3)
+    bt.build_batch_meta([2, 0, 1], [1, 1, 1], [12, 30, 25])  # into the same buffers
+    assert torch.equal(bk.attend_shared(q, 0, 0.125, plan), want)
+    got = bk.attend_sparse(q, 0, 0.125, sparse)
+    assert torch.equal(got[0], want_s[0]) and torch.equal(got[1], want_s[1])
+    bk.check_status()
+    bt.check_status()
