@@ -554,7 +554,8 @@ class B200PagedBackend:
             plan.meta = self._plan_meta(plan, meta, seen)
             plan.workspace, plan.ws_ptr, plan.ws_bytes = None, None, 0
             return plan
-        if workspace is None or workspace.numel() < need or workspace.device != self.device:
+        if (workspace is None or workspace.dtype != torch.uint8 or workspace.numel() < need
+                or workspace.device != self.device or not workspace.is_contiguous()):
             workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
         plan.workspace, plan.ws_ptr, plan.ws_bytes = workspace, workspace.data_ptr(), workspace.numel()
         N.check(self._lib.pkv_plan_shared(

@@ -482,3 +482,16 @@ def test_plans_of_device_built_steps():
     assert torch.equal(got[0], want_s[0]) and torch.equal(got[1], want_s[1])
     bk.check_status()
     bt.check_status()
+
+
+def test_workspaces_that_are_not_taken_over():
+    """Too small, of another type or without the memory its shape says: the plan makes its own."""
+    bk, meta, q, shared, tables = sh.build(sh.CASES["one family"], 8, 2)
+    first = bk.plan_shared(meta, shared)
+    n = first.workspace.numel()
+    for ws in (first.workspace[:n - 1], torch.empty(n // 4, dtype=torch.float32, device=DEV),
+               torch.empty(1, dtype=torch.uint8, device=DEV).expand(n), torch.empty(n, dtype=torch.uint8)):
+        plan = bk.plan_shared(meta, shared, workspace=ws)
+        assert plan.workspace is not ws and plan.workspace.numel() == n
+    sh.close(bk.attend_shared(q, 0, 0.125, plan), sh.attend64(bk, meta, q, tables, 0.125), bk)
+    assert bk.plan_shared(meta, shared, workspace=first.workspace).workspace is first.workspace
