@@ -281,10 +281,11 @@ PKV_API int pkv_attend_sparse(const pkv_pool* pool, const pkv_page_index* index,
  * group. prefix_pages[g] * block_size must not exceed any member's
  * kv_len - query_len; page lists that disagree are computed without sharing and
  * set PKV_DEV_META_BAD, as do sequences whose tables are inconsistent: their rows
- * are zeros. The plan is made once per step and reused by every layer with the
- * same batch and workspace (device, 256-byte aligned, of
- * pkv_shared_workspace_size bytes). Two launches per layer. Geometry of the
- * decode kernel only (PKV_ERR_UNSUPPORTED, and a workspace size of 0, otherwise:
+ * are zeros. A batch with more than 16384 new tokens in groups that share (8192
+ * of sequences with several) is computed without sharing. The plan is made once
+ * per step and reused by every layer with the same batch and workspace (device,
+ * 256-byte aligned, of pkv_shared_workspace_size bytes). Two launches per layer.
+ * Geometry of the decode kernel only (PKV_ERR_UNSUPPORTED, and a workspace size of 0, otherwise:
  * use pkv_attend). pkv_check_shared makes the plan's check of the groups alone,
  * for any geometry: PKV_DEV_META_BAD where page lists disagree. */
 PKV_API size_t pkv_shared_workspace_size(const pkv_pool* pool, int32_t n_heads, int32_t n_seqs, int32_t n_tokens,

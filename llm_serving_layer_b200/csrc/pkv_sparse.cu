@@ -21,11 +21,11 @@
 //
 // Bound by HBM once rows are many: 256 sequences of 1.4 to 4.1 k tokens, 64 pages
 // each (2048 rows, fp16, 8 KV heads of 64): 537 MB of keys and values, 47 MB of
-// index; the attention alone 90 us = 6.0 TB/s (0.92 of the copy rate), with the
-// selection 107 us. Each row's chain (plan row, page ids, index entries,
+// index; the attention alone 92 us = 5.8 TB/s (0.90 of the copy rate), with the
+// selection 108 us. Each row's chain (plan row, page ids, index entries,
 // selection, page reads: about 11000 cycles before the first page is asked for)
 // is hidden by the other CTAs of the SM there, and is the time itself where rows
-// are few: 2048 pages of one sequence 12.7 us, of which the chain is two thirds.
+// are few: 2048 pages of one sequence 12.8 us, of which the chain is two thirds.
 #include <algorithm>
 #include <mutex>
 #include <string>

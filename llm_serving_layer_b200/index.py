@@ -35,7 +35,7 @@ __all__ = ["PageIndex"]
 class PageIndex:
     """Index of every page of ``backend``'s pool: ``codes`` int8
     ``[layers, blocks, kv heads, 2, head_dim]`` and ``scales`` fp32
-    ``[layers, blocks, kv heads]`` on its device (1/16 of the pool's bytes for
+    ``[layers, blocks, kv heads]`` on its device (1/31 of the pool's bytes for
     16-token fp16 pages). Fresh entries are zero."""
 
     def __init__(self, backend: Any):
